@@ -372,6 +372,120 @@ int qgql_quantize_device(int32_t bits, int32_t out_features, int32_t in_features
                          const float *w_dev, uint8_t *q_dev, float *scale_f32_dev,
                          uint16_t *scale_f16_dev, void *stream);
 
+/* ---- tokens in expert order ------------------------------------------------
+ * The steps around the experts' products as calls of their own, for callers
+ * that run the experts themselves (on qgq8_* below, on their own kernels, or
+ * for training): the pairs (token, rank) that a router selected, sorted by
+ * expert, the token rows gathered in that order, and the expert rows weighted
+ * and summed back per token (model/moe.go:82-85).  T tokens, k selected
+ * experts each, pair p = t * k + j.  All pointers are DEVICE pointers on the
+ * calling thread's current device; the work is enqueued on `stream` (NULL =
+ * legacy default stream) and the call returns.  No call allocates, keeps
+ * anything between calls or uses a workspace: calls on different streams
+ * overlap freely and every call can be captured into a CUDA graph.
+ * Rows are QGMOE_DT_F32, _F16 or _BF16, contiguous, of 1..QGMOE_MAX_ROW
+ * elements (16-byte aligned rows, multiples of 8 elements, are read and
+ * written 16 bytes at a time); arithmetic is float32, rounded once to the
+ * output's type.  T * k is at most QGMOE_MAX_PAIRS; T = 0 is allowed.
+ * Outputs may not overlap inputs. */
+#define QGMOE_MAX_PAIRS (1 << 30)
+#define QGMOE_MAX_ROW (1 << 24)
+
+/* sel_idx [T, k] int32 -> offsets [E + 1] (first row of each expert, then the
+ * number of pairs that have one), pair_row [T, k] (the pair's row) and, unless
+ * NULL, row_pair [T * k] (the row's pair).  Rows of an expert are in the
+ * order of their pairs.  A sel_idx outside [0, E) -- padding tokens, experts
+ * of another rank -- has no row: pair_row is -1, and the last rows, which no
+ * pair owns, have row_pair -1.  The same expert twice in a token is two
+ * pairs.  E <= 1024. */
+int qgmoe_sort_tokens(const int32_t *sel_idx, int32_t T, int32_t k, int32_t E, int32_t *offsets,
+                      int32_t *pair_row, int32_t *row_pair, void *stream);
+
+/* rows[pair_row[t, j]] = x[t]: x [T, H] -> rows [T * k, H].  Rows that no pair
+ * owns are left as they are; a pair_row outside [0, T * k) counts as a pair
+ * without a row, here and below. */
+int qgmoe_gather_rows(const void *x, int32_t x_dtype, int32_t T, int32_t k, int32_t H,
+                      const int32_t *pair_row, void *rows, int32_t rows_dtype, void *stream);
+/* Its gradient: grad_x[t] = sum_j grad_rows[pair_row[t, j]], in rank order. */
+int qgmoe_gather_rows_backward(const void *grad_rows, int32_t rows_dtype, int32_t T, int32_t k,
+                               int32_t H, const int32_t *pair_row, void *grad_x, int32_t x_dtype,
+                               void *stream);
+
+/* out[t] = sum_j w[t, j] * rows[pair_row[t, j]], in rank order over the pairs
+ * that have a row (zeros for a token without one; such a pair's weight is not
+ * used): rows [T * k, H], w [T, k] f32 -> out [T, H]. */
+int qgmoe_combine_rows(const void *rows, int32_t rows_dtype, const float *w, int32_t T, int32_t k,
+                       int32_t H, const int32_t *pair_row, void *out, int32_t out_dtype,
+                       void *stream);
+/* Its gradients: grad_rows[pair_row[p]] = w[p] * grad_out[t] (of rows' type;
+ * rows that no pair owns are left as they are) and grad_w[p] =
+ * <rows[pair_row[p]], grad_out[t]> (0 for a pair without a row).  grad_rows
+ * or grad_w may be NULL; then w, or rows, is not read and may be NULL too. */
+int qgmoe_combine_rows_backward(const void *grad_out, int32_t out_dtype, const void *rows,
+                                int32_t rows_dtype, const float *w, int32_t T, int32_t k,
+                                int32_t H, const int32_t *pair_row, void *grad_rows,
+                                float *grad_w, void *stream);
+
+/* ---- 8-bit integer products ---------------------------------------------------
+ * y[r, o] = (sum_i c[r, i] * q[o, i]) * scale[o] * s[r]: int8 codes and a
+ * scale for each row (token) times int8 weights and a scale for each output
+ * channel, on the tensor cores' integer path (the group-32 QuantLinear below
+ * dequantises to floating point instead).  The integer sum is exact; the
+ * products with the scales are float32, rounded once to y's type.
+ * No reference counterpart: qwen-go's quantised linears keep float
+ * activations.  Both operands' codes follow the rounding of its quantisers
+ * (model/moe.go:165-188) with a whole row as the group. */
+
+/* Codes and scales of rows: scale = max(max|x| / 127, 1e-8), code =
+ * clamp(round(x / scale), -127, 127), halves away from zero; a row that holds
+ * an infinity or NaN gets scale NaN and codes 0, so that its products are
+ * NaN.  x [T, K] (QGMOE_DT_F32 / F16 / BF16).  pair_row NULL (k = 1): codes
+ * [T, K] with row pitch ld, scale [T].  With pair_row [T, k]
+ * (qgmoe_sort_tokens): row t goes to the rows pair_row[t, 0..k) of codes
+ * [T * k, K] and scale [T * k] -- gathered and quantised in one pass; other
+ * rows are left as they are.  ld is a multiple of 16, codes 16-byte aligned;
+ * bytes of a row between K and ld are undefined.  The same call makes the
+ * weights' codes from float rows.  DEVICE pointers on the current device;
+ * stream and capture rules as for qgmoe_gather_rows. */
+int qgq8_quantize_rows(const void *x, int32_t x_dtype, int32_t T, int32_t k, int32_t K,
+                       const int32_t *pair_row, int8_t *codes, int64_t ld, float *scale,
+                       void *stream);
+
+typedef struct qgq8 qgq8_t;
+/* Weights: `groups` matrices (1 = a linear layer; the experts of a layer
+ * otherwise) q [groups, out, in] int8 and scale [groups, out] f32, copied in
+ * tile order (host pointers, or device pointers with weights_on_device; the
+ * call blocks and, for the latter, waits for the whole device).  swiglu: the
+ * rows of a group are gate rows, then as many up rows (the layout of
+ * gate_up above), and y = silu(gate) * up with out / 2 columns, applied in
+ * float32 before the rounding to y's type.  groups <= 1024, in <= 131071. */
+int qgq8_create(int32_t groups, int32_t out_features, int32_t in_features, const int8_t *q,
+                const float *scale, int32_t swiglu, int32_t weights_on_device, int32_t device,
+                qgq8_t **out);
+int qgq8_destroy(qgq8_t *h);
+/* codes [R, in] (pitch ld) and scale [R] -> y [R, out] (out / 2 with swiglu),
+ * contiguous, QGMOE_DT_F32 / F16 / BF16.  offsets: device int32 [groups + 1],
+ * the rows of group g are offsets[g] .. offsets[g + 1]; rows outside every
+ * group are left as they are.  A group whose range is not inside [0, R] is
+ * skipped and raises the error flag (qgq8_sync).  NULL with one group: all
+ * R rows.  DEVICE pointers; enqueued on `stream` (NULL = the handle's
+ * stream, cudaStreamLegacy = the legacy default stream).  Nothing is kept between calls: calls of one handle may overlap on
+ * the GPU and be captured into graphs.  The caller's current device is left
+ * as it was. */
+int qgq8_matmul_device(qgq8_t *h, const int8_t *codes, int64_t ld, const float *scale, int32_t R,
+                       const int32_t *offsets, void *y, int32_t y_dtype, void *stream);
+/* qgq8_quantize_rows into the caller's codes / scale (R = T * k rows), then
+ * qgq8_matmul_device on them, in one call. */
+int qgq8_forward_device(qgq8_t *h, const void *x, int32_t x_dtype, int32_t T, int32_t k,
+                        const int32_t *pair_row, const int32_t *offsets, int8_t *codes, int64_t ld,
+                        float *scale, void *y, int32_t y_dtype, void *stream);
+/* One group, HOST pointers, blocking: x [T, in] f32 -> y f32. */
+int qgq8_forward(qgq8_t *h, const float *x, int32_t T, float *y);
+/* Waits for `stream` (NULL = the handle's stream) and reports any device
+ * flag raised since the last check: QGMOE_ERR_DEVICE_FLAG for bad offsets,
+ * QGMOE_ERR_TIMEOUT for a wait that ran out. */
+int qgq8_sync(qgq8_t *h, void *stream);
+
 /* ---- utilities -------------------------------------------------------------- */
 /* Fills dev[0..n) with stdv * N(0,1) from the counter-based generator
  * (splitmix64 + Box-Muller) keyed by (seed, stream), values offset..offset+n. */

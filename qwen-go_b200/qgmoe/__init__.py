@@ -14,6 +14,8 @@ module exposes the same objects over the C ABI in include/qgmoe.h:
     quantize_int8(w) / quantize_int4(w) -> (codes, scales)  on the GPU
     MoeMLP.from_file(path, prefix, top_k)  a layer from a safetensors file
     LayerFile(path).tensor(name) / .layer_desc(prefix, top_k)   the mapped file
+    sort_tokens / gather_rows / combine_rows and their gradients   (qgmoe.rows)
+    quantize_rows, Int8Linear(qweight, scale)   8-bit integer products (qgmoe.int8)
     qgmoe.checkpoint.save_layer / save_layer_raw, python -m qgmoe.quantize_layer
 
 Every call goes to the CUDA library; there is no CPU fallback.  A failing
@@ -111,6 +113,25 @@ SIGNATURES = {
                         C.c_int),
     "qgmoe_route_static": ([_vp, _vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
                             _vp, _vp, _vp, _vp], C.c_int),
+    "qgmoe_sort_tokens": ([_vp, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, _vp], C.c_int),
+    "qgmoe_gather_rows": ([_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, C.c_int32,
+                           _vp], C.c_int),
+    "qgmoe_gather_rows_backward": ([_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp,
+                                    C.c_int32, _vp], C.c_int),
+    "qgmoe_combine_rows": ([_vp, C.c_int32, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, _vp,
+                            C.c_int32, _vp], C.c_int),
+    "qgmoe_combine_rows_backward": ([_vp, C.c_int32, _vp, C.c_int32, _vp, C.c_int32, C.c_int32,
+                                     C.c_int32, _vp, _vp, _vp, _vp], C.c_int),
+    "qgq8_quantize_rows": ([_vp, C.c_int32, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, C.c_int64,
+                            _vp, _vp], C.c_int),
+    "qgq8_create": ([C.c_int32, C.c_int32, C.c_int32, _vp, _vp, C.c_int32, C.c_int32, C.c_int32,
+                     C.POINTER(_vp)], C.c_int),
+    "qgq8_destroy": ([_vp], C.c_int),
+    "qgq8_matmul_device": ([_vp, _vp, C.c_int64, _vp, C.c_int32, _vp, _vp, C.c_int32, _vp], C.c_int),
+    "qgq8_forward_device": ([_vp, _vp, C.c_int32, C.c_int32, C.c_int32, _vp, _vp, _vp, C.c_int64,
+                             _vp, _vp, C.c_int32, _vp], C.c_int),
+    "qgq8_forward": ([_vp, _vp, C.c_int32, _vp], C.c_int),
+    "qgq8_sync": ([_vp, _vp], C.c_int),
     "qgmoe_strerror": ([C.c_int], C.c_char_p),
     "qgmoe_last_error": ([], C.c_char_p),
     "qgmoe_device_ok": ([C.c_int32], C.c_int),
@@ -452,3 +473,8 @@ class LayerFile:
         _check(lib().qgmoe_file_layer_desc(self.h, prefix.encode(), top_k, router_mode, device,
                                            C.byref(d)), "qgmoe_file_layer_desc")
         return d
+
+
+from .int8 import Int8Linear, quantize_rows  # noqa: E402
+from .rows import (TokenOrder, combine_rows, combine_rows_backward, gather_rows,  # noqa: E402
+                   gather_rows_backward, sort_tokens)

@@ -1,0 +1,189 @@
+"""8-bit integer linears: rows quantised per token, weights per output channel.
+
+    codes, scale = quantize_rows(x)                 [T, K] int8, [T] float32
+    lin = Int8Linear(qweight, scale)                one linear, or one per expert
+    y = lin.forward_device(x)                       quantise + product
+    y = lin.forward_device(x, order=order)          tokens -> rows in expert order, by expert
+    y = lin.forward_device(rows, offsets=order.offsets)   rows already in expert order
+    y = lin.matmul_device(codes, scale)             codes in hand
+
+over the C ABI in include/qgmoe.h (qgq8_*).  Tensor, stream and result rules
+are those of qgmoe.rows; the codes and scales that forward_device needs are
+allocated by torch on the stream that the call runs on, so calls may overlap
+and be captured.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import numpy as np
+
+import qgmoe as _q
+
+from .rows import TokenOrder, _call, _cuda, _need, _on, _result, _row_dtype
+
+
+def _pitch(k: int) -> int:
+    return (k + 15) & ~15
+
+
+def _codes(n: int, k: int, device):
+    """[n, pitch] int8 for rows of k codes, and [n] float32 scales."""
+    import torch
+    return (torch.empty((n, _pitch(k)), dtype=torch.int8, device=device),
+            torch.empty(n, dtype=torch.float32, device=device))
+
+
+def quantize_rows(x, order: TokenOrder | None = None, stream=None):
+    """x [T, K] -> (codes [R, K] int8, scale [R] float32): R = T, or with
+    `order` the T * k rows in expert order (rows that no pair owns hold
+    anything).  The codes' row pitch is K rounded up to 16."""
+    dev = _cuda(x, "x")
+    if x.dim() != 2 or x.shape[1] < 1:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected [rows, row length]")
+    _need(x, "x", dev if order is None else order.device)
+    if order is not None and x.shape[0] != order.n_tokens:
+        raise ValueError(f"x: {x.shape[0]} rows, the order has {order.n_tokens} tokens")
+    xd = _row_dtype(x, "x")
+    T, K = x.shape
+    with _on(dev, stream) as s:
+        codes, scale = _codes(T if order is None else order.n_rows, K, dev)
+        _call("qgq8_quantize_rows", x.data_ptr(), xd, T, 1 if order is None else order.top_k, K,
+              None if order is None else order.pair_row.data_ptr(), codes.data_ptr(), _pitch(K),
+              scale.data_ptr(), s)
+    return codes[:, :K], scale
+
+
+class Int8Linear:
+    """y = x W^T in 8-bit integers on one B200.
+
+    qweight int8 [out, in] with scale [out] float32, or stacked
+    [groups, out, in] with [groups, out] for one linear per expert; numpy
+    (host) arrays or CUDA tensors, copied.  swiglu: the out rows are gate rows,
+    then up rows, and y = silu(gate) * up has out // 2 columns."""
+
+    def __init__(self, qweight, scale, swiglu: bool = False, device: int | None = None):
+        shape = tuple(qweight.shape)
+        if len(shape) not in (2, 3) or tuple(scale.shape) != shape[:-1]:
+            raise ValueError(f"qweight {shape}, scale {tuple(scale.shape)}: expected [out, in] and "
+                             "[out], or [groups, out, in] and [groups, out]")
+        if str(qweight.dtype).split(".")[-1] != "int8" or \
+                str(scale.dtype).split(".")[-1] != "float32":
+            raise ValueError(f"qweight {qweight.dtype}, scale {scale.dtype}: expected int8, float32")
+        on_dev = _q._is_dev(qweight)
+        if _q._is_dev(scale) != on_dev:
+            raise ValueError("qweight and scale must be both host arrays or both device tensors")
+        if on_dev:
+            if device is None:
+                device = qweight.device.index
+            if scale.device != qweight.device or qweight.device.index != device:
+                raise ValueError(f"qweight on {qweight.device}, scale on {scale.device}, "
+                                 f"the linear on cuda:{device}")
+            if not (qweight.is_contiguous() and scale.is_contiguous()):
+                raise ValueError("qweight and scale must be contiguous")
+        else:
+            qweight = np.ascontiguousarray(qweight)
+            scale = np.ascontiguousarray(scale)
+        self.h = None
+        self.device = 0 if device is None else device
+        self.groups = shape[0] if len(shape) == 3 else 1
+        self.in_features = shape[-1]
+        self.out_features = shape[-2] // 2 if swiglu else shape[-2]
+        h = C.c_void_p()
+        _call("qgq8_create", self.groups, shape[-2], shape[-1], _q._ptr(qweight), _q._ptr(scale),
+              int(bool(swiglu)), int(on_dev), self.device, C.byref(h))
+        self.h = h
+
+    def close(self):
+        if getattr(self, "h", None):
+            _q.lib().qgq8_destroy(self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def forward(self, x: np.ndarray) -> np.ndarray:
+        """x [in] or [T, in] float32 from host memory (blocking; one group)."""
+        x = np.ascontiguousarray(x, np.float32)
+        if x.shape[-1] != self.in_features:
+            raise ValueError(f"x: rows of {x.shape[-1]}, expected {self.in_features}")
+        x2 = x.reshape(-1, self.in_features)
+        y = np.empty((x2.shape[0], self.out_features), np.float32)
+        _call("qgq8_forward", self.h, _q._ptr(x2), x2.shape[0], _q._ptr(y))
+        return y.reshape(x.shape[:-1] + (self.out_features,))
+
+    def _offsets(self, offsets, device):
+        import torch
+        if offsets is None:
+            if self.groups != 1:
+                raise ValueError(f"{self.groups} groups: offsets (or order) needed")
+            return None
+        _need(offsets, "offsets", device, (self.groups + 1,), torch.int32)
+        return offsets.data_ptr()
+
+    def forward_device(self, x, y=None, order: TokenOrder | None = None, offsets=None, dtype=None,
+                       stream=None):
+        """Enqueue y = x W^T on device tensors; y of `dtype` (default: x's).
+        One linear: x [T, in] -> y [T, out].  One per expert: x [T, in] with
+        `order` -> y [T * k, out] in expert order, or x [R, in] already in
+        that order with `offsets` -> y [R, out]; rows that no pair owns, or
+        outside the offsets, are left as they are in y."""
+        dev = _cuda(x, "x")
+        if dev.index != self.device:
+            raise ValueError(f"x: on {dev}, the linear is on cuda:{self.device}")
+        if x.dim() != 2 or x.shape[1] != self.in_features or not x.is_contiguous():
+            raise ValueError(f"x: shape {tuple(x.shape)}, expected contiguous "
+                             f"[rows, {self.in_features}]")
+        xd = _row_dtype(x, "x")
+        T, k, pair_row = x.shape[0], 1, None
+        if order is not None:
+            if offsets is not None:
+                raise ValueError("order has its own offsets")
+            if order.n_tokens != T or order.device != dev:
+                raise ValueError(f"x: {T} rows on {dev}, the order has {order.n_tokens} tokens "
+                                 f"on {order.device}")
+            k, pair_row, offsets = order.top_k, order.pair_row.data_ptr(), order.offsets
+        off = self._offsets(offsets, dev)
+        with _on(dev, stream) as s:
+            y = _result(y, "y", x, (T * k, self.out_features), dtype)
+            codes, scale = _codes(T * k, self.in_features, dev)
+            _call("qgq8_forward_device", self.h, x.data_ptr(), xd, T, k, pair_row, off,
+                  codes.data_ptr(), codes.stride(0) if T else _pitch(self.in_features),
+                  scale.data_ptr(), y.data_ptr(), _row_dtype(y, "y"), s)
+        return y
+
+    def matmul_device(self, codes, scale, y=None, offsets=None, dtype=None, stream=None):
+        """Enqueue the product of codes [R, in] int8 (row pitch a multiple of
+        16, as quantize_rows gives them) and scale [R] float32; y [R, out] of
+        `dtype` (default float32)."""
+        import torch
+        dev = _cuda(codes, "codes")
+        if dev.index != self.device:
+            raise ValueError(f"codes: on {dev}, the linear is on cuda:{self.device}")
+        if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != self.in_features or \
+                (codes.shape[1] > 1 and codes.stride(1) != 1):
+            raise ValueError(f"codes: {codes.dtype} {tuple(codes.shape)}, expected int8 "
+                             f"[rows, {self.in_features}] with unit stride along a row")
+        R = codes.shape[0]
+        _need(scale, "scale", dev, (R,), torch.float32)
+        ld = codes.stride(0) if R > 1 else _pitch(self.in_features)
+        off = self._offsets(offsets, dev)
+        with _on(dev, stream) as s:
+            y = _result(y, "y", scale, (R, self.out_features), dtype)
+            _call("qgq8_matmul_device", self.h, codes.data_ptr(), ld, scale.data_ptr(), R, off,
+                  y.data_ptr(), _row_dtype(y, "y"), s)
+        return y
+
+    def sync(self, stream=None):
+        """Waits for the stream (None: the device's current one); raises on a
+        device error flag (qgq8_sync)."""
+        with _on(_device(self.device), stream) as s:
+            _call("qgq8_sync", self.h, s)
+
+
+def _device(index: int):
+    import torch
+    return torch.device("cuda", index)

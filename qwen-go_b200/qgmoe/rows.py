@@ -1,0 +1,237 @@
+"""Tokens in expert order: sort, gather, combine and their gradients.
+
+    order = sort_tokens(sel_idx, n_experts)        offsets, pair_row, row_pair
+    rows = gather_rows(x, order)                   token rows in expert order
+    ...                                            the experts, on rows
+    out = combine_rows(rows, weights, order)       weighted, summed back per token
+    grad_rows, grad_weights = combine_rows_backward(grad_out, rows, weights, order)
+    grad_x = gather_rows_backward(grad_rows, order)
+
+over the C ABI in include/qgmoe.h (qgmoe_sort_tokens and the calls after it).
+Tensors are torch CUDA tensors, contiguous, all on one device (which need not
+be the current one).  Work is enqueued on `stream` (a torch stream or a
+cudaStream_t), by default torch's current stream of that device; results are
+allocated there, and with a stream of another than the inputs' the caller
+orders the two and keeps the inputs until the work is done.  A result tensor may be
+given (out=...), for captured graphs and for rows that no pair owns, which
+every call leaves as they are: a result allocated here holds anything there.
+"""
+from __future__ import annotations
+
+import contextlib
+
+import qgmoe as _q
+
+MAX_EXPERTS = 1024
+
+_DT = None
+
+
+def _dtypes():
+    global _DT
+    if _DT is None:
+        import torch
+        _DT = {torch.float32: _q.DT_F32, torch.float16: _q.DT_F16, torch.bfloat16: _q.DT_BF16}
+    return _DT
+
+
+def _row_dtype(t, what: str) -> int:
+    dt = _dtypes().get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
+    return dt
+
+
+def _need(t, what: str, device, shape=None, dtype=None):
+    """A contiguous tensor on `device` of that shape and type."""
+    if not t.is_cuda or t.device != device:
+        raise ValueError(f"{what}: on {t.device}, expected {device}")
+    if not t.is_contiguous():
+        raise ValueError(f"{what}: not contiguous")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
+
+
+def _cuda(t, what: str):
+    if not getattr(t, "is_cuda", False):
+        raise ValueError(f"{what}: a CUDA tensor is needed")
+    return t.device
+
+
+# torch's default stream has handle 0, which the library takes for "the
+# handle's own stream"; this is its other name, cudaStreamLegacy.
+_LEGACY = 1
+
+
+@contextlib.contextmanager
+def _torch_on(device, stream):
+    import torch
+    if isinstance(stream, torch.cuda.Stream):
+        st = stream
+        if st.device != device:
+            raise ValueError(f"stream of {st.device}, expected {device}")
+    elif stream in (0, _LEGACY):
+        st = torch.cuda.default_stream(device)
+    else:
+        st = torch.cuda.ExternalStream(stream, device=device)
+    with torch.cuda.device(device), torch.cuda.stream(st):
+        yield st.cuda_stream or _LEGACY
+
+
+class _Here:
+    """The device is current and no stream was given: nothing to switch."""
+    __slots__ = ("s",)
+
+    def __init__(self, s):
+        self.s = s
+
+    def __enter__(self):
+        return self.s
+
+    def __exit__(self, *exc):
+        return False
+
+
+def _on(device, stream):
+    """Context in which torch allocates for, and the library launches on,
+    `stream` of `device`; gives the stream's handle."""
+    import torch
+    if stream is None:
+        if device.index == torch.cuda.current_device():
+            return _Here(torch.cuda.current_stream().cuda_stream or _LEGACY)
+        return _torch_on(device, torch.cuda.current_stream(device))
+    return _torch_on(device, stream)
+
+
+def _call(name, *args):
+    _q._check(getattr(_q.lib(), name)(*args), name)
+
+
+class TokenOrder:
+    """The pairs (token, rank) of a batch sorted by expert:
+
+      offsets  [n_experts + 1] int32  first row of each expert, then the number of rows that
+                                      a pair owns
+      pair_row [n_tokens, top_k]      row of each pair, -1 without one
+      row_pair [n_tokens * top_k]     pair of each row, -1 without one
+
+    The tensors are allocated once and refilled by sort(), so that a decode
+    loop or a captured graph allocates nothing; what a later sort() fills must
+    not be needed any more by work of another stream."""
+
+    def __init__(self, n_tokens: int, top_k: int, n_experts: int, device=None):
+        import torch
+        if n_tokens < 0 or top_k < 1 or n_tokens * top_k > 1 << 30:
+            raise ValueError(f"bad n_tokens={n_tokens}, top_k={top_k}")
+        if not 1 <= n_experts <= MAX_EXPERTS:
+            raise ValueError(f"n_experts={n_experts} (1..{MAX_EXPERTS})")
+        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else \
+            torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
+        if dev.index is None:
+            dev = torch.device(dev.type, torch.cuda.current_device())
+        self.n_tokens, self.top_k, self.n_experts, self.device = n_tokens, top_k, n_experts, dev
+        self.n_rows = n_tokens * top_k
+        kw = dict(dtype=torch.int32, device=dev)
+        self.offsets = torch.zeros(n_experts + 1, **kw)
+        self.pair_row = torch.full((n_tokens, top_k), -1, **kw)
+        self.row_pair = torch.full((self.n_rows,), -1, **kw)
+
+    def sort(self, sel_idx, stream=None) -> "TokenOrder":
+        """sel_idx [n_tokens, top_k] int32, as a router selects (MoeMLP's
+        sel_idx, qgmoe_route_static); ids outside [0, n_experts) get no row."""
+        import torch
+        _need(sel_idx, "sel_idx", self.device, (self.n_tokens, self.top_k), torch.int32)
+        with _on(self.device, stream) as s:
+            _call("qgmoe_sort_tokens", sel_idx.data_ptr(), self.n_tokens, self.top_k,
+                  self.n_experts, self.offsets.data_ptr(), self.pair_row.data_ptr(),
+                  self.row_pair.data_ptr(), s)
+        return self
+
+
+def sort_tokens(sel_idx, n_experts: int, stream=None) -> TokenOrder:
+    """A new TokenOrder of sel_idx [T, k] int32."""
+    dev = _cuda(sel_idx, "sel_idx")
+    if sel_idx.dim() != 2:
+        raise ValueError(f"sel_idx: shape {tuple(sel_idx.shape)}, expected [tokens, top_k]")
+    with _on(dev, stream) as s:
+        order = TokenOrder(sel_idx.shape[0], sel_idx.shape[1], n_experts, dev)
+        return order.sort(sel_idx, None if stream is None else s)
+
+
+def _rows_of(t, what: str, order: TokenOrder, n: int):
+    _need(t, what, order.device)
+    if t.dim() != 2 or t.shape[0] != n or t.shape[1] < 1:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected [{n}, row length]")
+    return _row_dtype(t, what)
+
+
+def _result(out, what: str, like, shape, dtype):
+    """`out` checked, or a new tensor (call inside _on())."""
+    if out is None:
+        import torch
+        return torch.empty(shape, dtype=like.dtype if dtype is None else dtype, device=like.device)
+    _need(out, what, like.device, shape, dtype)
+    return out
+
+
+def gather_rows(x, order: TokenOrder, out=None, dtype=None, stream=None):
+    """x [T, H] -> rows [T * k, H] in expert order, of `dtype` (default: x's)."""
+    xd = _rows_of(x, "x", order, order.n_tokens)
+    H = x.shape[1]
+    with _on(order.device, stream) as s:
+        out = _result(out, "out", x, (order.n_rows, H), dtype)
+        _call("qgmoe_gather_rows", x.data_ptr(), xd, order.n_tokens, order.top_k, H,
+              order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return out
+
+
+def gather_rows_backward(grad_rows, order: TokenOrder, out=None, dtype=None, stream=None):
+    """The gradient of gather_rows: grad_rows [T * k, H] -> grad_x [T, H]."""
+    gd = _rows_of(grad_rows, "grad_rows", order, order.n_rows)
+    H = grad_rows.shape[1]
+    with _on(order.device, stream) as s:
+        out = _result(out, "out", grad_rows, (order.n_tokens, H), dtype)
+        _call("qgmoe_gather_rows_backward", grad_rows.data_ptr(), gd, order.n_tokens, order.top_k,
+              H, order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return out
+
+
+def _weights(w, order: TokenOrder):
+    import torch
+    _need(w, "weights", order.device, (order.n_tokens, order.top_k), torch.float32)
+
+
+def combine_rows(rows, weights, order: TokenOrder, out=None, dtype=None, stream=None):
+    """rows [T * k, H], weights [T, k] float32 -> out [T, H]: each token's rows
+    weighted and summed in rank order."""
+    rd = _rows_of(rows, "rows", order, order.n_rows)
+    _weights(weights, order)
+    H = rows.shape[1]
+    with _on(order.device, stream) as s:
+        out = _result(out, "out", rows, (order.n_tokens, H), dtype)
+        _call("qgmoe_combine_rows", rows.data_ptr(), rd, weights.data_ptr(), order.n_tokens,
+              order.top_k, H, order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return out
+
+
+def combine_rows_backward(grad_out, rows, weights, order: TokenOrder, grad_rows=None,
+                          grad_weights=None, stream=None):
+    """The gradients of combine_rows: (grad_rows [T * k, H] of rows' type,
+    grad_weights [T, k] float32)."""
+    import torch
+    gd = _rows_of(grad_out, "grad_out", order, order.n_tokens)
+    rd = _rows_of(rows, "rows", order, order.n_rows)
+    _weights(weights, order)
+    H = rows.shape[1]
+    if grad_out.shape[1] != H:
+        raise ValueError(f"grad_out: rows of {grad_out.shape[1]}, expected {H}")
+    with _on(order.device, stream) as s:
+        grad_rows = _result(grad_rows, "grad_rows", rows, (order.n_rows, H), rows.dtype)
+        grad_weights = _result(grad_weights, "grad_weights", weights,
+                               (order.n_tokens, order.top_k), torch.float32)
+        _call("qgmoe_combine_rows_backward", grad_out.data_ptr(), gd, rows.data_ptr(), rd,
+              weights.data_ptr(), order.n_tokens, order.top_k, H, order.pair_row.data_ptr(),
+              grad_rows.data_ptr(), grad_weights.data_ptr(), s)
+    return grad_rows, grad_weights

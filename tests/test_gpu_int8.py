@@ -1,0 +1,430 @@
+"""8-bit integer products (qgq8_*) against plain 64-bit forms.
+
+Codes and scales are equal to the definition's bit for bit: the scale and the
+quotient are float32 divisions, and a 64-bit quotient of float32 values rounds
+to the same float32.  Products: the integer sum is exact, its conversion and
+the two products with the scales are three roundings of u = 2^-24, the output
+type adds half an epsilon.  SwiGLU of gate g and up value v, each within 3u:
+silu's relative condition number is at most 1 + |g|, expf and the fast
+quotient are within 2 ulp (4u) each, the sum 1 + e and the product one
+rounding each: (3(1 + |g|) + 4 + 4 + 1 + 1 + 3)u in all."""
+import ctypes as C
+
+import numpy as np
+import pytest
+
+import qg_oracle as O
+import qgmoe
+from test_gpu_rows import U, dtypes, f64, half, plain_order, rand, routing, torch_
+
+pytestmark = pytest.mark.gpu
+
+
+def plain_quantize(x64):
+    """(codes float64, scale float32) of rows, by the definition."""
+    s = np.maximum((np.abs(x64).max(1) / 127.0).astype(np.float32), np.float32(1e-8))
+    v = (x64 / s.astype(np.float64)[:, None]).astype(np.float32).astype(np.float64)
+    return np.clip(np.copysign(np.floor(np.abs(v) + 0.5), v), -127, 127), s
+
+
+def check_rows(y, c, s, q, ws, swiglu=False, rows=slice(None)):
+    """y (torch) against codes c [R, I], scales s, weights q [O, I], ws [O]."""
+    v = (c.astype(np.float64) @ q.astype(np.float64).T) * s.astype(np.float64)[:, None] * \
+        ws.astype(np.float64)
+    n = 3.0
+    if swiglu:
+        g, u = np.split(v, 2, 1)
+        v = g / (1 + np.exp(-g)) * u
+        n = 16 + 3 * np.abs(g)
+    # float32 results below 2^-126 lose bits: the absolute term
+    small = 2.0 ** -25 if y.dtype == torch_().float16 else 2.0 ** -126
+    tol = 1.01 * (n * U + half(y.dtype)) * np.abs(v) + small
+    err = np.abs(f64(y)[rows] - v)
+    assert np.all(err <= tol), (float((err / tol).max()), np.unravel_index((err / tol).argmax(), err.shape))
+
+
+def weights(shape, seed):
+    rng = np.random.default_rng(seed)
+    q = np.clip(np.round(rng.standard_normal(shape) * 40), -127, 127).astype(np.int8)
+    return q, (rng.random(shape[:-1]) * 1e-3 + 1e-4).astype(np.float32)
+
+
+# ---- quantise -----------------------------------------------------------------
+@pytest.mark.parametrize("T,K", [(1, 1), (3, 5), (7, 16), (5, 100), (9, 768), (4, 1000), (3, 1001),
+                                 (33, 2048), (2, 2056), (3, 4096), (2, 8192), (2, 9000), (2, 20000)])
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+def test_quantize_rows(T, K, dt):
+    x = rand((T, K), dtypes()[dt], T * K)
+    codes, scale = qgmoe.quantize_rows(x)
+    c, s = plain_quantize(f64(x))
+    np.testing.assert_array_equal(scale.cpu().numpy(), s)
+    np.testing.assert_array_equal(codes.cpu().numpy(), c)
+    assert codes.shape == (T, K) and codes.stride(0) % 16 == 0
+
+
+def test_quantize_rows_at_the_edges():
+    """Ties away from zero, zero rows, rows under the scale's floor, the
+    largest values, and rows with an infinity or NaN, whose products are NaN."""
+    t = torch_()
+    x = t.zeros((8, 40))
+    x[0, :6] = t.tensor([127.0, 0.5, -0.5, 1.5, -2.5, 126.5])  # scale 1
+    x[2, 0], x[2, 1] = 1e-10, -1e-7
+    x[3, 0], x[3, 39] = 3.4e38, -3.4e38
+    x[4, 7] = float("inf")
+    x[5, 39] = float("nan")
+    x[6, :2] = t.tensor([-float("inf"), float("nan")])
+    x[7, 3] = 1e-42
+    codes, scale = qgmoe.quantize_rows(x.cuda())
+    c, s = codes.cpu().numpy(), scale.cpu().numpy()
+    assert c[0, :6].tolist() == [127, 1, -1, 2, -3, 127] and s[0] == 1
+    for r in (0, 1, 2, 3, 7):
+        want = plain_quantize(x.double().numpy()[r:r + 1])
+        assert np.array_equal(c[r], want[0][0]) and s[r] == want[1][0]
+    assert s[1] == np.float32(1e-8) and not c[1].any()
+    for r in (4, 5, 6):
+        assert np.isnan(s[r]) and not c[r].any()
+    lin = qgmoe.Int8Linear(*weights((24, 40), 1))
+    y = lin.matmul_device(codes, scale).cpu().numpy()
+    assert np.isnan(y[[4, 5, 6]]).all() and np.isfinite(y[[0, 1, 2, 3, 7]]).all()
+
+
+def test_quantize_rows_unaligned():
+    t = torch_()
+    x = rand((5, 1001), t.float16, 3)[1:]
+    assert x.data_ptr() % 16
+    codes, scale = qgmoe.quantize_rows(x)
+    c, s = plain_quantize(f64(x))
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(scale.cpu().numpy(), s)
+    flat = rand((4 * 64 + 1,), t.float32, 4)
+    x = flat[1:].view(4, 64)
+    codes, scale = qgmoe.quantize_rows(x)
+    c, s = plain_quantize(f64(x))
+    assert np.array_equal(codes.cpu().numpy(), c) and np.array_equal(scale.cpu().numpy(), s)
+
+
+@pytest.mark.parametrize("K", [40, 1001, 2048, 9000])
+def test_quantize_in_expert_order(K):
+    t = torch_()
+    T, k, E = 29, 3, 7
+    idx = routing(T, k, E, K, 0.2)
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), E)
+    x = rand((T, K), t.bfloat16, 2)
+    codes, scale = qgmoe.quantize_rows(x, order)
+    n = int(order.offsets[-1])
+    tok = (order.row_pair[:n] // k).long().cpu().numpy()
+    c, s = plain_quantize(f64(x))
+    assert np.array_equal(codes.cpu().numpy()[:n], c[tok])
+    assert np.array_equal(scale.cpu().numpy()[:n], s[tok])
+
+
+# ---- dense products --------------------------------------------------------------
+@pytest.mark.parametrize("T,K,N", [(1, 1, 1), (3, 37, 5), (1, 2048, 4096), (16, 128, 128),
+                                   (17, 129, 130), (64, 256, 300), (65, 1000, 1500), (300, 512, 640),
+                                   (1000, 2048, 256), (257, 4097, 129)])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+def test_linear(T, K, N, xt, yt):
+    x = rand((T, K), dtypes()[xt], K)
+    q, ws = weights((N, K), N)
+    lin = qgmoe.Int8Linear(q, ws)
+    y = lin.forward_device(x, dtype=dtypes()[yt])
+    assert y.shape == (T, N)
+    check_rows(y, *plain_quantize(f64(x)), q, ws)
+    lin.sync()
+    lin.close()
+
+
+def test_codes_at_the_limits_of_32_bits():
+    """The longest row, every code -128: the sum is 2^14 * 131071 < 2^31."""
+    t = torch_()
+    K = 131071
+    lin = qgmoe.Int8Linear(np.full((3, K), -128, np.int8), np.ones(3, np.float32))
+    codes = t.full((2, K + 1), -128, dtype=t.int8, device="cuda")[:, :K]
+    codes[1] = 127
+    y = lin.matmul_device(codes, t.ones(2, device="cuda")).cpu().numpy()
+    assert np.all(y[0] == np.float32(16384 * K)) and np.all(y[1] == np.float32(-128 * 127 * K))
+
+
+def test_codes_with_a_pitch_and_device_weights():
+    t = torch_()
+    q, ws = weights((70, 100), 3)
+    lin = qgmoe.Int8Linear(t.from_numpy(q).cuda(), t.from_numpy(ws).cuda())
+    buf = t.randint(-128, 128, (9, 160), dtype=t.int8, device="cuda")
+    scale = t.rand(9, device="cuda") + 0.5
+    y = lin.matmul_device(buf[:, :100], scale, dtype=t.float32)
+    check_rows(y, buf[:, :100].cpu().numpy(), scale.cpu().numpy(), q, ws)
+    y1 = lin.matmul_device(buf[4:5, :100], scale[4:5])
+    assert t.equal(y1, y[4:5])
+    out = t.full((9, 70), 3.0, device="cuda", dtype=t.bfloat16)
+    assert lin.matmul_device(buf[:, :100], scale, y=out) is out
+    assert t.equal(out, y.bfloat16())
+
+
+def test_host_forward():
+    q, ws = weights((130, 96), 5)
+    lin = qgmoe.Int8Linear(q, ws)
+    for T in (3, 40, 7):
+        x = O.randn(T, 1, (T, 96))
+        y = lin.forward(x)
+        check_rows(torch_().from_numpy(y), *plain_quantize(x.astype(np.float64)), q, ws)
+    assert lin.forward(x[0]).shape == (130,)
+    assert lin.forward(np.zeros((0, 96), np.float32)).shape == (0, 130)
+    assert np.array_equal(lin.forward(x[0]), lin.forward(x)[0])
+
+
+def test_no_rows():
+    t = torch_()
+    lin = qgmoe.Int8Linear(*weights((8, 16), 1))
+    assert lin.forward_device(t.empty((0, 16), device="cuda")).shape == (0, 8)
+
+
+# ---- products by expert -------------------------------------------------------------
+@pytest.mark.parametrize("T,k,E,K,N,bad", [
+    (1, 1, 1, 64, 64, 0.0), (1, 8, 128, 256, 130, 0.0), (5, 2, 3, 100, 40, 0.3),
+    (64, 8, 128, 128, 96, 0.0), (200, 4, 16, 300, 257, 0.1), (700, 2, 3, 256, 200, 0.5),
+    (50, 3, 1024, 33, 17, 0.0), (40, 2, 6, 64, 64, 1.0)])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_experts(T, k, E, K, N, bad, swiglu):
+    t = torch_()
+    idx = routing(T, min(k, E), E, T, bad)
+    k = idx.shape[1]
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), E)
+    off, _pr, rp = plain_order(idx, E)
+    q, ws = weights((E, 2 * N if swiglu else N, K), E)
+    ws *= 10
+    lin = qgmoe.Int8Linear(q, ws, swiglu=swiglu)
+    x = rand((T, K), t.float32, T)
+    y = t.full((T * k, N), 9.0, device="cuda")
+    assert lin.forward_device(x, y, order=order) is y
+    lin.sync()
+    n = off[-1]
+    assert t.all(y[n:] == 9.0)
+    c, s = plain_quantize(f64(x))
+    tok = rp[:n] // k
+    for e in range(E):
+        r = slice(off[e], off[e + 1])
+        if off[e + 1] > off[e]:
+            check_rows(y, c[tok[r]], s[tok[r]], q[e], ws[e], swiglu, r)
+    # the same rows handed over in expert order already
+    rows = qgmoe.gather_rows(x, order)
+    y2 = t.full((T * k, N), 9.0, device="cuda")
+    lin.forward_device(rows, y2, offsets=order.offsets)
+    assert t.equal(y, y2)
+    for dt in (t.float16, t.bfloat16):
+        yd = t.full((T * k, N), 9.0, device="cuda", dtype=dt)
+        lin.forward_device(x, yd, order=order)
+        assert t.equal(yd, y.to(dt))
+
+
+def test_swiglu_far_from_zero():
+    """Gates from -200 to 200: silu's limits, no NaN."""
+    t = torch_()
+    q = np.zeros((2 * 21, 1), np.int8)
+    q[:21, 0] = np.linspace(-100, 100, 21).astype(np.int8)
+    q[21:, 0] = 100
+    ws = np.full(42, 2.0, np.float32)
+    lin = qgmoe.Int8Linear(q, ws, swiglu=True)
+    codes = t.ones((1, 16), dtype=t.int8, device="cuda")[:, :1]
+    y = lin.matmul_device(codes, t.ones(1, device="cuda"))
+    assert t.isfinite(y).all()
+    check_rows(y, np.ones((1, 1)), np.ones(1, np.float32), q, ws, True)
+
+
+def test_groups_outside_the_rows_are_skipped_and_flagged():
+    """Offsets that no sort gives: out of order, negative, past the rows.  The
+    kernel checks each group's range before it follows it."""
+    t = torch_()
+    G, K, N, R = 5, 64, 32, 20
+    q, ws = weights((G, N, K), 2)
+    lin = qgmoe.Int8Linear(q, ws)
+    codes = t.randint(-127, 128, (R, K), dtype=t.int8, device="cuda")
+    scale = t.ones(R, device="cuda")
+    y = t.full((R, N), 4.0, device="cuda")
+    off = t.tensor([0, 5, 3, 21, 6, 10], dtype=t.int32, device="cuda")
+    lin.matmul_device(codes, scale, y=y, offsets=off)
+    with pytest.raises(qgmoe.QgmoeError) as e:
+        lin.sync()
+    assert e.value.status == qgmoe.ERR_DEVICE_FLAG and "offsets" in str(e.value)
+    lin.sync()  # cleared
+    c, s = codes.cpu().numpy(), scale.cpu().numpy()
+    check_rows(y, c[:5], s[:5], q[0], ws[0], rows=slice(0, 5))
+    check_rows(y, c[6:10], s[6:10], q[4], ws[4], rows=slice(6, 10))
+    assert t.all(y[5:6] == 4.0) and t.all(y[10:] == 4.0)
+    off = t.tensor([-4, 5, 8, 8, 12, 20], dtype=t.int32, device="cuda")
+    lin.matmul_device(codes, scale, y=y, offsets=off)
+    with pytest.raises(qgmoe.QgmoeError):
+        lin.sync()
+    check_rows(y, c[5:8], s[5:8], q[1], ws[1], rows=slice(5, 8))
+
+
+def test_rows_past_2_gb():
+    """Output rows whose offsets pass 2^31 bytes and elements."""
+    t = torch_()
+    T, K, N = 140000, 16, 16384
+    if t.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    q, ws = weights((N, K), 7)
+    lin = qgmoe.Int8Linear(q, ws)
+    x = rand((T, K), t.float32, 1)
+    y = lin.forward_device(x, dtype=t.bfloat16)
+    for lo in (0, 70001, 131071, T - 5):
+        check_rows(y[lo:lo + 5], *plain_quantize(f64(x[lo:lo + 5])), q, ws)
+
+
+# ---- together, streams, graphs -----------------------------------------------------
+@pytest.mark.parametrize("T,E,k,H,I", [(1, 16, 4, 128, 64), (9, 8, 2, 256, 96), (300, 16, 4, 512, 160)])
+def test_layer_of_8_bit_experts(T, E, k, H, I):
+    """Router, order, gate_up with SwiGLU, down, combine as one run, each step
+    against the plain form of what it was given, and the layer against the
+    64-bit layer of the same weights within what quantising the rows costs:
+    a code is at most half a step of amax / 127 off."""
+    t = torch_()
+    rng = np.random.default_rng(T)
+    router = t.from_numpy((rng.standard_normal((E, H)) * 0.2).astype(np.float32)).cuda()
+    gu = t.from_numpy((rng.standard_normal((E * 2 * I, H)) * 0.05).astype(np.float32)).cuda()
+    dn = t.from_numpy((rng.standard_normal((E * H, I)) * 0.05).astype(np.float32)).cuda()
+    # the row quantiser makes the weights' codes and channel scales too
+    (gq, gs), (dq, ds) = qgmoe.quantize_rows(gu), qgmoe.quantize_rows(dn)
+    gate_up = qgmoe.Int8Linear(gq.contiguous().view(E, 2 * I, H), gs.view(E, 2 * I), swiglu=True)
+    down = qgmoe.Int8Linear(dq.contiguous().view(E, H, I), ds.view(E, H))
+    x = rand((T, H), t.float32, T)
+    st = t.cuda.current_stream().cuda_stream
+    sel = t.empty((T, k), dtype=t.int32, device="cuda")
+    w = t.empty((T, k), device="cuda")
+    assert qgmoe.lib().qgmoe_route_static(x.data_ptr(), router.data_ptr(), T, H, E, k, 0,
+                                          sel.data_ptr(), w.data_ptr(), None, st) == 0
+    order = qgmoe.sort_tokens(sel, E)
+    h = gate_up.forward_device(x, order=order)
+    d = down.forward_device(h, offsets=order.offsets)
+    out = qgmoe.combine_rows(d, w, order)
+    gate_up.sync()
+    down.sync()
+
+    off, pr, rp = plain_order(sel.cpu().numpy(), E)
+    tok = rp // k
+    c, s = plain_quantize(f64(x))
+    ch, sh = plain_quantize(f64(h))
+    gq_, gs_ = gq.cpu().numpy().reshape(E, 2 * I, H), gs.cpu().numpy().reshape(E, 2 * I)
+    dq_, ds_ = dq.cpu().numpy().reshape(E, H, I), ds.cpu().numpy().reshape(E, H)
+    x64, w64 = f64(x), f64(w)
+    ref = np.zeros((T, H))
+    slack = np.zeros((T, H))
+    for e in range(E):
+        r = slice(off[e], off[e + 1])
+        if r.start == r.stop:
+            continue
+        check_rows(h, c[tok[r]], s[tok[r]], gq_[e], gs_[e], True, r)
+        check_rows(d, ch[r], sh[r], dq_[e], ds_[e], False, r)
+        # the layer on unquantised rows, and how far quantised rows may take it
+        W = gq_[e].astype(np.float64) * gs_[e][:, None].astype(np.float64)
+        D = dq_[e].astype(np.float64) * ds_[e][:, None].astype(np.float64)
+        v = x64[tok[r]] @ W.T
+        dv = (s[tok[r]].astype(np.float64) / 2)[:, None] * np.abs(W).sum(1)
+        g, u = np.split(v, 2, 1)
+        dg, du = np.split(dv, 2, 1)
+        sil = g / (1 + np.exp(-g))
+        h64 = sil * u
+        # |silu'| <= 1.1
+        dh = 1.1 * dg * (np.abs(u) + du) + np.abs(sil) * du + (sh[r].astype(np.float64) / 2)[:, None]
+        y64, dy = h64 @ D.T, dh @ np.abs(D).T
+        for i, p in enumerate(rp[r]):
+            ref[p // k] += w64.reshape(-1)[p] * y64[i]
+            slack[p // k] += w64.reshape(-1)[p] * dy[i]
+    assert np.all(np.abs(f64(out) - ref) <= 1.001 * slack + 1e-6)
+
+
+def test_two_streams_on_one_handle():
+    t = torch_()
+    q, ws = weights((300, 512), 3)
+    lin = qgmoe.Int8Linear(q, ws)
+    xs = [rand((T, 512), t.float32, T) for T in (40, 700)]
+    want = [lin.forward_device(x) for x in xs]
+    streams = [t.cuda.Stream(), t.cuda.Stream()]
+    for s in streams:
+        s.wait_stream(t.cuda.current_stream())
+    for _ in range(20):
+        got = [lin.forward_device(x, stream=s) for x, s in zip(xs, streams)]
+        for s in streams:
+            s.synchronize()
+        for g, w in zip(got, want):
+            assert t.equal(g, w)
+
+
+def test_two_captured_graphs_of_one_handle():
+    t = torch_()
+    E, T, k, K, N = 8, 24, 2, 200, 72
+    q, ws = weights((E, 2 * N, K), 3)
+    lin = qgmoe.Int8Linear(q, ws, swiglu=True)
+
+    def build(seed):
+        idx = t.from_numpy(routing(T, k, E, seed)).cuda()
+        x = rand((T, K), t.bfloat16, seed)
+        order = qgmoe.TokenOrder(T, k, E)
+
+        def step():
+            return lin.forward_device(x, order=order.sort(idx))
+        step()
+        t.cuda.synchronize()
+        graph = t.cuda.CUDAGraph()
+        with t.cuda.graph(graph):
+            y = step()
+        return idx, x, graph, y, step
+
+    a, b = build(1), build(2)
+    for i in range(3):
+        for idx, x, *_ in (a, b):
+            idx.copy_(t.from_numpy(routing(T, k, E, 30 + i)).cuda())
+            x.copy_(rand((T, K), t.bfloat16, 60 + i))
+        a[2].replay()
+        b[2].replay()
+        t.cuda.synchronize()
+        for _i, _x, _g, y, step in (a, b):
+            assert t.equal(y, step())
+    lin.sync()
+
+
+def test_current_device_is_left():
+    t = torch_()
+    lin = qgmoe.Int8Linear(*weights((8, 16), 1))
+    assert t.cuda.current_device() == 0
+    lin.forward_device(t.zeros((2, 16), device="cuda"))
+    assert t.cuda.current_device() == 0
+
+
+def test_device_refusals():
+    t = torch_()
+    lin = qgmoe.Int8Linear(*weights((2, 8, 16), 1))
+    one = qgmoe.Int8Linear(*weights((8, 16), 1))
+    order = qgmoe.TokenOrder(4, 2, 2)
+    x = t.zeros((4, 16), device="cuda")
+    codes, scale = qgmoe.quantize_rows(x)
+    bad = [
+        lambda: lin.forward_device(x),                                   # groups without offsets
+        lambda: lin.forward_device(x, order=order, offsets=order.offsets),
+        lambda: lin.forward_device(x[:3], order=order),
+        lambda: lin.forward_device(x, offsets=order.offsets[:2]),
+        lambda: lin.forward_device(x, order=qgmoe.TokenOrder(4, 2, 3)),
+        lambda: one.forward_device(x[:, :8]),
+        lambda: one.forward_device(x.double()),
+        lambda: one.forward_device(x.cpu()),
+        lambda: one.forward_device(x, t.zeros((4, 9), device="cuda")),
+        lambda: one.matmul_device(codes.float(), scale),
+        lambda: one.matmul_device(codes, scale[:2]),
+        lambda: one.matmul_device(codes.t().contiguous().t(), scale),
+        lambda: one.forward(np.zeros((2, 15), np.float32)),
+        lambda: qgmoe.quantize_rows(x[:, ::2]),
+        lambda: qgmoe.quantize_rows(x[:3], order),
+        lambda: qgmoe.quantize_rows(x.to(t.int32)),
+        lambda: qgmoe.Int8Linear(t.zeros((8, 16), dtype=t.int8, device="cuda"), np.zeros(8, np.float32)),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"case {i} was taken")
+    # the library's own: a pitch that is no multiple of 16, codes off a 16-byte boundary
+    buf = t.zeros(4 * 24 + 16, dtype=t.int8, device="cuda")
+    for c in (buf[:96].view(4, 24)[:, :16], buf[1:65].view(4, 16)):
+        with pytest.raises(qgmoe.QgmoeError) as e:
+            one.matmul_device(c, scale)
+        assert e.value.status == qgmoe.ERR_INVALID_ARG
+    with pytest.raises(qgmoe.QgmoeError):
+        lin.forward(np.zeros((2, 16), np.float32))

@@ -1,0 +1,391 @@
+"""Tokens in expert order (qgmoe_sort_tokens and the calls after it) against
+plain 64-bit forms.
+
+Tolerances count roundings, u = 2^-24 for float32 and half an epsilon of the
+output's type: a sum of n fused products has error at most n u sum|terms|
+(first order), a product u |value|, and the final rounding eps/2 |value|; a
+factor 1.01 covers the second order."""
+import numpy as np
+import pytest
+
+import qgmoe
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def torch_():
+    import torch
+    return torch
+
+
+def dtypes():
+    t = torch_()
+    return {"f32": t.float32, "f16": t.float16, "bf16": t.bfloat16}
+
+
+def half(dtype):
+    """Largest relative error of one rounding to dtype; none for float32,
+    where the last operation's rounding is already counted."""
+    t = torch_()
+    return 0.0 if dtype == t.float32 else t.finfo(dtype).eps / 2
+
+
+def routing(T, k, E, seed, bad=0.0, repeat=False):
+    rng = np.random.default_rng(seed)
+    if repeat:
+        idx = rng.integers(0, E, (T, k))
+    else:
+        idx = np.argsort(rng.random((T, E)), 1)[:, :k]
+    if bad:
+        wrong = np.array([-1, E, np.iinfo(np.int32).min, np.iinfo(np.int32).max, E + 7])
+        m = rng.random((T, k)) < bad
+        idx = np.where(m, rng.choice(wrong, (T, k)), idx)
+    return idx.astype(np.int32)
+
+
+def plain_order(idx, E):
+    """(offsets, pair_row, row_pair) by a loop over the pairs of each expert."""
+    flat = idx.reshape(-1)
+    offsets, row_pair = [0], []
+    for e in range(E):
+        row_pair += [p for p in np.nonzero(flat == e)[0]]
+        offsets.append(len(row_pair))
+    pair_row = np.full(flat.size, -1, np.int32)
+    pair_row[row_pair] = np.arange(len(row_pair))
+    rp = np.full(flat.size, -1, np.int32)
+    rp[:len(row_pair)] = row_pair
+    return np.array(offsets, np.int32), pair_row.reshape(idx.shape), rp
+
+
+def check_order(order, idx, E):
+    offsets, pair_row, row_pair = plain_order(idx, E)
+    np.testing.assert_array_equal(order.offsets.cpu().numpy(), offsets)
+    np.testing.assert_array_equal(order.pair_row.cpu().numpy(), pair_row)
+    np.testing.assert_array_equal(order.row_pair.cpu().numpy(), row_pair)
+
+
+def rand(shape, dtype, seed):
+    t = torch_()
+    g = t.Generator(device="cuda")
+    g.manual_seed(seed)
+    return t.randn(shape, device="cuda", generator=g).to(dtype)
+
+
+def f64(t):
+    return t.detach().cpu().double().numpy()
+
+
+# ---- sort -------------------------------------------------------------------
+@pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 128), (3, 2, 5), (64, 8, 128), (333, 6, 60),
+                                   (100, 32, 64), (513, 1, 1024), (4097, 8, 128), (16384, 2, 3)])
+@pytest.mark.parametrize("bad", [0.0, 0.3, 1.0])
+def test_sort(T, k, E, bad):
+    idx = routing(T, k, E, T + k, bad)
+    order = qgmoe.sort_tokens(torch_().from_numpy(idx).cuda(), E)
+    check_order(order, idx, E)
+
+
+def test_sort_same_expert_twice_and_one_expert_for_all():
+    idx = routing(700, 4, 3, 1, 0.1, repeat=True)
+    check_order(qgmoe.sort_tokens(torch_().from_numpy(idx).cuda(), 3), idx, 3)
+    idx = np.full((900, 2), 5, np.int32)
+    check_order(qgmoe.sort_tokens(torch_().from_numpy(idx).cuda(), 8), idx, 8)
+
+
+def test_sort_of_no_tokens():
+    t = torch_()
+    order = qgmoe.sort_tokens(t.empty((0, 4), dtype=t.int32, device="cuda"), 7)
+    assert order.offsets.tolist() == [0] * 8
+    x = t.empty((0, 16), device="cuda")
+    assert qgmoe.gather_rows(x, order).shape == (0, 16)
+    assert qgmoe.combine_rows(x, t.empty((0, 4), device="cuda"), order).shape == (0, 16)
+
+
+def test_sort_unaligned_ids_and_without_row_pair():
+    """The ids start 4 bytes past a 16-byte boundary; row_pair is optional."""
+    t = torch_()
+    idx = routing(129, 3, 9, 4, 0.2)
+    buf = t.full((idx.size + 1,), -1, dtype=t.int32, device="cuda")
+    buf[1:] = t.from_numpy(idx.reshape(-1)).cuda()
+    offsets = t.full((10,), -7, dtype=t.int32, device="cuda")
+    pair_row = t.full(idx.shape, -7, dtype=t.int32, device="cuda")
+    assert qgmoe.lib().qgmoe_sort_tokens(buf.data_ptr() + 4, 129, 3, 9, offsets.data_ptr(),
+                                         pair_row.data_ptr(), None, None) == 0
+    t.cuda.synchronize()
+    want = plain_order(idx, 9)
+    np.testing.assert_array_equal(offsets.cpu().numpy(), want[0])
+    np.testing.assert_array_equal(pair_row.cpu().numpy(), want[1])
+
+
+# ---- gather -------------------------------------------------------------------
+@pytest.mark.parametrize("H", [1, 7, 8, 1000, 1001, 2048, 4104])
+@pytest.mark.parametrize("xt,yt", [("f32", "f32"), ("f32", "bf16"), ("bf16", "bf16"),
+                                   ("f16", "f32"), ("bf16", "f16"), ("f32", "f16")])
+def test_gather_is_a_copy_rounded_once(H, xt, yt):
+    """Bit for bit torch's conversion; rows that no pair owns keep what they
+    held."""
+    t = torch_()
+    T, k, E = 37, 3, 11
+    idx = routing(T, k, E, H, 0.2)
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), E)
+    x = rand((T, H), dtypes()[xt], H)
+    out = t.full((T * k, H), 7.5, dtype=dtypes()[yt], device="cuda")
+    assert qgmoe.gather_rows(x, order, out=out) is out
+    want = t.full_like(out, 7.5)
+    n = int(order.offsets[-1])
+    want[:n] = x[(order.row_pair[:n] // k).long()].to(out.dtype)
+    assert t.equal(out, want)
+
+
+def test_gather_default_type_and_unaligned_rows():
+    t = torch_()
+    idx = routing(20, 2, 4, 3)
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), 4)
+    x = rand((21, 1001), t.bfloat16, 5)[1:]  # rows start 2 bytes past a boundary
+    assert x.is_contiguous() and x.data_ptr() % 16
+    out = qgmoe.gather_rows(x, order)
+    assert out.dtype == t.bfloat16
+    assert t.equal(out, x[(order.row_pair // 2).long()])
+    y = rand((20, 64), t.float32, 6).flatten()
+    y = t.cat([y[:1], y])[1:].view(20, 64)   # a multiple of 8 elements, base not aligned
+    assert y.data_ptr() % 16
+    assert t.equal(qgmoe.gather_rows(y, order), y[(order.row_pair // 2).long()])
+
+
+# ---- combine --------------------------------------------------------------------
+def combine_case(T, k, E, H, rt, seed, bad):
+    t = torch_()
+    idx = routing(T, k, E, seed, bad)
+    if T > 2:
+        idx[2] = -1  # a token that no expert takes
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), E)
+    rows = rand((T * k, H), dtypes()[rt], seed + 1)
+    w = t.softmax(rand((T, k), t.float32, seed + 2), 1)
+    n = int(order.offsets[-1])
+    rows[n:] = float("nan")                      # rows that no pair owns
+    w[order.pair_row < 0] = float("nan")         # weights of pairs without a row
+    pr = order.pair_row.cpu().numpy()
+    live = pr >= 0
+    r64 = np.where(live[:, :, None], np.nan_to_num(f64(rows))[np.maximum(pr, 0)], 0.0)
+    w64 = np.where(live, np.nan_to_num(f64(w)), 0.0)
+    return order, rows, w, r64, w64, pr, live, n
+
+
+@pytest.mark.parametrize("T,k,E,H", [(1, 1, 1, 1), (1, 8, 16, 2048), (32, 4, 16, 1024),
+                                     (37, 3, 11, 1001), (19, 32, 40, 264), (300, 5, 9, 4104)])
+@pytest.mark.parametrize("rt,ot", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"),
+                                   ("f16", "f32"), ("f16", "bf16"), ("f32", "f16")])
+def test_combine_and_gather_backward(T, k, E, H, rt, ot):
+    order, rows, w, r64, w64, _pr, _live, _n = combine_case(T, k, E, H, rt, 7 * T + H, 0.2)
+    out = qgmoe.combine_rows(rows, w, order, dtype=dtypes()[ot])
+    ref = (r64 * w64[:, :, None]).sum(1)
+    tol = 1.01 * (k * U * (np.abs(r64) * w64[:, :, None]).sum(1) + half(out.dtype) * np.abs(ref))
+    assert np.all(np.abs(f64(out) - ref) <= tol + (2.0 ** -25 if ot == "f16" else 0))
+    if T > 2:
+        assert not f64(out)[2].any()
+    grad = qgmoe.gather_rows_backward(rows, order, dtype=dtypes()[ot])
+    ref = r64.sum(1)
+    tol = 1.01 * (k * U * np.abs(r64).sum(1) + half(out.dtype) * np.abs(ref))
+    assert np.all(np.abs(f64(grad) - ref) <= tol + (2.0 ** -25 if ot == "f16" else 0))
+
+
+@pytest.mark.parametrize("T,k,E,H", [(1, 1, 1, 1), (1, 8, 16, 2048), (33, 4, 16, 1024),
+                                     (37, 3, 11, 1001), (19, 32, 40, 264), (300, 5, 9, 4104)])
+@pytest.mark.parametrize("rt,gt", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32"),
+                                   ("bf16", "f32"), ("f32", "bf16")])
+def test_combine_backward(T, k, E, H, rt, gt):
+    t = torch_()
+    order, rows, w, r64, w64, pr, live, n = combine_case(T, k, E, H, rt, 5 * T + H, 0.2)
+    g = rand((T, H), dtypes()[gt], 3)
+    g64 = f64(g)
+    keep = t.full_like(rows, 2.5)
+    grad_rows, grad_w = qgmoe.combine_rows_backward(g, rows, w, order, grad_rows=keep)
+    assert grad_rows is keep and grad_w.dtype == t.float32
+    ref = w64[:, :, None] * g64[:, None, :]
+    got = f64(grad_rows)
+    assert np.all(got[n:] == 2.5)
+    tol = 1.01 * (U + half(rows.dtype)) * np.abs(ref)
+    err = np.abs(np.where(live[:, :, None], got[np.maximum(pr, 0)], 0.0) - ref)
+    assert np.all(err <= tol + (2.0 ** -25 if rt == "f16" else 0))
+    terms = r64 * g64[:, None, :]
+    # a lane sums at most 8 ceil(H / 256) products, five sums join the lanes
+    tol = 1.01 * (8 * -(-H // 256) + 5) * U * np.abs(terms).sum(2)
+    assert np.all(np.abs(f64(grad_w) - terms.sum(2)) <= tol)
+    assert not f64(grad_w)[~live].any()
+
+
+def test_gradients_against_differences():
+    """The loss sum(c * out) is linear in rows and in weights, and the token
+    gradient is linear in x: central differences of the 64-bit form agree
+    with the kernels' gradients up to the roundings of the gradients."""
+    t = torch_()
+    T, k, E, H = 6, 2, 3, 9
+    idx = routing(T, k, E, 2)
+    order = qgmoe.sort_tokens(t.from_numpy(idx).cuda(), E)
+    x, w, c = rand((T, H), t.float32, 1), rand((T, k), t.float32, 2), rand((T, H), t.float32, 3)
+    pr = order.pair_row.cpu().numpy()
+    x64, w64, c64 = f64(x), f64(w), f64(c)
+
+    def loss(x64, w64):
+        rows = np.zeros((T * k, H))
+        rows[pr.reshape(-1)] = np.repeat(x64, k, 0)
+        return float((c64 * (rows[pr] * w64[:, :, None]).sum(1)).sum())
+
+    grad_rows, grad_w = qgmoe.combine_rows_backward(c, qgmoe.gather_rows(x, order), w, order)
+    grad_x = qgmoe.gather_rows_backward(grad_rows, order)
+    h = 2.0 ** -10
+    for got, arg in ((f64(grad_x), 0), (f64(grad_w), 1)):
+        for at in np.ndindex(got.shape):
+            a = [x64.copy(), w64.copy()]
+            b = [x64.copy(), w64.copy()]
+            a[arg][at] += h
+            b[arg][at] -= h
+            num = (loss(*a) - loss(*b)) / (2 * h)
+            size = np.abs(c64[at[0]]).max() * max(np.abs(w64[at[0]]).sum(), np.abs(x64[at[0]]).sum())
+            # linear: the difference is exact but for 64-bit cancellation
+            assert abs(got[at] - num) <= 16 * U * size + 1e-9, (arg, at)
+
+
+@pytest.mark.parametrize("which", ["rows", "weights"])
+def test_combine_backward_of_one_input_only(which):
+    t = torch_()
+    order, rows, w, _r, _w, _pr, _live, n = combine_case(30, 4, 8, 512, "f32", 9, 0.0)
+    g = rand((30, 512), t.float32, 3)
+    both = qgmoe.combine_rows_backward(g, rows, w, order)
+    out = t.full_like(rows if which == "rows" else w, -3.0)
+    a = dict(rows=(None, w.data_ptr(), out.data_ptr(), None),
+             weights=(rows.data_ptr(), None, None, out.data_ptr()))[which]
+    assert qgmoe.lib().qgmoe_combine_rows_backward(
+        g.data_ptr(), 0, a[0], 0, a[1], 30, 4, 512, order.pair_row.data_ptr(), a[2], a[3],
+        t.cuda.current_stream().cuda_stream) == 0
+    assert t.equal(out[:n] if which == "rows" else out, both[0][:n] if which == "rows" else both[1])
+
+
+def test_rows_outside_the_buffer_count_as_none():
+    """pair_row values that no sort gives are bounds-checked, not followed."""
+    t = torch_()
+    T, k, H = 5, 2, 16
+    order = qgmoe.TokenOrder(T, k, 4)
+    order.pair_row.copy_(t.tensor([[0, 10], [1 << 30, 1], [-5, 2], [3, 4], [5, 6]]))
+    x = rand((T, H), t.float32, 1)
+    rows = t.zeros((T * k, H), device="cuda")
+    qgmoe.gather_rows(x, order, out=rows)
+    want = t.zeros_like(rows)
+    for r, tok in ((0, 0), (1, 1), (2, 2), (3, 3), (4, 3), (5, 4), (6, 4)):
+        want[r] = x[tok]
+    assert t.equal(rows, want)
+    w = t.ones((T, k), device="cuda")
+    out = qgmoe.combine_rows(rows, w, order)
+    assert t.equal(out, x * t.tensor([1., 1., 1., 2., 2.], device="cuda")[:, None])
+    _gr, gw = qgmoe.combine_rows_backward(x, rows, w, order)
+    assert gw[0, 1] == 0 and gw[1, 0] == 0 and gw[2, 0] == 0
+
+
+def test_other_stream_and_results_reused():
+    """Work on a stream of its own, results allocated for it, while the
+    default stream keeps allocating."""
+    t = torch_()
+    T, k, E, H = 256, 4, 16, 512
+    side = t.cuda.Stream()
+    for i in range(20):
+        idx = routing(T, k, E, i)
+        di = t.from_numpy(idx).cuda()
+        x = rand((T, H), t.float32, i)
+        w = t.full((T, k), 0.25, device="cuda")
+        side.wait_stream(t.cuda.current_stream())
+        order = qgmoe.sort_tokens(di, E, stream=side)
+        out = qgmoe.combine_rows(qgmoe.gather_rows(x, order, stream=side), w, order, stream=side)
+        junk = [t.randn(T * k, H, device="cuda") for _ in range(3)]
+        side.synchronize()
+        assert t.equal(out, x)
+        check_order(order, idx, E)
+        del junk, di
+
+
+def test_two_captured_graphs_interleaved():
+    t = torch_()
+    T, k, E, H = 64, 2, 8, 264
+
+    def build(seed):
+        idx = t.from_numpy(routing(T, k, E, seed)).cuda()
+        x, w = rand((T, H), t.bfloat16, seed), rand((T, k), t.float32, seed + 1)
+        g = rand((T, H), t.bfloat16, seed + 2)
+        order = qgmoe.TokenOrder(T, k, E)
+
+        def step():
+            order.sort(idx)
+            rows = qgmoe.gather_rows(x, order)
+            out = qgmoe.combine_rows(rows, w, order)
+            gr, gw = qgmoe.combine_rows_backward(g, rows, w, order)
+            return out, gr, gw, qgmoe.gather_rows_backward(gr, order)
+        step()
+        t.cuda.synchronize()
+        graph = t.cuda.CUDAGraph()
+        with t.cuda.graph(graph):
+            res = step()
+        return idx, x, graph, res, step
+
+    a, b = build(1), build(2)
+    for i in range(3):
+        for idx, x, *_ in (a, b):
+            idx.copy_(t.from_numpy(routing(T, k, E, 100 + i)).cuda())
+            x.copy_(rand((T, H), t.bfloat16, 50 + i))
+        a[2].replay()
+        b[2].replay()
+        t.cuda.synchronize()
+        for _idx, _x, _g, res, step in (a, b):
+            for got, want in zip(res, step()):
+                assert t.equal(got, want)
+
+
+def test_long_offsets():
+    """Rows past 2^31 bytes and 2^31 elements from the start."""
+    t = torch_()
+    T, k, H = 300000, 1, 8192
+    if t.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip("needs 20 GB")
+    x = t.zeros((T, H), dtype=t.bfloat16, device="cuda")
+    x[:, 0] = t.arange(T, device="cuda") % 251
+    x[:, -1] = t.arange(T, device="cuda") % 241
+    idx = (t.arange(T - 1, -1, -1, device="cuda") * 7 // T).to(t.int32).view(T, k)
+    order = qgmoe.sort_tokens(idx.contiguous(), 7)
+    rows = qgmoe.gather_rows(x, order)
+    tok = order.row_pair.long()
+    assert t.equal(rows[:, 0], x[tok, 0]) and t.equal(rows[:, -1], x[tok, -1])
+    out = qgmoe.combine_rows(rows, t.ones((T, k), device="cuda"), order)
+    assert t.equal(out[:, 0], x[:, 0]) and t.equal(out[:, -1], x[:, -1])
+
+
+# ---- refusals ------------------------------------------------------------------------
+def test_python_refusals():
+    t = torch_()
+    order = qgmoe.TokenOrder(4, 2, 3)
+    x = t.zeros((4, 8), device="cuda")
+    rows = t.zeros((8, 8), device="cuda")
+    w = t.zeros((4, 2), device="cuda")
+    bad = [
+        lambda: order.sort(t.zeros((4, 2), dtype=t.int64, device="cuda")),
+        lambda: order.sort(t.zeros((4, 3), dtype=t.int32, device="cuda")),
+        lambda: order.sort(t.zeros((4, 2), dtype=t.int32)),
+        lambda: order.sort(t.zeros((2, 4), dtype=t.int32, device="cuda").t()),
+        lambda: qgmoe.sort_tokens(t.zeros(4, dtype=t.int32, device="cuda"), 3),
+        lambda: qgmoe.TokenOrder(4, 2, 1025),
+        lambda: qgmoe.TokenOrder(4, 0, 3),
+        lambda: qgmoe.gather_rows(t.zeros((5, 8), device="cuda"), order),
+        lambda: qgmoe.gather_rows(x.double(), order),
+        lambda: qgmoe.gather_rows(x.cpu(), order),
+        lambda: qgmoe.gather_rows(t.zeros((4, 16), device="cuda")[:, ::2], order),
+        lambda: qgmoe.gather_rows(x, order, out=t.zeros((8, 9), device="cuda")),
+        lambda: qgmoe.gather_rows(x, order, out=rows, dtype=t.float16),
+        lambda: qgmoe.combine_rows(rows, w.half(), order),
+        lambda: qgmoe.combine_rows(rows, w[:3], order),
+        lambda: qgmoe.combine_rows(x, w, order),
+        lambda: qgmoe.combine_rows_backward(t.zeros((4, 9), device="cuda"), rows, w, order),
+        lambda: qgmoe.combine_rows_backward(x, rows, w, order, grad_rows=rows.half()),
+        lambda: qgmoe.gather_rows_backward(x, order),
+    ]
+    for i, f in enumerate(bad):
+        with pytest.raises(ValueError):
+            f()
+            pytest.fail(f"case {i} was taken")
