@@ -20,6 +20,7 @@ import numpy as np
 
 import qgmoe as _q
 
+from . import rows as _rows
 from .rows import TokenOrder, _call, _cuda, _need, _on, _result, _row_dtype
 
 
@@ -27,31 +28,30 @@ def _pitch(k: int) -> int:
     return (k + 15) & ~15
 
 
-def _codes(n: int, k: int, device):
-    """[n, pitch] int8 for rows of k codes, and [n] float32 scales."""
-    import torch
-    return (torch.empty((n, _pitch(k)), dtype=torch.int8, device=device),
-            torch.empty(n, dtype=torch.float32, device=device))
-
-
 def quantize_rows(x, order: TokenOrder | None = None, stream=None):
     """x [T, K] -> (codes [R, K] int8, scale [R] float32): R = T, or with
     `order` the T * k rows in expert order (rows that no pair owns hold
     anything).  The codes' row pitch is K rounded up to 16."""
     dev = _cuda(x, "x")
+    return _on(dev, stream, _quantize, x, order)
+
+
+def _quantize(x, order, s):
+    _need(x, "x", x.device if order is None else order.device)
     if x.dim() != 2 or x.shape[1] < 1:
         raise ValueError(f"x: shape {tuple(x.shape)}, expected [rows, row length]")
-    _need(x, "x", dev if order is None else order.device)
-    if order is not None and x.shape[0] != order.n_tokens:
-        raise ValueError(f"x: {x.shape[0]} rows, the order has {order.n_tokens} tokens")
-    xd = _row_dtype(x, "x")
     T, K = x.shape
-    with _on(dev, stream) as s:
-        codes, scale = _codes(T if order is None else order.n_rows, K, dev)
-        _call("qgq8_quantize_rows", x.data_ptr(), xd, T, 1 if order is None else order.top_k, K,
-              None if order is None else order.pair_row.data_ptr(), codes.data_ptr(), _pitch(K),
-              scale.data_ptr(), s)
-    return codes[:, :K], scale
+    R, k, pair_row = T, 1, None
+    if order is not None:
+        if T != order.n_tokens:
+            raise ValueError(f"x: {T} rows, the order has {order.n_tokens} tokens")
+        R, k, pair_row = order.n_rows, order.top_k, order.pair_row.data_ptr()
+    dt, ld = _row_dtype(x, "x"), _pitch(K)
+    codes = x.new_empty((R, ld), dtype=_rows._torch.int8)
+    scale = x.new_empty(R, dtype=_rows._torch.float32)
+    _call("qgq8_quantize_rows", x.data_ptr(), dt, T, k, K, pair_row, codes.data_ptr(), ld,
+          scale.data_ptr(), s)
+    return codes if ld == K else codes[:, :K], scale
 
 
 class Int8Linear:
@@ -116,12 +116,11 @@ class Int8Linear:
         return y.reshape(x.shape[:-1] + (self.out_features,))
 
     def _offsets(self, offsets, device):
-        import torch
         if offsets is None:
             if self.groups != 1:
                 raise ValueError(f"{self.groups} groups: offsets (or order) needed")
             return None
-        _need(offsets, "offsets", device, (self.groups + 1,), torch.int32)
+        _need(offsets, "offsets", device, (self.groups + 1,), _rows._torch.int32)
         return offsets.data_ptr()
 
     def forward_device(self, x, y=None, order: TokenOrder | None = None, offsets=None, dtype=None,
@@ -134,56 +133,61 @@ class Int8Linear:
         dev = _cuda(x, "x")
         if dev.index != self.device:
             raise ValueError(f"x: on {dev}, the linear is on cuda:{self.device}")
-        if x.dim() != 2 or x.shape[1] != self.in_features or not x.is_contiguous():
-            raise ValueError(f"x: shape {tuple(x.shape)}, expected contiguous "
-                             f"[rows, {self.in_features}]")
-        xd = _row_dtype(x, "x")
-        T, k, pair_row = x.shape[0], 1, None
+        return _on(dev, stream, self._forward, x, y, order, offsets, dtype)
+
+    def _forward(self, x, y, order, offsets, dtype, s):
+        shape, K = x.shape, self.in_features
+        if len(shape) != 2 or shape[1] != K or not x.is_contiguous():
+            raise ValueError(f"x: shape {tuple(shape)}, expected contiguous [rows, {K}]")
+        dt, T = _row_dtype(x, "x"), shape[0]
+        R, k, pair_row = T, 1, None
         if order is not None:
             if offsets is not None:
                 raise ValueError("order has its own offsets")
-            if order.n_tokens != T or order.device != dev:
-                raise ValueError(f"x: {T} rows on {dev}, the order has {order.n_tokens} tokens "
-                                 f"on {order.device}")
-            k, pair_row, offsets = order.top_k, order.pair_row.data_ptr(), order.offsets
-        off = self._offsets(offsets, dev)
-        with _on(dev, stream) as s:
-            y = _result(y, "y", x, (T * k, self.out_features), dtype)
-            codes, scale = _codes(T * k, self.in_features, dev)
-            _call("qgq8_forward_device", self.h, x.data_ptr(), xd, T, k, pair_row, off,
-                  codes.data_ptr(), codes.stride(0) if T else _pitch(self.in_features),
-                  scale.data_ptr(), y.data_ptr(), _row_dtype(y, "y"), s)
+            if order.n_tokens != T or order.device != x.device:
+                raise ValueError(f"x: {T} rows on {x.device}, the order has {order.n_tokens} "
+                                 f"tokens on {order.device}")
+            R, k, pair_row, offsets = order.n_rows, order.top_k, order.pair_row.data_ptr(), \
+                order.offsets
+        off = self._offsets(offsets, x.device)
+        y = _result(y, "y", x, (R, self.out_features), dtype)
+        # codes [R, pitch], then their scales: one allocation
+        ld = _pitch(K)
+        work = x.new_empty(R * (ld + 4), dtype=_rows._torch.int8)
+        at = work.data_ptr()
+        _call("qgq8_forward_device", self.h, x.data_ptr(), dt, T, k, pair_row, off, at, ld,
+              at + R * ld, y.data_ptr(), _row_dtype(y, "y"), s)
         return y
 
     def matmul_device(self, codes, scale, y=None, offsets=None, dtype=None, stream=None):
         """Enqueue the product of codes [R, in] int8 (row pitch a multiple of
         16, as quantize_rows gives them) and scale [R] float32; y [R, out] of
         `dtype` (default float32)."""
-        import torch
         dev = _cuda(codes, "codes")
         if dev.index != self.device:
             raise ValueError(f"codes: on {dev}, the linear is on cuda:{self.device}")
-        if codes.dtype != torch.int8 or codes.dim() != 2 or codes.shape[1] != self.in_features or \
-                (codes.shape[1] > 1 and codes.stride(1) != 1):
-            raise ValueError(f"codes: {codes.dtype} {tuple(codes.shape)}, expected int8 "
-                             f"[rows, {self.in_features}] with unit stride along a row")
-        R = codes.shape[0]
-        _need(scale, "scale", dev, (R,), torch.float32)
-        ld = codes.stride(0) if R > 1 else _pitch(self.in_features)
-        off = self._offsets(offsets, dev)
-        with _on(dev, stream) as s:
-            y = _result(y, "y", scale, (R, self.out_features), dtype)
-            _call("qgq8_matmul_device", self.h, codes.data_ptr(), ld, scale.data_ptr(), R, off,
-                  y.data_ptr(), _row_dtype(y, "y"), s)
+        return _on(dev, stream, self._matmul, codes, scale, y, offsets, dtype)
+
+    def _matmul(self, codes, scale, y, offsets, dtype, s):
+        shape, K = codes.shape, self.in_features
+        if codes.dtype != _rows._torch.int8 or len(shape) != 2 or shape[1] != K or \
+                (K > 1 and codes.stride(1) != 1):
+            raise ValueError(f"codes: {codes.dtype} {tuple(shape)}, expected int8 [rows, {K}] "
+                             "with unit stride along a row")
+        R = shape[0]
+        _need(scale, "scale", codes.device, (R,), _rows._torch.float32)
+        ld = codes.stride(0) if R > 1 else _pitch(K)
+        off = self._offsets(offsets, codes.device)
+        y = _result(y, "y", scale, (R, self.out_features), dtype)
+        _call("qgq8_matmul_device", self.h, codes.data_ptr(), ld, scale.data_ptr(), R, off,
+              y.data_ptr(), _row_dtype(y, "y"), s)
         return y
 
     def sync(self, stream=None):
         """Waits for the stream (None: the device's current one); raises on a
         device error flag (qgq8_sync)."""
-        with _on(_device(self.device), stream) as s:
-            _call("qgq8_sync", self.h, s)
+        torch = _rows._torch or _rows._load()
+        _on(torch.device("cuda", self.device), stream, self._sync)
 
-
-def _device(index: int):
-    import torch
-    return torch.device("cuda", index)
+    def _sync(self, s):
+        _call("qgq8_sync", self.h, s)

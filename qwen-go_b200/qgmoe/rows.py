@@ -24,32 +24,37 @@ import qgmoe as _q
 
 MAX_EXPERTS = 1024
 
+# torch, imported by the first call: importing qgmoe does not need it
+_torch = None
 _DT = None
+_raw_stream = _cur_device = None
 
 
-def _dtypes():
-    global _DT
-    if _DT is None:
-        import torch
-        _DT = {torch.float32: _q.DT_F32, torch.float16: _q.DT_F16, torch.bfloat16: _q.DT_BF16}
-    return _DT
+def _load():
+    global _torch, _DT, _raw_stream, _cur_device
+    import torch
+    _DT = {torch.float32: _q.DT_F32, torch.float16: _q.DT_F16, torch.bfloat16: _q.DT_BF16}
+    _raw_stream = torch._C._cuda_getCurrentRawStream
+    _cur_device = torch.cuda.current_device
+    _torch = torch
+    return torch
 
 
 def _row_dtype(t, what: str) -> int:
-    dt = _dtypes().get(t.dtype)
+    dt = _DT.get(t.dtype)
     if dt is None:
         raise ValueError(f"{what}: float32, float16 or bfloat16, got {t.dtype}")
     return dt
 
 
 def _need(t, what: str, device, shape=None, dtype=None):
-    """A contiguous tensor on `device` of that shape and type."""
-    if not t.is_cuda or t.device != device:
+    """A contiguous tensor on `device` of that shape (a tuple) and type."""
+    if t.device != device:
         raise ValueError(f"{what}: on {t.device}, expected {device}")
     if not t.is_contiguous():
         raise ValueError(f"{what}: not contiguous")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected {shape}")
     if dtype is not None and t.dtype != dtype:
         raise ValueError(f"{what}: {t.dtype}, expected {dtype}")
 
@@ -57,6 +62,8 @@ def _need(t, what: str, device, shape=None, dtype=None):
 def _cuda(t, what: str):
     if not getattr(t, "is_cuda", False):
         raise ValueError(f"{what}: a CUDA tensor is needed")
+    if _torch is None:
+        _load()
     return t.device
 
 
@@ -67,46 +74,42 @@ _LEGACY = 1
 
 @contextlib.contextmanager
 def _torch_on(device, stream):
-    import torch
-    if isinstance(stream, torch.cuda.Stream):
+    if stream is None:
+        st = _torch.cuda.current_stream(device)
+    elif isinstance(stream, _torch.cuda.Stream):
         st = stream
         if st.device != device:
             raise ValueError(f"stream of {st.device}, expected {device}")
     elif stream in (0, _LEGACY):
-        st = torch.cuda.default_stream(device)
+        st = _torch.cuda.default_stream(device)
     else:
-        st = torch.cuda.ExternalStream(stream, device=device)
-    with torch.cuda.device(device), torch.cuda.stream(st):
+        st = _torch.cuda.ExternalStream(stream, device=device)
+    with _torch.cuda.device(device), _torch.cuda.stream(st):
         yield st.cuda_stream or _LEGACY
 
 
-class _Here:
-    """The device is current and no stream was given: nothing to switch."""
-    __slots__ = ("s",)
-
-    def __init__(self, s):
-        self.s = s
-
-    def __enter__(self):
-        return self.s
-
-    def __exit__(self, *exc):
-        return False
+def _on(device, stream, enqueue, *args):
+    """enqueue(*args, s) where torch allocates for, and the library launches
+    on, `stream` of `device`; s is the stream's handle.  Nothing is switched
+    when the device is current and no stream is given: the Python side of a
+    decode-sized call costs as much as its kernel."""
+    index = device.index
+    if stream is None and index == _cur_device():
+        return enqueue(*args, _raw_stream(index) or _LEGACY)
+    with _torch_on(device, stream) as s:
+        return enqueue(*args, s)
 
 
-def _on(device, stream):
-    """Context in which torch allocates for, and the library launches on,
-    `stream` of `device`; gives the stream's handle."""
-    import torch
-    if stream is None:
-        if device.index == torch.cuda.current_device():
-            return _Here(torch.cuda.current_stream().cuda_stream or _LEGACY)
-        return _torch_on(device, torch.cuda.current_stream(device))
-    return _torch_on(device, stream)
+_fns = {}
 
 
 def _call(name, *args):
-    _q._check(getattr(_q.lib(), name)(*args), name)
+    fn = _fns.get(name)
+    if fn is None:
+        fn = _fns[name] = getattr(_q.lib(), name)
+    rc = fn(*args)
+    if rc:
+        _q._check(rc, name)
 
 
 class TokenOrder:
@@ -122,15 +125,17 @@ class TokenOrder:
     not be needed any more by work of another stream."""
 
     def __init__(self, n_tokens: int, top_k: int, n_experts: int, device=None):
-        import torch
+        torch = _torch or _load()
         if n_tokens < 0 or top_k < 1 or n_tokens * top_k > 1 << 30:
             raise ValueError(f"bad n_tokens={n_tokens}, top_k={top_k}")
         if not 1 <= n_experts <= MAX_EXPERTS:
             raise ValueError(f"n_experts={n_experts} (1..{MAX_EXPERTS})")
-        dev = torch.device("cuda", torch.cuda.current_device()) if device is None else \
-            torch.device(device) if not isinstance(device, int) else torch.device("cuda", device)
-        if dev.index is None:
-            dev = torch.device(dev.type, torch.cuda.current_device())
+        if device is None or isinstance(device, int):
+            dev = torch.device("cuda", _cur_device() if device is None else device)
+        else:
+            dev = torch.device(device)
+            if dev.index is None:
+                dev = torch.device(dev.type, _cur_device())
         self.n_tokens, self.top_k, self.n_experts, self.device = n_tokens, top_k, n_experts, dev
         self.n_rows = n_tokens * top_k
         kw = dict(dtype=torch.int32, device=dev)
@@ -141,13 +146,13 @@ class TokenOrder:
     def sort(self, sel_idx, stream=None) -> "TokenOrder":
         """sel_idx [n_tokens, top_k] int32, as a router selects (MoeMLP's
         sel_idx, qgmoe_route_static); ids outside [0, n_experts) get no row."""
-        import torch
-        _need(sel_idx, "sel_idx", self.device, (self.n_tokens, self.top_k), torch.int32)
-        with _on(self.device, stream) as s:
-            _call("qgmoe_sort_tokens", sel_idx.data_ptr(), self.n_tokens, self.top_k,
-                  self.n_experts, self.offsets.data_ptr(), self.pair_row.data_ptr(),
-                  self.row_pair.data_ptr(), s)
+        _need(sel_idx, "sel_idx", self.device, (self.n_tokens, self.top_k), _torch.int32)
+        _on(self.device, stream, self._sort, sel_idx)
         return self
+
+    def _sort(self, sel_idx, s):
+        _call("qgmoe_sort_tokens", sel_idx.data_ptr(), self.n_tokens, self.top_k, self.n_experts,
+              self.offsets.data_ptr(), self.pair_row.data_ptr(), self.row_pair.data_ptr(), s)
 
 
 def sort_tokens(sel_idx, n_experts: int, stream=None) -> TokenOrder:
@@ -155,64 +160,69 @@ def sort_tokens(sel_idx, n_experts: int, stream=None) -> TokenOrder:
     dev = _cuda(sel_idx, "sel_idx")
     if sel_idx.dim() != 2:
         raise ValueError(f"sel_idx: shape {tuple(sel_idx.shape)}, expected [tokens, top_k]")
-    with _on(dev, stream) as s:
+
+    def build(s):
         order = TokenOrder(sel_idx.shape[0], sel_idx.shape[1], n_experts, dev)
-        return order.sort(sel_idx, None if stream is None else s)
+        return order.sort(sel_idx)
+    return _on(dev, stream, build)
 
 
 def _rows_of(t, what: str, order: TokenOrder, n: int):
+    """(row dtype, row length) of [n, H] rows on the order's device."""
     _need(t, what, order.device)
-    if t.dim() != 2 or t.shape[0] != n or t.shape[1] < 1:
-        raise ValueError(f"{what}: shape {tuple(t.shape)}, expected [{n}, row length]")
-    return _row_dtype(t, what)
+    shape = t.shape
+    if len(shape) != 2 or shape[0] != n or shape[1] < 1:
+        raise ValueError(f"{what}: shape {tuple(shape)}, expected [{n}, row length]")
+    return _row_dtype(t, what), shape[1]
 
 
 def _result(out, what: str, like, shape, dtype):
-    """`out` checked, or a new tensor (call inside _on())."""
+    """`out` checked, or a new tensor (call on the stream that fills it)."""
     if out is None:
-        import torch
-        return torch.empty(shape, dtype=like.dtype if dtype is None else dtype, device=like.device)
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
     _need(out, what, like.device, shape, dtype)
     return out
 
 
 def gather_rows(x, order: TokenOrder, out=None, dtype=None, stream=None):
     """x [T, H] -> rows [T * k, H] in expert order, of `dtype` (default: x's)."""
-    xd = _rows_of(x, "x", order, order.n_tokens)
-    H = x.shape[1]
-    with _on(order.device, stream) as s:
-        out = _result(out, "out", x, (order.n_rows, H), dtype)
-        _call("qgmoe_gather_rows", x.data_ptr(), xd, order.n_tokens, order.top_k, H,
-              order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return _on(order.device, stream, _gather, x, order, out, dtype)
+
+
+def _gather(x, order, out, dtype, s):
+    dt, H = _rows_of(x, "x", order, order.n_tokens)
+    out = _result(out, "out", x, (order.n_rows, H), dtype)
+    _call("qgmoe_gather_rows", x.data_ptr(), dt, order.n_tokens, order.top_k, H,
+          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
     return out
 
 
 def gather_rows_backward(grad_rows, order: TokenOrder, out=None, dtype=None, stream=None):
     """The gradient of gather_rows: grad_rows [T * k, H] -> grad_x [T, H]."""
-    gd = _rows_of(grad_rows, "grad_rows", order, order.n_rows)
-    H = grad_rows.shape[1]
-    with _on(order.device, stream) as s:
-        out = _result(out, "out", grad_rows, (order.n_tokens, H), dtype)
-        _call("qgmoe_gather_rows_backward", grad_rows.data_ptr(), gd, order.n_tokens, order.top_k,
-              H, order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return _on(order.device, stream, _gather_backward, grad_rows, order, out, dtype)
+
+
+def _gather_backward(grad_rows, order, out, dtype, s):
+    dt, H = _rows_of(grad_rows, "grad_rows", order, order.n_rows)
+    out = _result(out, "out", grad_rows, (order.n_tokens, H), dtype)
+    _call("qgmoe_gather_rows_backward", grad_rows.data_ptr(), dt, order.n_tokens, order.top_k, H,
+          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
     return out
-
-
-def _weights(w, order: TokenOrder):
-    import torch
-    _need(w, "weights", order.device, (order.n_tokens, order.top_k), torch.float32)
 
 
 def combine_rows(rows, weights, order: TokenOrder, out=None, dtype=None, stream=None):
     """rows [T * k, H], weights [T, k] float32 -> out [T, H]: each token's rows
     weighted and summed in rank order."""
-    rd = _rows_of(rows, "rows", order, order.n_rows)
-    _weights(weights, order)
-    H = rows.shape[1]
-    with _on(order.device, stream) as s:
-        out = _result(out, "out", rows, (order.n_tokens, H), dtype)
-        _call("qgmoe_combine_rows", rows.data_ptr(), rd, weights.data_ptr(), order.n_tokens,
-              order.top_k, H, order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+    return _on(order.device, stream, _combine, rows, weights, order, out, dtype)
+
+
+def _combine(rows, weights, order, out, dtype, s):
+    T, k = order.n_tokens, order.top_k
+    dt, H = _rows_of(rows, "rows", order, order.n_rows)
+    _need(weights, "weights", order.device, (T, k), _torch.float32)
+    out = _result(out, "out", rows, (T, H), dtype)
+    _call("qgmoe_combine_rows", rows.data_ptr(), dt, weights.data_ptr(), T, k, H,
+          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
     return out
 
 
@@ -220,18 +230,20 @@ def combine_rows_backward(grad_out, rows, weights, order: TokenOrder, grad_rows=
                           grad_weights=None, stream=None):
     """The gradients of combine_rows: (grad_rows [T * k, H] of rows' type,
     grad_weights [T, k] float32)."""
-    import torch
-    gd = _rows_of(grad_out, "grad_out", order, order.n_tokens)
-    rd = _rows_of(rows, "rows", order, order.n_rows)
-    _weights(weights, order)
-    H = rows.shape[1]
-    if grad_out.shape[1] != H:
-        raise ValueError(f"grad_out: rows of {grad_out.shape[1]}, expected {H}")
-    with _on(order.device, stream) as s:
-        grad_rows = _result(grad_rows, "grad_rows", rows, (order.n_rows, H), rows.dtype)
-        grad_weights = _result(grad_weights, "grad_weights", weights,
-                               (order.n_tokens, order.top_k), torch.float32)
-        _call("qgmoe_combine_rows_backward", grad_out.data_ptr(), gd, rows.data_ptr(), rd,
-              weights.data_ptr(), order.n_tokens, order.top_k, H, order.pair_row.data_ptr(),
-              grad_rows.data_ptr(), grad_weights.data_ptr(), s)
+    return _on(order.device, stream, _combine_backward, grad_out, rows, weights, order, grad_rows,
+               grad_weights)
+
+
+def _combine_backward(grad_out, rows, weights, order, grad_rows, grad_weights, s):
+    T, k = order.n_tokens, order.top_k
+    gd, H = _rows_of(grad_out, "grad_out", order, T)
+    rd, Hr = _rows_of(rows, "rows", order, order.n_rows)
+    if H != Hr:
+        raise ValueError(f"grad_out: rows of {H}, expected {Hr}")
+    _need(weights, "weights", order.device, (T, k), _torch.float32)
+    grad_rows = _result(grad_rows, "grad_rows", rows, (order.n_rows, H), rows.dtype)
+    grad_weights = _result(grad_weights, "grad_weights", weights, (T, k), _torch.float32)
+    _call("qgmoe_combine_rows_backward", grad_out.data_ptr(), gd, rows.data_ptr(), rd,
+          weights.data_ptr(), T, k, H, order.pair_row.data_ptr(), grad_rows.data_ptr(),
+          grad_weights.data_ptr(), s)
     return grad_rows, grad_weights
