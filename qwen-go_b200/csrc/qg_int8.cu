@@ -10,13 +10,18 @@
 //
 // Swap-AB on the tensor cores, as the group-32 GEMMs (qg_umma.cu) do it:
 //   D[channels, rows] = Q[channels, I] * C[rows, I]^T   (tcgen05.mma kind::i8)
-// so that one tile is 128 channels x up to 256 rows, a batch of few rows costs
-// a narrow N instead of an empty M, and 32 lanes of a warp hold 32 neighbouring
-// channels of one row, which go out as one coalesced run without a detour
-// through shared memory.  Both operands are tiled TMA loads of 128-byte rows
-// (128B swizzle), accumulators are int32 in TMEM, double-buffered: eight
-// epilogue warps drain one buffer while the next tile accumulates.
-//
+// so that a batch of few rows costs a narrow N instead of an empty M.  Both
+// operands are tiled TMA loads of 128-byte rows (128B swizzle), accumulators
+// are int32 in TMEM, drained by eight epilogue warps while the next tile
+// accumulates.  Two kernels:
+//   k_i8       one CTA per tile of 128 channels x up to 16 or 64 rows, for few
+//              rows per group: a stream of weights;
+//   k_i8_pair  a CTA pair (cta_group::2) per tile of 256 channels x up to 512
+//              rows, for prompts.  A tile's operands come from L2, and an
+//              SM gets about 43 bytes a clock from it (128 x 256 tiles of one
+//              CTA need 96 at the MMA's full rate and ran at 45 % of it): the
+//              pair shares its row codes, and 512 rows a tile halve what the
+//              weights cost, 47 bytes a clock in all.
 // Persistent, one CTA per SM, units (group, row tile, channel tile) with the
 // channel tile fastest, so that concurrent CTAs share a row tile and, over the
 // following units, the group's weights in L2.  Every wait is bounded; a wait
@@ -33,7 +38,7 @@
 namespace qg {
 using namespace sm100;
 
-constexpr int I8_M = 128;          // weight rows per tile (= TMEM lanes)
+constexpr int I8_M = 128;          // weight rows per CTA tile (= TMEM lanes)
 constexpr int I8_BK = 128;         // codes per stage: one swizzled 128-byte row
 constexpr int I8_EPI_WARPS = 8;    // warps 0-7: TMEM lane quarter = warp & 3
 constexpr int I8_LOAD_WARP = 8;
@@ -42,6 +47,12 @@ constexpr int I8_THREADS = 10 * 32;
 constexpr int I8_MAX_GROUPS = QG_MAX_EXPERTS;
 constexpr int I8_MAX_IN = 131071;  // 131071 * 128 * 128 < 2^31: exact int32 sums
 constexpr long long I8_WAIT_CYCLES = 4000000000LL;  // ~2 s
+// Epilogue staging of a warp: 32 rows of 32 16-bit channels, 80 bytes apart so
+// that the 8 rows a stmatrix writes fall into different banks; then the scales
+// of its rows, up to four runs of 32.
+constexpr int I8_ROW_PITCH = 80;
+constexpr int I8_RUNS = 4;
+constexpr int I8_STAGING = 32 * I8_ROW_PITCH + I8_RUNS * 128;
 
 // NT: most rows of a tile.  Stages fill the shared memory that one CTA per SM
 // may use, so that as many loads as possible are in flight.
@@ -49,91 +60,437 @@ template <int NT>
 struct I8Cfg {
     static constexpr int A_BYTES = I8_M * I8_BK;
     static constexpr int B_BYTES = NT * I8_BK;
-    static constexpr int BOX = NT < 64 ? NT : 64;  // rows of one TMA box of the row codes
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int BUF = NT < 32 ? 32 : NT;  // TMEM columns per accumulator buffer
     static constexpr int TMEM_COLS = 2 * BUF;
-    static constexpr int S = 208 * 1024 / STAGE_BYTES < 12 ? 208 * 1024 / STAGE_BYTES : 12;
+    static constexpr int S = 192 * 1024 / STAGE_BYTES;
     static constexpr int BAR_BYTES = 8 * (2 * S + 5) + 16;
-    static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4;
-    static constexpr int SMEM = S * STAGE_BYTES + TAB_BYTES + 16 + BAR_BYTES + 1024;
+    static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12;
+    static constexpr int SMEM =
+        S * STAGE_BYTES + I8_EPI_WARPS * I8_STAGING + BAR_BYTES + TAB_BYTES + 1024;
     static_assert(SMEM <= 232448, "shared memory budget");
-    static_assert(STAGE_BYTES % 1024 == 0 && (BOX * I8_BK) % 1024 == 0, "1024-byte aligned tiles");
+    static_assert(STAGE_BYTES % 1024 == 0, "1024-byte aligned tiles");
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM budget");
 };
+// The pair kernel: a tile's rows are one or two parts of up to 256, each an
+// accumulator of 256 TMEM columns; a CTA holds half of a part's row codes.
+constexpr int I8P_PART = 256;
+constexpr int I8P_NT = 2 * I8P_PART;
+constexpr int I8P_BOX = 64;
+constexpr int I8P_HALF_BYTES = I8P_PART / 2 * I8_BK;
+// Stages whose second part waits at the start and the end of a tile (below).
+constexpr int I8P_STAGGER = 2;
+using I8Pair = I8Cfg<I8P_PART>;
 
 struct I8Args {
     const float *xs;         // [R] row scales
     const float *ws;         // [G * RT * 128] channel scales in tile order
     const int32_t *offsets;  // [G + 1] device, or null: one group of R rows
-    int G, R, RT, KB, cols;  // RT channel tiles per group, KB 128-code blocks, y columns
-    int nt;                  // rows of a tile (<= NT, a multiple of 16)
+    int G, R, RT, KB, cols;  // RT 128-row weight tiles per group, KB 128-code blocks, y columns
+    int CT;                  // channel tiles per group: those with channels, or RT / 2 for pairs
+    int nt, gran;            // most rows of a tile; tiles are multiples of gran rows
     void *y;                 // [R, cols]
+    int vec;                 // y rows are 16-byte aligned
     int *err;
 };
 
 // kind::i8 instruction descriptor: int8 A/B, int32 D, both K-major.
-__device__ __forceinline__ uint32_t idesc_i8(int N) {
+__device__ __forceinline__ uint32_t idesc_i8(int M, int N) {
     return (2u << 4)                     // D format S32
            | (1u << 7) | (1u << 10)      // A, B signed 8 bits
            | ((uint32_t)(N >> 3) << 17)  // N / 8
-           | ((uint32_t)(I8_M >> 4) << 24);
+           | ((uint32_t)(M >> 4) << 24);
 }
 
 // One 128-code block as four K=32 MMAs; descriptors advance by 32 bytes.
+#define QG_I8_MMA(GROUP)                                                                      \
+    asm volatile(                                                                             \
+        "{\n\t.reg .pred p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"                      \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                           \
+        "setp.eq.b32 t, %3, %3;\n\t"                                                          \
+        "add.u64 a1, %1, 2;\n\tadd.u64 a2, %1, 4;\n\tadd.u64 a3, %1, 6;\n\t"                  \
+        "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"                  \
+        "tcgen05.mma." GROUP ".kind::i8 [%0], %1, %2, %3, p;\n\t"                             \
+        "tcgen05.mma." GROUP ".kind::i8 [%0], a1, b1, %3, t;\n\t"                             \
+        "tcgen05.mma." GROUP ".kind::i8 [%0], a2, b2, %3, t;\n\t"                             \
+        "tcgen05.mma." GROUP ".kind::i8 [%0], a3, b3, %3, t;\n\t}" ::"r"(d_tmem),             \
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)                                   \
+        : "memory")
 __device__ __forceinline__ void umma_i8_k128(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
                                              uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "setp.eq.b32 t, %3, %3;\n\t"
-        "add.u64 a1, %1, 2;\n\tadd.u64 a2, %1, 4;\n\tadd.u64 a3, %1, 6;\n\t"
-        "add.u64 b1, %2, 2;\n\tadd.u64 b2, %2, 4;\n\tadd.u64 b3, %2, 6;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], a1, b1, %3, t;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], a2, b2, %3, t;\n\t"
-        "tcgen05.mma.cta_group::1.kind::i8 [%0], a3, b3, %3, t;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
-        : "memory");
+    QG_I8_MMA("cta_group::1");
+}
+__device__ __forceinline__ void umma2_i8_k128(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                              uint32_t idesc, uint32_t accumulate) {
+    QG_I8_MMA("cta_group::2");
 }
 
+// ---- CTA pairs ---------------------------------------------------------------
+__device__ __forceinline__ void tmem_alloc2(uint32_t *dst, uint32_t ncols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(dst)),
+                 "r"(ncols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
+                 : "memory");
+}
+// Arrives on *bar of both CTAs once every MMA this thread issued is complete.
+__device__ __forceinline__ void umma2_commit(uint64_t *bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(smem_u32(bar)),
+        "h"((uint16_t)3)
+        : "memory");
+}
+// Tile load into this CTA that signals the barrier at cluster address `bar`.
+__device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *map, int x, int y,
+                                                 uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+// Relaxed: what it announces is that TMEM was read, and those reads are
+// complete.  A release at cluster scope would also wait for the warp's global
+// stores, which no one who waits here reads.
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
+                 : "memory");
+}
+
+// ---- units ---------------------------------------------------------------------
 struct I8Unit {
-    int g, rt, row0, n;
+    int g, ct, row0, n;
 };
 
-// Unit u from the groups' tile prefix (shared memory).  Row tiles of a group
-// all have a.nt rows but the last.
+// Row tiles before each group, and their total at prefix[G] (one warp).  A
+// group whose range is not one has none and raises the flag.
+__device__ __forceinline__ void i8_prefix(const I8Args &a, int *prefix, int lane) {
+    int total = 0;
+    for (int g0 = 0; g0 < a.G; g0 += 32) {
+        const int g = g0 + lane;
+        int n = 0;
+        if (g < a.G) {
+            if (a.offsets) {
+                const int b = *(const volatile int32_t *)(a.offsets + g);
+                const int e = *(const volatile int32_t *)(a.offsets + g + 1);
+                if (b < 0 || e < b || e > a.R)
+                    atomicOr(a.err, QG_FLAG_BAD_GROUP);
+                else
+                    n = e - b;
+            } else {
+                n = a.R;
+            }
+        }
+        int t = (n + a.nt - 1) / a.nt, sum = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(~0u, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (g < a.G) prefix[g] = total + sum - t;
+        total += __shfl_sync(~0u, sum, 31);
+    }
+    if (lane == 0) prefix[a.G] = total;
+}
+
+// Unit u.  The row tiles of a group are as even as multiples of gran allow.
 __device__ __forceinline__ I8Unit i8_unit(const I8Args &a, const int *prefix, int u) {
     I8Unit w;
-    const int ti = u / a.RT;
-    w.rt = u - ti * a.RT;
+    const int ti = u / a.CT;
+    w.ct = u - ti * a.CT;
     int lo = 0, hi = a.G - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (prefix[mid] <= ti) lo = mid; else hi = mid - 1;
     }
     w.g = lo;
-    const int tt = ti - prefix[lo];
     int begin = 0, end = a.R;
     if (a.offsets) {
         begin = *(const volatile int32_t *)(a.offsets + lo);
         end = *(const volatile int32_t *)(a.offsets + lo + 1);
     }
-    w.row0 = begin + tt * a.nt;
-    w.n = min(a.nt, end - w.row0);
+    const int tiles = prefix[lo + 1] - prefix[lo];
+    int size = (end - begin + tiles - 1) / tiles;
+    size = (size + a.gran - 1) / a.gran * a.gran;
+    w.row0 = begin + (ti - prefix[lo]) * size;
+    w.n = min(size, end - w.row0);
     return w;
 }
 
-__device__ __forceinline__ void i8_store(float *p, float v) { *p = v; }
-__device__ __forceinline__ void i8_store(__half *p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void i8_store(__nv_bfloat16 *p, float v) { *p = __float2bfloat16_rn(v); }
-
+// ---- epilogue --------------------------------------------------------------------
 // silu(g) * u = g / (1 + e^-g) * u in float32.  e^-g may overflow to infinity,
 // where the quotient is the right limit, -0.
 __device__ __forceinline__ float swiglu(float g, float u) {
     return __fdividef(g, 1.f + expf(-g)) * u;
 }
+// 16 TMEM lanes x 32 columns: register 4i + 2h + b of a thread is lane
+// lane/4 + 8h, column 8i + 2(lane%4) + b.
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, int (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+// 32 TMEM lanes x 16 columns: a thread is a lane.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, int (&v)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+          "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]),
+          "=r"(v[14]), "=r"(v[15])
+        : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// Four 8x8 matrices of 16-bit pairs, stored transposed: lane l gives the
+// address of stored row l % 8 of matrix l / 8.
+__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
+                     addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
+// Two float32 in a register pair: (float(a), float(b)) * s * t.
+__device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 scaled(int a, int b, uint64_t s, uint64_t t) {
+    float2 r;
+    asm("{\n\t.reg .b64 x;\n\t"
+        "mov.b64 x, {%2, %3};\n\t"
+        "mul.rn.f32x2 x, x, %4;\n\t"
+        "mul.rn.f32x2 x, x, %5;\n\t"
+        "mov.b64 {%0, %1}, x;\n\t}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"((float)a), "f"((float)b), "l"(s), "l"(t));
+    return r;
+}
+__device__ __forceinline__ uint64_t ld_shared_u64(uint32_t addr) {
+    uint64_t v;
+    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ ulonglong2 ld_shared_u64x2(uint32_t addr) {
+    ulonglong2 v;
+    asm volatile("ld.shared.v2.b64 {%0, %1}, [%2];" : "=l"(v.x), "=l"(v.y) : "r"(addr));
+    return v;
+}
+__device__ __forceinline__ void stmatrix2_trans(uint32_t addr, uint32_t r0, uint32_t r1) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x2.trans.shared.b16 [%0], {%1, %2};" ::"r"(addr),
+                 "r"(r0), "r"(r1)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t pack2(__half *, float a, float b) {
+    __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 *, float a, float b) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&h);
+}
 
+// One accumulator of n rows (TMEM columns) by this warp: lane quarter q = 32
+// weight rows of tile rt; the two warps of a quarter take alternate runs of 32
+// rows (half 0 / 1).  y = float(sum) * ws * xs, the row's scale last: it is as
+// large as the activations are, and the sum times it may overflow where y does
+// not.
+//   float32, plain: a lane is a channel, a store 32 neighbouring ones of a row.
+//   SwiGLU: of a quarter's 32 weight rows the first 16 are gate, the others
+//     the up rows of the same 16 channels (k_i8_layout); read 16 lanes at a
+//     time, both land in the same thread.
+//   16-bit: pairs of rows packed in a thread, transposed through the warp's
+//     staging, written 16 bytes at a time.
+// The tile's scales are fetched before its accumulator is waited for
+// (prepare), and a run's TMEM columns while the run before is converted: with
+// two warps per quarter nothing else hides those latencies, and an epilogue
+// that took longer than the tile's MMAs held the whole kernel at 36 % of the
+// tensor pipe.
+template <typename TO, bool SWIGLU>
+struct I8Epilogue {
+    static constexpr bool F32 = sizeof(TO) == 4;
+    static constexpr bool LANES = F32 && !SWIGLU;  // a lane is a channel
+    static constexpr int CH = SWIGLU ? 16 : 32;    // channels of this warp
+    // 16-bit rows leave in 16-byte chunks, a store ROWS rows
+    static constexpr int CHUNKS = CH / 8, ROWS = 32 / CHUNKS;
+
+    const I8Args &a;
+    int q, half, lane;
+    uint32_t staging;
+    float sw[4];  // scales of the weight rows this thread converts
+
+    __device__ __forceinline__ I8Epilogue(const I8Args &a, int warp, int lane, uint32_t staging)
+        : a(a), q(warp & 3), half(warp >> 2), lane(lane), staging(staging) {}
+
+    // ws: the quarter's 32 channel scales
+    __device__ __forceinline__ void prepare(const float *ws, int64_t row0, int n) {
+        float sx[I8_RUNS];
+#pragma unroll
+        for (int i = 0; i < I8_RUNS; i++) {
+            const int c = half * 32 + i * 64 + lane;
+            sx[i] = c < n ? *(const volatile float *)(a.xs + row0 + c) : 0.f;
+        }
+        if constexpr (LANES) {
+            sw[0] = ws[lane];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) sw[i] = ws[(lane >> 2) + 8 * i];
+        }
+#pragma unroll
+        for (int i = 0; i < I8_RUNS; i++)
+            st_shared_f32(staging + 32 * I8_ROW_PITCH + i * 128 + lane * 4, sx[i]);
+        __syncwarp();
+    }
+
+    __device__ __forceinline__ void fetch(uint32_t tmem, int (&v)[2][16]) {
+        if constexpr (LANES) {
+            tmem_ld_32x16(tmem, v[0]);
+            tmem_ld_32x16(tmem + 16, v[1]);
+        } else {
+            tmem_ld_16x32(tmem, v[0]);
+            tmem_ld_16x32(tmem + (16u << 16), v[1]);
+        }
+    }
+
+    // A run: 32 rows, nc of them real.  yp: this thread's place in the first
+    // one (place()).  Two values at a time: mul.f32x2 halves the products, and
+    // walking the rows by their pitch instead of multiplying for each halves
+    // the rest; the epilogue is bound by its instructions.
+    __device__ __forceinline__ void run(const int (&v)[2][16], uint32_t scales, TO *yp, int nc,
+                                        int o0) {
+        const int64_t pitch = a.cols;
+        if constexpr (LANES) {
+            const uint64_t s2 = pack_f32x2(sw[0], sw[0]);
+            const bool mine = o0 + lane < a.cols, whole = nc == 32;
+#pragma unroll
+            for (int c = 0; c < 32; c += 4) {
+                const ulonglong2 sx = ld_shared_u64x2(scales + c * 4);
+                const int *x = &v[c >> 4][c & 15];
+                const float2 f0 = scaled(x[0], x[1], s2, sx.x), f1 = scaled(x[2], x[3], s2, sx.y);
+                const float f[4] = {f0.x, f0.y, f1.x, f1.y};
+#pragma unroll
+                for (int b = 0; b < 4; b++) {
+                    if (mine && (whole || c + b < nc)) *yp = f[b];
+                    yp += pitch;
+                }
+            }
+        } else {
+            const int ro = lane >> 2, co = (lane & 3) * 2;
+            const uint32_t to = staging + (lane & 7) * I8_ROW_PITCH +
+                                (SWIGLU ? (lane >> 3) & 1 : lane >> 3) * 16;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint64_t sx = ld_shared_u64(scales + (i * 8 + co) * 4);
+                float2 f[4];  // weight rows ro + 8e, a pair of rows each
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int *x = &v[e >> 1][i * 4 + (e & 1) * 2];
+                    f[e] = scaled(x[0], x[1], pack_f32x2(sw[e], sw[e]), sx);
+                }
+                if constexpr (SWIGLU) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        f[e].x = swiglu(f[e].x, f[2 + e].x);
+                        f[e].y = swiglu(f[e].y, f[2 + e].y);
+                    }
+                }
+                if constexpr (F32) {  // eight neighbouring channels of four rows per store
+                    const int c = i * 8 + co;
+#pragma unroll
+                    for (int e = 0; e < 2; e++)
+                        if (o0 + ro + 8 * e < a.cols) {
+                            if (c < nc) yp[8 * e] = f[e].x;
+                            if (c + 1 < nc) yp[pitch + 8 * e] = f[e].y;
+                        }
+                    yp += 8 * pitch;
+                } else {
+                    uint32_t p[4];
+#pragma unroll
+                    for (int e = 0; e < (SWIGLU ? 2 : 4); e++)
+                        p[e] = pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y);
+                    if constexpr (SWIGLU)
+                        stmatrix2_trans(to + i * 8 * I8_ROW_PITCH, p[0], p[1]);
+                    else
+                        stmatrix4_trans(to + i * 8 * I8_ROW_PITCH, p);
+                }
+            }
+            if constexpr (!F32) {
+                __syncwarp();
+                const uint32_t from =
+                    staging + (lane / CHUNKS) * I8_ROW_PITCH + (lane % CHUNKS) * 16;
+#pragma unroll
+                for (int p = 0; p < CHUNKS; p++) {
+                    const uint4 u = ld_shared_v4(from + p * ROWS * I8_ROW_PITCH);
+                    if (p * ROWS + lane / CHUNKS < nc) {
+                        const int o = o0 + lane % CHUNKS * 8;
+                        if (a.vec) {  // cols % 8 == 0: a chunk is inside or outside
+                            if (o < a.cols) *reinterpret_cast<uint4 *>(yp) = u;
+                        } else {
+                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                            for (int e = 0; e < 8; e++)
+                                if (o + e < a.cols)
+                                    reinterpret_cast<uint16_t *>(yp)[e] =
+                                        (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                        }
+                    }
+                    yp += ROWS * pitch;
+                }
+                __syncwarp();  // the staging is written again
+            }
+        }
+    }
+    // Where this thread's first store of a run that starts at y row r0 goes.
+    __device__ __forceinline__ TO *place(int64_t r0, int o0) const {
+        int row, col;
+        if constexpr (LANES) {
+            row = 0;
+            col = lane;
+        } else if constexpr (F32) {
+            row = (lane & 3) * 2;
+            col = lane >> 2;
+        } else {
+            row = lane / CHUNKS;
+            col = lane % CHUNKS * 8;
+        }
+        return static_cast<TO *>(a.y) + (r0 + row) * a.cols + o0 + col;
+    }
+
+    // tmem: the accumulator's first column in this warp's lane quarter.
+    // read() is called once the warp's columns have been read, before the last
+    // of them are converted.
+    template <typename F>
+    __device__ __forceinline__ void drain(uint32_t tmem, int64_t row0, int n, int rt, F read) {
+        const int o0 = (rt * 4 + q) * CH;
+        TO *yp = place(row0 + half * 32, o0);
+        int v[2][2][16];
+        if (half * 32 < n) fetch(tmem + half * 32, v[0]); else read();
+#pragma unroll
+        for (int i = 0; i < I8_RUNS; i++) {
+            const int c0 = half * 32 + i * 64;
+            if (c0 < n) {
+                tmem_wait_ld();
+                if (i + 1 < I8_RUNS && c0 + 64 < n) fetch(tmem + c0 + 64, v[(i + 1) & 1]); else read();
+                run(v[i & 1], staging + 32 * I8_ROW_PITCH + i * 128, yp, min(32, n - c0), o0);
+                yp += 64 * (int64_t)a.cols;
+            }
+        }
+        __syncwarp();  // the scales are written again
+    }
+};
+
+// ---- one CTA per tile ---------------------------------------------------------------
 template <int NT, typename TO, bool SWIGLU>
 __global__ void __launch_bounds__(I8_THREADS, 1)
 k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
@@ -146,7 +503,9 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     uint8_t *base = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES);
+    const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
+    uint64_t *full = reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES +
+                                                  I8_EPI_WARPS * I8_STAGING);
     uint64_t *empty = full + S;
     uint64_t *accFull = empty + S;     // [2]
     uint64_t *accEmpty = accFull + 2;  // [2]
@@ -175,39 +534,12 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         tmem_relinquish();
     }
     pdl_wait();
-    if (warp == 0) {  // row tiles before each group; a group whose range is not one has none
-        int total = 0;
-        for (int g0 = 0; g0 < a.G; g0 += 32) {
-            const int g = g0 + lane;
-            int n = 0;
-            if (g < a.G) {
-                if (a.offsets) {
-                    const int b = *(const volatile int32_t *)(a.offsets + g);
-                    const int e = *(const volatile int32_t *)(a.offsets + g + 1);
-                    if (b < 0 || e < b || e > a.R)
-                        atomicOr(a.err, QG_FLAG_BAD_GROUP);
-                    else
-                        n = e - b;
-                } else {
-                    n = a.R;
-                }
-            }
-            int t = (n + a.nt - 1) / a.nt, sum = t;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(~0u, sum, o);
-                if (lane >= o) sum += v;
-            }
-            if (g < a.G) prefix[g] = total + sum - t;
-            total += __shfl_sync(~0u, sum, 31);
-        }
-        if (lane == 0) prefix[a.G] = total;
-    }
+    if (warp == 0) i8_prefix(a, prefix, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int n_units = prefix[a.G] * a.RT;
+    const int n_units = prefix[a.G] * a.CT;
 
     auto fail = [&]() {
         if (!ld_volatile_shared(abort_addr)) {
@@ -218,14 +550,12 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     if (warp < I8_EPI_WARPS) {
         // ============ epilogue: TMEM -> scaled rows ===============================
-        // Warp w reads lane quarter w & 3; the two warps of a quarter take
-        // alternate runs of 32 row columns.
-        const int q = warp & 3, half = warp >> 2;
+        I8Epilogue<TO, SWIGLU> epi(a, warp, lane, staging + warp * I8_STAGING);
         int lt = 0;
         for (int u = blockIdx.x; u < n_units; u += gridDim.x, lt++) {
             const int buf = lt & 1;
             const I8Unit w = i8_unit(a, prefix, u);
-            const float sw = a.ws[((size_t)w.g * a.RT + w.rt) * I8_M + q * 32 + lane];
+            epi.prepare(a.ws + ((size_t)w.g * a.RT + w.ct) * I8_M + epi.q * 32, w.row0, w.n);
             // the lanes wait one by one and must leave the loop together
             if (!__all_sync(~0u, mbar_wait(&accFull[buf], (lt >> 1) & 1, abort_addr,
                                            I8_WAIT_CYCLES))) {
@@ -233,45 +563,11 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
                 break;
             }
             tc_fence_after();
-            for (int c0 = half * 32; c0 < w.n; c0 += 64) {
-                const int nc = min(32, w.n - c0);
-                const int64_t r0 = (int64_t)w.row0 + c0;
-                const float sx = lane < nc ? *(const volatile float *)(a.xs + r0 + lane) : 0.f;
-                float v[32];
-                tmem_ld32(tmem + buf * Cfg::BUF + c0 + ((uint32_t)(q * 32) << 16), v);
-#pragma unroll
-                for (int c = 0; c < 32; c++)
-                    // the row's scale last: it is as large as the activations
-                    // are, and the sum times it may overflow where y does not
-                    v[c] = (float)__float_as_int(v[c]) * sw * __shfl_sync(~0u, sx, c);
-                if constexpr (SWIGLU) {
-                    // lanes 0-15 hold gate rows, 16-31 the up rows of the same
-                    // columns: per two rows one exchange gives each half-warp
-                    // gate and up of one of them
-                    const int o = w.rt * 64 + q * 16 + (lane & 15);
-                    const bool up = lane >= 16;
-                    TO *yp = static_cast<TO *>(a.y) + r0 * a.cols + o;
-#pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float other = __shfl_xor_sync(~0u, up ? v[c] : v[c + 1], 16);
-                        const float h = up ? swiglu(other, v[c + 1]) : swiglu(v[c], other);
-                        const int cc = c + up;
-                        if (cc < nc && o < a.cols) i8_store(yp + (int64_t)cc * a.cols, h);
-                    }
-                } else {
-                    const int o = w.rt * I8_M + q * 32 + lane;
-                    TO *yp = static_cast<TO *>(a.y) + r0 * a.cols + o;
-                    if (o < a.cols) {
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (c < nc) i8_store(yp + (int64_t)c * a.cols, v[c]);
-                    }
-                }
+            epi.drain(tmem + buf * Cfg::BUF + ((uint32_t)(epi.q * 32) << 16), w.row0, w.n, w.ct, [&] {
+                tc_fence_before();
                 __syncwarp();
-            }
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&accEmpty[buf]);
+                if (lane == 0) mbar_arrive(&accEmpty[buf]);
+            });
         }
     } else if (warp == I8_LOAD_WARP) {
         // ============ loads: weight tile and row tile of each 128-code block ======
@@ -280,8 +576,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
             bool ok = true;
             for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
                 const I8Unit w = i8_unit(a, prefix, u);
-                const int wrow = (w.g * a.RT + w.rt) * I8_M;
-                const int boxes = (w.n + Cfg::BOX - 1) / Cfg::BOX;
+                const int wrow = (w.g * a.RT + w.ct) * I8_M;
                 for (int kb = 0; kb < a.KB; kb++, g++) {
                     const int s = g % S;
                     if (!mbar_wait(&empty[s], ((g / S) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
@@ -290,11 +585,9 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
                         break;
                     }
                     uint8_t *dst = base + s * Cfg::STAGE_BYTES;
-                    mbar_arrive_expect_tx(&full[s], Cfg::A_BYTES + boxes * Cfg::BOX * I8_BK);
+                    mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
                     tma_load_2d(dst, &tmap_w, kb * I8_BK, wrow, &full[s]);
-                    for (int b = 0; b < boxes; b++)
-                        tma_load_2d(dst + Cfg::A_BYTES + b * Cfg::BOX * I8_BK, &tmap_x, kb * I8_BK,
-                                    w.row0 + b * Cfg::BOX, &full[s]);
+                    tma_load_2d(dst + Cfg::A_BYTES, &tmap_x, kb * I8_BK, w.row0, &full[s]);
                 }
             }
             // our own copies land before the shared memory goes, also when
@@ -310,7 +603,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
             bool ok = true;
             for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x, lt++) {
                 const I8Unit w = i8_unit(a, prefix, u);
-                const uint32_t idesc = idesc_i8((w.n + 15) & ~15);
+                const uint32_t idesc = idesc_i8(I8_M, (w.n + 15) & ~15);
                 const int buf = lt & 1;
                 if (!mbar_wait(&accEmpty[buf], ((lt >> 1) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
                     fail();
@@ -347,6 +640,246 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::TMEM_COLS);
     }
+}
+
+// ---- a CTA pair per tile ---------------------------------------------------------------
+// CTA r of the pair holds weight rows [256 ct + 128 r, + 128) and, of each
+// part of N row codes, rows [r N/2, + N/2); CTA 0 issues the MMAs, which read
+// both CTAs' shared memory and leave each CTA its 128 channels of all rows.
+// All loads of a stage signal CTA 0's full barrier; commits signal both CTAs.
+//
+// A tile of two parts fills both accumulators, so the next tile's first part
+// can only start when its accumulator is drained.  To have MMAs to issue
+// meanwhile, the second part lags behind by I8P_STAGGER stages at the start of
+// a tile and catches up at its end: the first part's accumulator is complete,
+// and its drain begins, that much before the second's.
+__device__ __forceinline__ int i8p_first(int n) {  // rows of the first part
+    return n <= I8P_PART ? n : ((n + 1) / 2 + 31) & ~31;
+}
+
+template <typename TO, bool SWIGLU>
+__global__ void __launch_bounds__(I8_THREADS, 1)
+k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
+          const I8Args a) {
+    pdl_launch_dependents();
+    using Cfg = I8Pair;
+    constexpr int S = Cfg::S;
+    extern __shared__ uint8_t smem_raw[];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int first_unit = blockIdx.x >> 1, unit_step = gridDim.x >> 1;
+
+    uint8_t *base = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
+    uint64_t *full = reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES +
+                                                  I8_EPI_WARPS * I8_STAGING);
+    uint64_t *empty = full + S;
+    uint64_t *accFull = empty + S;     // [2]
+    uint64_t *accEmpty = accFull + 2;  // [2]
+    uint64_t *drain = accEmpty + 2;
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(drain + 1);
+    const uint32_t abort_addr = smem_u32(tmem_slot + 1);
+    int *prefix = reinterpret_cast<int *>(tmem_slot + 4);
+
+    if (tid == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int b = 0; b < 2; b++) {
+            mbar_init(&accFull[b], 1);
+            mbar_init(&accEmpty[b], 2 * I8_EPI_WARPS);  // both CTAs' epilogues
+        }
+        mbar_init(drain, 1);
+        st_volatile_shared(abort_addr, 0);
+        fence_mbar_init();
+        prefetch_tmap(&tmap_w);
+        prefetch_tmap(&tmap_x);
+    }
+    if (warp == I8_MMA_WARP) tmem_alloc2(tmem_slot, 512);
+    pdl_wait();
+    if (warp == 0) i8_prefix(a, prefix, lane);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();  // the other CTA's barriers are initialised
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int n_units = prefix[a.G] * a.CT;
+
+    auto fail = [&]() {
+        if (!ld_volatile_shared(abort_addr)) {
+            st_volatile_shared(abort_addr, 1);
+            atomicOr(a.err, QG_FLAG_TIMEOUT);
+        }
+    };
+
+    if (warp < I8_EPI_WARPS) {
+        // ============ epilogue of this CTA's 128 channels =========================
+        I8Epilogue<TO, SWIGLU> epi(a, warp, lane, staging + warp * I8_STAGING);
+        int sc = 0;  // accumulators used so far
+        bool ok = true;
+        for (int u = first_unit; u < n_units && ok; u += unit_step) {
+            const I8Unit w = i8_unit(a, prefix, u);
+            const int rt = w.ct * 2 + rank, n0 = i8p_first(w.n);
+            for (int p = 0; p < 2; p++) {
+                const int n = p ? w.n - n0 : n0;
+                if (n == 0) break;
+                const int buf = sc & 1;
+                const int64_t row0 = (int64_t)w.row0 + (p ? n0 : 0);
+                epi.prepare(a.ws + ((size_t)w.g * a.RT + rt) * I8_M + epi.q * 32, row0, n);
+                // the lanes wait one by one and must leave the loop together
+                if (!__all_sync(~0u, mbar_wait(&accFull[buf], (sc >> 1) & 1, abort_addr,
+                                               I8_WAIT_CYCLES))) {
+                    fail();
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+                epi.drain(tmem + buf * I8P_PART + ((uint32_t)(epi.q * 32) << 16), row0, n, rt,
+                          [&] {
+                              tc_fence_before();
+                              __syncwarp();
+                              if (lane == 0)
+                                  mbar_arrive_cluster(mapa_shared(smem_u32(&accEmpty[buf]), 0));
+                          });
+                sc++;
+            }
+        }
+    } else if (warp == I8_LOAD_WARP) {
+        // ============ this CTA's half of the loads ================================
+        if (lane == 0) {
+            int g = 0;
+            bool ok = true;
+            for (int u = first_unit; u < n_units && ok; u += unit_step) {
+                const I8Unit w = i8_unit(a, prefix, u);
+                const int wrow = (w.g * a.RT + w.ct * 2 + rank) * I8_M;
+                const int n0 = i8p_first(w.n), n1 = w.n - n0;
+                // half of each part's rows, and the boxes that cover them
+                const int h0 = ((n0 + 31) & ~31) / 2, h1 = ((n1 + 31) & ~31) / 2;
+                const int b0 = (h0 + I8P_BOX - 1) / I8P_BOX, b1 = (h1 + I8P_BOX - 1) / I8P_BOX;
+                const int r0 = w.row0 + rank * h0, r1 = w.row0 + n0 + rank * h1;
+                const uint32_t bytes = 2 * (Cfg::A_BYTES + (b0 + b1) * I8P_BOX * I8_BK);
+                for (int kb = 0; kb < a.KB; kb++, g++) {
+                    const int s = g % S;
+                    if (!mbar_wait(&empty[s], ((g / S) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
+                        fail();
+                        ok = false;
+                        break;
+                    }
+                    uint8_t *dst = base + s * Cfg::STAGE_BYTES, *dx = dst + Cfg::A_BYTES;
+                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
+                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
+                    const int x = kb * I8_BK;
+                    tma_load_2d_pair(dst, &tmap_w, x, wrow, bar);
+                    for (int b = 0; b < b0; b++)
+                        tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x, r0 + b * I8P_BOX,
+                                         bar);
+                    for (int b = 0; b < b1; b++)
+                        tma_load_2d_pair(dx + I8P_HALF_BYTES + b * I8P_BOX * I8_BK, &tmap_x, x,
+                                         r1 + b * I8P_BOX, bar);
+                }
+            }
+            // the pair's copies land before the shared memory goes: CTA 0 sees
+            // them on its barriers and CTA 1 leaves with it (below); when a
+            // role gave up, some may not be counted there, and both CTAs give
+            // them time
+            if (rank == 0)
+                for (int i = g > S ? g - S : 0; i < g; i++)
+                    mbar_wait(&full[i % S], (i / S) & 1, abort_addr, I8_WAIT_CYCLES);
+            if (!ok || ld_volatile_shared(abort_addr)) {
+                const long long t0 = clock64();
+                while (clock64() - t0 < 1000000) {
+                }
+            }
+        }
+        __syncwarp();
+    } else if (rank == 0) {
+        // ============ MMA issuer of the pair ======================================
+        if (lane == 0) {
+            int g = 0, sc = 0;
+            bool ok = true;
+            auto wait_stage = [&](int i) {
+                if (mbar_wait(&full[i % S], (i / S) & 1, abort_addr, I8_WAIT_CYCLES)) {
+                    tc_fence_after();
+                    return true;
+                }
+                return false;
+            };
+            auto wait_acc = [&](int i) {
+                if (mbar_wait(&accEmpty[i & 1], ((i >> 1) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
+                    tc_fence_after();
+                    return true;
+                }
+                return false;
+            };
+            for (int u = first_unit; u < n_units && ok; u += unit_step) {
+                const I8Unit w = i8_unit(a, prefix, u);
+                const int n0 = i8p_first(w.n), n1 = w.n - n0;
+                const uint32_t id0 = idesc_i8(2 * I8_M, (n0 + 31) & ~31);
+                const uint32_t id1 = idesc_i8(2 * I8_M, (n1 + 31) & ~31);
+                auto part = [&](int p, int kb) {
+                    const uint32_t st = smem_u32(base + ((g + kb) % S) * Cfg::STAGE_BYTES);
+                    umma2_i8_k128(tmem + ((sc + p) & 1) * I8P_PART, desc_k_sw128(st),
+                                  desc_k_sw128(st + Cfg::A_BYTES + p * I8P_HALF_BYTES),
+                                  p ? id1 : id0, kb != 0);
+                };
+                ok = wait_acc(sc);
+                if (n1 == 0) {
+                    for (int kb = 0; kb < a.KB && ok; kb++) {
+                        if (!(ok = wait_stage(g + kb))) break;
+                        part(0, kb);
+                        umma2_commit(&empty[(g + kb) % S]);
+                    }
+                    if (ok) umma2_commit(&accFull[sc & 1]);
+                    sc++;
+                } else {
+                    // blocks [0, head): the first part alone, then the second;
+                    // the middle ones together; [tail, KB) as the first ones
+                    const int head = min(I8P_STAGGER, a.KB);
+                    const int tail = max(head, a.KB - I8P_STAGGER);
+                    for (int kb = 0; kb < head && ok; kb++)
+                        if ((ok = wait_stage(g + kb))) part(0, kb);
+                    if (ok && head == a.KB) umma2_commit(&accFull[sc & 1]);
+                    ok = ok && wait_acc(sc + 1);
+                    for (int kb = 0; kb < head && ok; kb++) {
+                        part(1, kb);
+                        umma2_commit(&empty[(g + kb) % S]);
+                    }
+                    for (int kb = head; kb < tail && ok; kb++) {
+                        if (!(ok = wait_stage(g + kb))) break;
+                        part(0, kb);
+                        part(1, kb);
+                        umma2_commit(&empty[(g + kb) % S]);
+                    }
+                    for (int kb = tail; kb < a.KB && ok; kb++)
+                        if ((ok = wait_stage(g + kb))) part(0, kb);
+                    if (ok && tail < a.KB) umma2_commit(&accFull[sc & 1]);
+                    for (int kb = tail; kb < a.KB && ok; kb++) {
+                        part(1, kb);
+                        umma2_commit(&empty[(g + kb) % S]);
+                    }
+                    if (ok) umma2_commit(&accFull[(sc + 1) & 1]);
+                    sc += 2;
+                }
+                g += a.KB;
+            }
+            if (!ok) {
+                fail();
+                umma2_commit(drain);
+                mbar_wait(drain, 0, 0, I8_WAIT_CYCLES);
+            }
+        }
+        __syncwarp();
+    }
+
+    // both CTAs stay until the pair's MMAs, loads and arrivals are through
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    if (warp == I8_MMA_WARP) tmem_dealloc2(tmem, 512);
+    cluster_sync();
 }
 
 // ---- weight layout -------------------------------------------------------------
@@ -436,7 +969,8 @@ using namespace qg;
 
 struct qgq8 {
     int device = 0;
-    int G = 0, O = 0, I = 0, cols = 0, RT = 0, KB = 0;
+    int G = 0, O = 0, I = 0, cols = 0, KB = 0;
+    int RT = 0, live = 0;  // 128-row weight tiles per group, and those that hold channels
     bool swiglu = false;
     cudaStream_t stream = nullptr;
     int8_t *w = nullptr;   // [G * RT * 128, ldw]
@@ -454,14 +988,48 @@ namespace qg {
 static int64_t i8_pitch(int64_t I) { return (I + 15) & ~int64_t(15); }
 
 // Most rows of a tile.  Short tiles for few rows per group (the stages then
-// hold mostly weights), 256 for prompts.
+// hold mostly weights), CTA pairs for prompts.
 static int i8_tile(int64_t rows_per_group) {
-    return rows_per_group <= 16 ? 16 : rows_per_group <= 64 ? 64 : 256;
+    return rows_per_group <= 16 ? 16 : rows_per_group <= 64 ? 64 : I8P_NT;
+}
+
+template <typename TO, bool SWIGLU>
+static int launch_i8_pair_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
+                            cudaStream_t s) {
+    auto kern = k_i8_pair<TO, SWIGLU>;
+    constexpr int smem = I8Pair::SMEM;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeClusterDimension;  // the pair lies along x
+    at[0].val.clusterDim.x = 2;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_pdl
+    at[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.gridDim = dim3(2);
+    cfg.blockDim = dim3(I8_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    // pairs that fit the device at once: SMs come in pairs, but not every
+    // device enables both SMs of each
+    static int pairs[64] = {0};
+    int n = h->device < 64 ? pairs[h->device] : 0;
+    if (!n) {
+        QG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        QG_CUDA(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+        if (n < 1) return set_error(QGMOE_ERR_CUDA, "no room for a CTA pair");
+        if (h->device < 64) pairs[h->device] = n;
+    }
+    cfg.gridDim = dim3(2 * (unsigned)(max_units < n ? max_units : n));
+    cfg.numAttrs = 2;
+    QG_CUDA(cudaLaunchKernelEx(&cfg, kern, h->tmap_w, tx, a));
+    return QGMOE_OK;
 }
 
 template <int NT, typename TO, bool SWIGLU>
-static int launch_i8_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
-                       cudaStream_t s) {
+static int launch_i8_cta_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a,
+                           int64_t max_units, cudaStream_t s) {
     auto kern = k_i8<NT, TO, SWIGLU>;
     constexpr int smem = I8Cfg<NT>::SMEM;
     static bool done[64] = {false};
@@ -473,6 +1041,15 @@ static int launch_i8_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, in
     if (max_units < grid) grid = max_units;
     QG_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8_THREADS), smem, s, 1, h->tmap_w, tx, a));
     return QGMOE_OK;
+}
+
+template <int NT, typename TO, bool SWIGLU>
+static int launch_i8_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
+                       cudaStream_t s) {
+    if constexpr (NT == I8P_NT)
+        return launch_i8_pair_t<TO, SWIGLU>(h, tx, a, max_units, s);
+    else
+        return launch_i8_cta_t<NT, TO, SWIGLU>(h, tx, a, max_units, s);
 }
 
 template <int NT>
@@ -511,7 +1088,7 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     const int64_t per = (R + (int64_t)h->G - 1) / h->G;  // mean rows of a group
     const int nt = i8_tile(per);
     CUtensorMap tx;
-    int rc = i8_encode_map(&tx, codes, R, h->I, ld, nt < 64 ? nt : 64);
+    int rc = i8_encode_map(&tx, codes, R, h->I, ld, nt < I8P_BOX ? nt : I8P_BOX);
     if (rc) return rc;
     I8Args a{};
     a.xs = scale;
@@ -522,15 +1099,19 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     a.RT = h->RT;
     a.KB = h->KB;
     a.cols = h->cols;
+    const bool pair = nt == I8P_NT;
+    a.CT = pair ? h->RT / 2 : h->live;
     a.nt = nt;
+    a.gran = pair ? 32 : 16;
     a.y = y;
+    a.vec = h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
     a.err = h->err_dev;
     // row tiles: full ones, and at most one partial for each group that has rows
     const int64_t tiles = R / nt + (R < h->G ? R : h->G);
-    const int64_t units = tiles * h->RT;
+    const int64_t units = tiles * a.CT;
     return nt == 16   ? launch_i8<16>(h, tx, a, ydt, units, s)
            : nt == 64 ? launch_i8<64>(h, tx, a, ydt, units, s)
-                      : launch_i8<256>(h, tx, a, ydt, units, s);
+                      : launch_i8<I8P_NT>(h, tx, a, ydt, units, s);
 }
 
 static void i8_free_work(qgq8 *h) {
@@ -612,7 +1193,7 @@ int qgq8_create(int32_t groups, int32_t O, int32_t I, const int8_t *q, const flo
     if (swiglu && O % 2)
         return set_error(QGMOE_ERR_INVALID_ARG, "SwiGLU needs gate and up rows: out=%d is odd", O);
     const int64_t cols = swiglu ? O / 2 : O, per = swiglu ? 64 : I8_M;
-    const int64_t RT = (cols + per - 1) / per;
+    const int64_t RT = (cols + 2 * per - 1) / (2 * per) * 2;  // whole CTA pairs
     if (RT * groups * I8_M > INT32_MAX)
         return set_error(QGMOE_ERR_INVALID_ARG, "groups=%d x out=%d is too many rows", groups, O);
     if (!q || !scale) return set_error(QGMOE_ERR_INVALID_ARG, "null weights");
@@ -627,6 +1208,7 @@ int qgq8_create(int32_t groups, int32_t O, int32_t I, const int8_t *q, const flo
     h->I = I;
     h->cols = (int)cols;
     h->RT = (int)RT;
+    h->live = (int)((cols + per - 1) / per);
     h->KB = (I + I8_BK - 1) / I8_BK;
     h->swiglu = swiglu != 0;
     int rc = QGMOE_OK;

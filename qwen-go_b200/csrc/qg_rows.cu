@@ -20,6 +20,7 @@
 #include <math_constants.h>
 
 #include "qg_common.cuh"
+#include "qg_sm100.cuh"
 
 namespace qg {
 
@@ -124,107 +125,146 @@ template <> struct Vec8<float> {  // two 16-byte loads
 };
 
 // ---- sort -------------------------------------------------------------------
-// One CTA per expert e: it reads every pair's expert once to count the pairs
-// before its range (e_p < e) and its own, and once more to give its own their
-// rows.  No workspace, no atomics, one launch; the order within an expert is
-// the pairs' own.  Each warp owns a contiguous range of pairs, so that its
-// rows follow those of the warps below it.
+// One cluster of up to eight CTAs, no workspace, one launch.  Each warp owns a
+// contiguous range of pairs and takes it 32 at a time: lanes with the same
+// expert find each other (match), rank themselves in lane order on top of the
+// warp's count of that expert so far, and the first adds their number to the
+// count.  The counts of the CTA's warps, then of the cluster's CTAs
+// (distributed shared memory), then of the experts are summed in order; a
+// pair's row is the three prefixes and its rank.  The order within an expert
+// is the pairs' own by construction; no atomics.
+// Every id is handled once: 32768 pairs over 128 experts take 5 us, where one
+// CTA per expert, each counting all pairs, took 12.
 constexpr int SORT_MAX_WARPS = 32;
+constexpr int SORT_STEPS = 4;  // steps of 32 whose loads are in flight together
 
-struct Ids4 {
-    int v[4];
-};
-__device__ __forceinline__ Ids4 load_ids(const int32_t *ids, int64_t i, int64_t hi, bool vec) {
-    Ids4 r;
-    if (vec && i + 4 <= hi) {
-        uint4 u;
-        asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
-                     : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
-                     : "l"(ids + i)
-                     : "memory");
-        r.v[0] = (int)u.x, r.v[1] = (int)u.y, r.v[2] = (int)u.z, r.v[3] = (int)u.w;
-    } else {
-#pragma unroll
-        for (int s = 0; s < 4; s++) r.v[s] = i + s < hi ? ld_i32(ids + i + s) : -1;
-    }
-    return r;
+__device__ __forceinline__ int ld_i32_if(bool on, const int32_t *p, int other) {
+    int v;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %3, 0;\n\tmov.b32 %0, %2;\n\t"
+        "@p ld.global.b32 %0, [%1];\n\t}"
+        : "=&r"(v)
+        : "l"(p), "r"(other), "r"((int)on)
+        : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
+    int v;
+    asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
 }
 
-__global__ void k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets,
-                              int32_t *pair_row, int32_t *row_pair) {
-    __shared__ int s_less[SORT_MAX_WARPS], s_eq[SORT_MAX_WARPS], s_valid[SORT_MAX_WARPS];
+__global__ void __launch_bounds__(SORT_MAX_WARPS * 32)
+k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_row,
+              int32_t *row_pair) {
+    extern __shared__ int sort_smem[];
     pdl_enter();
-    const int e = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int nw = blockDim.x >> 5;
-    const bool vec = (reinterpret_cast<uintptr_t>(ids) & 15) == 0;
-    int64_t per = ((int64_t)N + nw - 1) / nw;
-    per = (per + 127) & ~int64_t(127);
-    const int64_t lo = per * warp, hi = min((int64_t)N, lo + per);
-    int less = 0, eq = 0, valid = 0;
-    for (int64_t i = lo + lane * 4; i < hi; i += 128) {
-        const Ids4 d = load_ids(ids, i, hi, vec);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int C = gridDim.z, rank = blockIdx.z;  // the grid is the cluster
+    int *hist = sort_smem;        // [nw][E]: counts, then the warps before
+    int *tot = hist + nw * E;     // [E] this CTA's counts
+    int *base = tot + E;          // [E + 1] counts of all, then first rows
+    int *mine = hist + warp * E;
+    int64_t per = ((int64_t)N + C * nw - 1) / (C * nw);
+    per = (per + 31) & ~int64_t(31);
+    const int64_t lo = min((int64_t)N, per * (rank * nw + warp)), hi = min((int64_t)N, lo + per);
+    const bool kept = per <= SORT_STEPS * 32;  // one round: ids and ranks stay in registers
+    const unsigned below = (1u << lane) - 1;
+    for (int e = lane; e < E; e += 32) mine[e] = 0;
+    __syncwarp();
+
+    int id[SORT_STEPS], rk[SORT_STEPS];
+    for (int64_t i0 = lo; i0 < hi; i0 += SORT_STEPS * 32) {
 #pragma unroll
-        for (int s = 0; s < 4; s++) {
-            less += (unsigned)d.v[s] < (unsigned)e;
-            eq += d.v[s] == e;
-            valid += (unsigned)d.v[s] < (unsigned)E;
+        for (int b = 0; b < SORT_STEPS; b++) {
+            const int64_t i = i0 + b * 32 + lane;
+            id[b] = ld_i32_if(i < hi, ids + i, -1);
         }
-    }
-    less = __reduce_add_sync(~0u, less);
-    eq = __reduce_add_sync(~0u, eq);
-    valid = __reduce_add_sync(~0u, valid);
-    if (lane == 0) {
-        s_less[warp] = less;
-        s_eq[warp] = eq;
-        s_valid[warp] = valid;
+#pragma unroll
+        for (int b = 0; b < SORT_STEPS; b++) {
+            const int64_t i = i0 + b * 32 + lane;
+            const bool valid = (unsigned)id[b] < (unsigned)E;
+            const unsigned peers = __match_any_sync(~0u, valid ? id[b] : -1);
+            const int ahead = __popc(peers & below);
+            const int so_far = valid ? mine[id[b]] : 0;
+            __syncwarp();
+            if (valid && ahead == 0) mine[id[b]] = so_far + __popc(peers);
+            __syncwarp();
+            rk[b] = so_far + ahead;
+            if (!kept && i < hi) pair_row[i] = rk[b];  // read back below by this thread
+        }
     }
     __syncthreads();
-    const int l = lane < nw ? s_less[lane] : 0;
-    const int q = lane < nw ? s_eq[lane] : 0;
-    const int start = __reduce_add_sync(~0u, l);
-    const int mine = __reduce_add_sync(~0u, q);
-    int row = start + __reduce_add_sync(~0u, lane < warp ? q : 0);
-    if (threadIdx.x == 0) {
-        offsets[e] = start;
-        if (e == E - 1) offsets[E] = start + mine;
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+        int sum = 0;
+#pragma unroll 8
+        for (int w = 0; w < nw; w++) {
+            const int v = hist[w * E + e];
+            hist[w * E + e] = sum;
+            sum += v;
+        }
+        tot[e] = sum;
     }
-    const unsigned below = (1u << lane) - 1;
-    for (int64_t i0 = lo; i0 < hi; i0 += 128) {
-        const int64_t i = i0 + lane * 4;
-        Ids4 d;
-        if (i < hi) {
-            d = load_ids(ids, i, hi, vec);
-        } else {
-            d.v[0] = d.v[1] = d.v[2] = d.v[3] = -1;
-        }
-        if (e == 0) {  // pairs without an expert
-#pragma unroll
-            for (int s = 0; s < 4; s++)
-                if (i + s < hi && (unsigned)d.v[s] >= (unsigned)E) pair_row[i + s] = -1;
-        }
-        unsigned m[4];
+    if (C > 1) sm100::cluster_sync(); else __syncthreads();
+    // counts of all CTAs to base, those of the CTAs before this one to tot
+    for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int before = 0, all = 0;
-#pragma unroll
-        for (int s = 0; s < 4; s++) {
-            m[s] = __ballot_sync(~0u, d.v[s] == e);
-            before += __popc(m[s] & below);
-            all += __popc(m[s]);
+        for (int c = 0; c < C; c++) {
+            const int v =
+                C > 1 ? ld_cluster_i32(sm100::mapa_shared(sm100::smem_u32(tot + e), c)) : tot[e];
+            if (c == rank) before = all;
+            all += v;
         }
-        int r = row + before;
+        base[e] = all;
+        // tot itself is still read by the other CTAs: hist's first row, whose
+        // values are all zero, takes the sum
+        hist[e] = before;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int sum = 0;
+        for (int e0 = 0; e0 < E; e0 += 32) {
+            const int e = e0 + lane, v = e < E ? base[e] : 0;
+            int x = v;
 #pragma unroll
-        for (int s = 0; s < 4; s++)
-            if (d.v[s] == e) {
-                pair_row[i + s] = r;
-                if (row_pair) row_pair[r] = (int)(i + s);
-                r++;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, x, o);
+                if (lane >= o) x += y;
             }
-        row += all;
+            if (e < E) base[e] = sum + x - v;
+            sum += __shfl_sync(~0u, x, 31);
+        }
+        if (lane == 0) base[E] = sum;
     }
-    if (e == 0 && row_pair) {  // rows without a pair
-        int total = 0;
-        for (int w = 0; w < nw; w++) total += s_valid[w];
-        for (int64_t i = total + (int64_t)threadIdx.x; i < N; i += blockDim.x) row_pair[i] = -1;
+    __syncthreads();
+    for (int64_t i0 = lo; i0 < hi; i0 += SORT_STEPS * 32) {
+        if (!kept) {
+#pragma unroll
+            for (int b = 0; b < SORT_STEPS; b++) {
+                const int64_t i = i0 + b * 32 + lane;
+                id[b] = ld_i32_if(i < hi, ids + i, -1);
+                rk[b] = ld_i32_if(i < hi, pair_row + i, 0);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < SORT_STEPS; b++) {
+            const int64_t i = i0 + b * 32 + lane;
+            if (i >= hi) continue;
+            int row = -1;
+            if ((unsigned)id[b] < (unsigned)E) {
+                row = base[id[b]] + hist[id[b]] + (warp ? mine[id[b]] : 0) + rk[b];
+                if (row_pair) row_pair[row] = (int)i;
+            }
+            pair_row[i] = row;
+        }
     }
+    const int total = base[E];
+    const int64_t t0 = (int64_t)rank * blockDim.x + threadIdx.x;
+    if (rank == 0)
+        for (int e = threadIdx.x; e <= E; e += blockDim.x) offsets[e] = base[e];
+    if (row_pair)  // rows without a pair
+        for (int64_t i = total + t0; i < N; i += (int64_t)C * blockDim.x) row_pair[i] = -1;
+    if (C > 1) sm100::cluster_sync();  // the other CTAs have read tot
 }
 
 // ---- gather -------------------------------------------------------------------
@@ -379,124 +419,190 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
 // scale = max(amax / 127, 1e-8), code = clamp(round_half_away(x / scale)),
 // the rule of quantizeInt8 (model/moe.go:165-188) with the whole row as the
 // group and an IEEE float32 quotient.  A row that holds an infinity or NaN has
-// scale NaN and codes 0, so that what is computed from it is NaN.  One CTA per
-// row; the row stays in registers between the maximum and the codes up to
-// CH * 8 values a thread, longer rows are read twice.  With pair_row, row t
-// goes to the k rows of its pairs.
-constexpr int QR_THREADS = 256;
+// scale NaN and codes 0, so that what is computed from it is NaN.  With
+// pair_row, row t goes to the k rows of its pairs.
+//
+// The quotient is formed as x * (1 / scale), within 2^-22 |q| < 4e-5 of the
+// exact one, and rounded by adding 1.5 * 2^23, which leaves the code in the
+// low byte.  Only where that lands within 1e-4 of a half, where the exact
+// quotient might round the other way, the eight values are divided (the test
+// is one maximum over them).  Five operations a value instead of some twenty:
+// 4096 rows of 2048 went from 14.8 us to the time of their bytes.
+//
+// A row belongs to `wpr` warps of a CTA.  It is copied to shared memory
+// asynchronously and read there twice, each thread the vectors it copied
+// itself, which keeps the code small and the registers few: a row per warp and
+// seven CTAs' rows in flight on an SM.  Rows beyond QR_ROW_BYTES are read from
+// memory twice (k_quantize_long).
+constexpr int QR_WARPS = 8;
+constexpr int QR_THREADS = QR_WARPS * 32;
+constexpr int QR_ROW_BYTES = 32 * 1024;
 
-__device__ __forceinline__ float amax_or_inf(float m, float v) {
-    const float a = fabsf(v);
-    return a <= FLT_MAX ? fmaxf(m, a) : CUDART_INF_F;
-}
 __device__ __forceinline__ uint32_t code_of(float v, float s) {
     const float q = fminf(fmaxf(roundf(__fdiv_rn(v, s)), -127.f), 127.f);
     return (uint32_t)(int)q & 0xFFu;
 }
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+__device__ __noinline__ uint32_t codes_exact(float a, float b, float c, float d, float s) {
+    return pack4(code_of(a, s), code_of(b, s), code_of(c, s), code_of(d, s));
+}
+// Largest magnitude as float bits (exponent all ones: infinity or NaN).
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
+template <typename T> __device__ __forceinline__ void fold_max(uint32_t &m, const Vec8<T> &x) {
+    float v[8];
+    x.get(v);
+#pragma unroll
+    for (int q = 0; q < 8; q++) m = max(m, abs_bits(v[q]));
+}
+__device__ __forceinline__ float scale_of(uint32_t m) {
+    return fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), 1e-8f);
+}
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
+    constexpr float MAGIC = 12582912.f;
+    uint32_t c[8];
+    float far = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; q++) {
+        const float t = __fmul_rn(v[q], inv);
+        const float r = __fadd_rn(t, MAGIC);
+        far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(r, MAGIC))));
+        c[q] = __float_as_uint(r);
+    }
+    if (far > 0.4999f)
+        return make_uint2(codes_exact(v[0], v[1], v[2], v[3], s),
+                          codes_exact(v[4], v[5], v[6], v[7], s));
+    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+template <typename T> __device__ __forceinline__ void ld_shared_vec8(uint32_t addr, Vec8<T> &v) {
+    if constexpr (sizeof(T) == 4) {
+        v.a = sm100::ld_shared_v4(addr);
+        v.b = sm100::ld_shared_v4(addr + 16);
+    } else {
+        v.r = sm100::ld_shared_v4(addr);
+    }
+}
 
-template <typename TI, bool VEC, int CH>
+template <typename TI>
 __global__ void __launch_bounds__(QR_THREADS)
-k_quantize_rows(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_t *codes,
+k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t *pair_row,
+                int8_t *codes, int64_t ld, float *scale) {
+    extern __shared__ __align__(16) unsigned char qr_smem[];
+    __shared__ uint32_t s_max[QR_WARPS];
+    pdl_enter();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int part = warp % wpr, span = wpr * 256, in_cta = warp / wpr;
+    const int64_t t = (int64_t)blockIdx.x * (QR_WARPS / wpr) + in_cta;
+    const bool on = t < T;
+    const TI *src = x + t * K;
+    const int c0 = (part * 32 + lane) * 8;
+    const uint32_t row = sm100::smem_u32(qr_smem) + in_cta * K * (int)sizeof(TI);
+    if (on)
+        for (int c = c0; c < K; c += span) {
+            cp_async16(row + c * sizeof(TI), src + c);
+            if (sizeof(TI) == 4) cp_async16(row + c * sizeof(TI) + 16, src + c + 4);
+        }
+    // destination rows, lane j the j-th of this run of up to 32
+    const int n_dst = pair_row ? k : 1;
+    int dst = -1;
+    if (on && lane < n_dst) dst = pair_row ? ld_i32(pair_row + t * k + lane) : (int)t;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    uint32_t m = 0;
+    if (on)
+#pragma unroll 2
+        for (int c = c0; c < K; c += span) {
+            Vec8<TI> in;
+            ld_shared_vec8(row + c * (int)sizeof(TI), in);
+            fold_max(m, in);
+        }
+    m = __reduce_max_sync(~0u, m);
+    if (wpr > 1) {
+        if (lane == 0) s_max[warp] = m;
+        __syncthreads();
+        for (int w = 0; w < wpr; w++) m = max(m, s_max[warp - part + w]);
+    }
+    if (!on) return;
+    const bool bad = m >= 0x7F800000u;
+    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
+    for (int j0 = 0; j0 < n_dst; j0 += 32) {
+        if (j0) dst = j0 + lane < n_dst ? ld_i32(pair_row + t * k + j0 + lane) : -1;
+        const int n = min(32, n_dst - j0);
+        if (part == 0 && lane < n && (unsigned)dst < (unsigned)N)
+            scale[dst] = bad ? CUDART_NAN_F : s;
+        for (int c = c0; c - lane * 8 < K; c += span) {  // whole warps: the rows are shuffled
+            uint2 u = make_uint2(0, 0);
+            if (c < K && !bad) {
+                Vec8<TI> in;
+                float v[8];
+                ld_shared_vec8(row + c * (int)sizeof(TI), in);
+                in.get(v);
+                u = codes_of(v, s, inv);
+            }
+#pragma unroll 4
+            for (int j = 0; j < n; j++) {
+                const int r = __shfl_sync(~0u, dst, j);
+                if ((unsigned)r < (unsigned)N && c < K)
+                    *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = u;
+            }
+        }
+    }
+}
+
+// One CTA per row, read twice: rows longer than the registers hold, and rows
+// that are not 16-byte aligned or no multiple of 8 (VEC false).
+template <typename TI, bool VEC>
+__global__ void __launch_bounds__(QR_THREADS)
+k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_t *codes,
                 int64_t ld, float *scale) {
-    __shared__ float s_max[QR_THREADS / 32];
+    __shared__ uint32_t s_max[QR_WARPS];
     pdl_enter();
     const int64_t t = blockIdx.x;
     const int tid = threadIdx.x, nt = blockDim.x;
     const TI *src = x + t * K;
-    float m = 0.f;
-    Vec8<TI> keep[CH > 0 ? CH : 1];
-    if constexpr (VEC && CH > 0) {
-#pragma unroll
-        for (int h = 0; h < CH; h++) {
-            const int c = (h * nt + tid) * 8;
-            keep[h].zero();
-            if (c < K) keep[h].load(src + c);
-        }
-#pragma unroll
-        for (int h = 0; h < CH; h++) {
-            float v[8];
-            keep[h].get(v);
-#pragma unroll
-            for (int q = 0; q < 8; q++) m = amax_or_inf(m, v[q]);
-        }
-    } else if constexpr (VEC) {
+    uint32_t m = 0;
+    if constexpr (VEC) {
+#pragma unroll 4
         for (int c = tid * 8; c < K; c += nt * 8) {
             Vec8<TI> in;
-            float v[8];
             in.load(src + c);
-            in.get(v);
-#pragma unroll
-            for (int q = 0; q < 8; q++) m = amax_or_inf(m, v[q]);
+            fold_max(m, in);
         }
     } else {
-        for (int c = tid; c < K; c += nt) m = amax_or_inf(m, Elem<TI>::load(src + c));
+#pragma unroll 4
+        for (int c = tid; c < K; c += nt) m = max(m, abs_bits(Elem<TI>::load(src + c)));
     }
-#pragma unroll
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, o));
+    m = __reduce_max_sync(~0u, m);
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
-    m = s_max[0];
-    for (int w = 1; w < nt >> 5; w++) m = fmaxf(m, s_max[w]);
-    const bool bad = m > FLT_MAX;
-    const float s = bad ? 1.f : fmaxf(__fdiv_rn(m, 127.f), 1e-8f);
-
+    for (int w = 0; w < nt >> 5; w++) m = max(m, s_max[w]);
+    const bool bad = m >= 0x7F800000u;
+    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
     const int n_dst = pair_row ? k : 1;
-    auto dst_row = [&](int j) -> int {
-        if (!pair_row) return (int)t;
-        return ld_i32(pair_row + t * k + j);
-    };
-    if (tid < n_dst) {
-        for (int j = tid; j < n_dst; j += nt) {
-            const int r = dst_row(j);
-            if ((unsigned)r < (unsigned)N) scale[r] = bad ? CUDART_NAN_F : s;
-        }
+    auto dst_row = [&](int j) { return pair_row ? ld_i32(pair_row + t * k + j) : (int)t; };
+    for (int j = tid; j < n_dst; j += nt) {
+        const int r = dst_row(j);
+        if ((unsigned)r < (unsigned)N) scale[r] = bad ? CUDART_NAN_F : s;
     }
-    auto emit8 = [&](int c, const float (&v)[8]) {
-        uint32_t lo = 0, hi = 0;
-        if (!bad) {
+    // ld is a multiple of 16, so a store of 8 that ends past K stays in the row
+    for (int c = tid * 8; c < K; c += nt * 8) {
+        float v[8];
+        if constexpr (VEC) {
+            Vec8<TI> in;
+            in.load(src + c);
+            in.get(v);
+        } else {
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-                lo |= code_of(v[q], s) << (8 * q);
-                hi |= code_of(v[4 + q], s) << (8 * q);
-            }
+            for (int q = 0; q < 8; q++) v[q] = c + q < K ? Elem<TI>::load(src + c + q) : 0.f;
         }
+        const uint2 u = bad ? make_uint2(0, 0) : codes_of(v, s, inv);
         for (int j = 0; j < n_dst; j++) {
             const int r = dst_row(j);
             if ((unsigned)r < (unsigned)N)
-                *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = make_uint2(lo, hi);
-        }
-    };
-    if constexpr (VEC && CH > 0) {
-#pragma unroll
-        for (int h = 0; h < CH; h++) {
-            const int c = (h * nt + tid) * 8;
-            if (c < K) {
-                float v[8];
-                keep[h].get(v);
-                emit8(c, v);
-            }
-        }
-    } else if constexpr (VEC) {
-        for (int c = tid * 8; c < K; c += nt * 8) {
-            Vec8<TI> in;
-            float v[8];
-            in.load(src + c);
-            in.get(v);
-            emit8(c, v);
-        }
-    } else {
-        // four codes a store; ld is a multiple of 16, so the store that ends
-        // past K stays in the row
-        for (int c = tid * 4; c < K; c += nt * 4) {
-            uint32_t u = 0;
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                if (!bad && c + q < K) u |= code_of(Elem<TI>::load(src + c + q), s) << (8 * q);
-            for (int j = 0; j < n_dst; j++) {
-                const int r = dst_row(j);
-                if ((unsigned)r < (unsigned)N)
-                    *reinterpret_cast<uint32_t *>(codes + (int64_t)r * ld + c) = u;
-            }
+                *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = u;
         }
     }
 }
@@ -563,19 +669,28 @@ static int launch_combine_rows(const void *rows, int rdt, const float *w, int T,
 int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32_t *pair_row,
                          int8_t *codes, int64_t ld, float *scale, cudaStream_t s) {
     const bool vec = K % 8 == 0 && aligned16(x);
-    int th = (((vec ? K / 8 : (K + 3) / 4) + 31) / 32) * 32;
-    if (th > QR_THREADS) th = QR_THREADS;
-    const int per = th * 8;
     const int N = pair_row ? T * k : T;
+    const int row_bytes = K * (dt == QGMOE_DT_F32 ? 4 : 2);
+    // Many rows: a warp per row (no barrier); few rows: up to eight warps, for
+    // latency.
+    int wpr = T < 1024 ? QR_WARPS : 1;
+    while (wpr > 1 && K <= wpr / 2 * 256) wpr /= 2;
+    while (wpr < QR_WARPS && QR_WARPS / wpr * (int64_t)row_bytes > QR_ROW_BYTES) wpr *= 2;
+    const int rows = QR_WARPS / wpr;
     return with_dtype(dt, [&](auto *ip) {
         using TI = std::remove_pointer_t<decltype(ip)>;
-        auto kern = !vec           ? k_quantize_rows<TI, false, 0>
-                    : K <= per     ? k_quantize_rows<TI, true, 1>
-                    : K <= 2 * per ? k_quantize_rows<TI, true, 2>
-                    : K <= 4 * per ? k_quantize_rows<TI, true, 4>
-                                   : k_quantize_rows<TI, true, 0>;
-        QG_CUDA(launch_pdl(kern, dim3((unsigned)T), dim3(th), 0, s, 1, static_cast<const TI *>(x),
-                           k, K, N, pair_row, codes, ld, scale));
+        if (!vec || rows * (int64_t)row_bytes > QR_ROW_BYTES) {
+            auto kern = vec ? k_quantize_long<TI, true> : k_quantize_long<TI, false>;
+            int th = ((K + 7) / 8 + 31) / 32 * 32;
+            if (th > QR_THREADS) th = QR_THREADS;
+            QG_CUDA(launch_pdl(kern, dim3((unsigned)T), dim3(th), 0, s, 1,
+                               static_cast<const TI *>(x), k, K, N, pair_row, codes, ld, scale));
+            return (int)QGMOE_OK;
+        }
+        QG_CUDA(launch_pdl(k_quantize_rows<TI>, dim3((unsigned)((T + (int64_t)rows - 1) / rows)),
+                           dim3(QR_THREADS), (size_t)(rows * row_bytes), s, 1,
+                           static_cast<const TI *>(x), T, k, K, N, wpr, pair_row, codes, ld,
+                           scale));
         return (int)QGMOE_OK;
     });
 }
@@ -613,12 +728,20 @@ int qgmoe_sort_tokens(const int32_t *sel_idx, int32_t T, int32_t k, int32_t E, i
     if (!offsets || (T > 0 && (!sel_idx || !pair_row)))
         return set_error(QGMOE_ERR_INVALID_ARG, "sort_tokens: null pointer argument");
     const int N = T * k;
-    // a warp per 512 pairs: fewer leave the reads of a CTA exposed, more only
-    // add warps that have nothing to count
-    int warps = (N + 511) / 512;
-    warps = warps < 1 ? 1 : warps > SORT_MAX_WARPS ? SORT_MAX_WARPS : warps;
-    QG_CUDA(launch_pdl(k_sort_tokens, dim3((unsigned)E), dim3(warps * 32), 0,
-                       static_cast<cudaStream_t>(stream), 1, sel_idx, N, E, offsets, pair_row,
+    // A warp per 128 pairs, up to eight CTAs of 32 warps; the counters of 32
+    // warps over 1024 experts are 128 KB.
+    int64_t warps = ((int64_t)N + SORT_STEPS * 32 - 1) / (SORT_STEPS * 32);
+    warps = warps < 1 ? 1 : warps;
+    int C = 1;
+    while (C < 8 && warps > C * SORT_MAX_WARPS) C *= 2;
+    int nw = (int)((warps + C - 1) / C);
+    if (nw > SORT_MAX_WARPS) nw = SORT_MAX_WARPS;
+    const size_t smem = sizeof(int) * ((size_t)(nw + 2) * E + 1);
+    if (smem > 48 * 1024)
+        QG_CUDA(cudaFuncSetAttribute(k_sort_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)smem));
+    QG_CUDA(launch_pdl(k_sort_tokens, dim3(1, 1, C), dim3(nw * 32), smem,
+                       static_cast<cudaStream_t>(stream), C, sel_idx, N, E, offsets, pair_row,
                        row_pair));
     return QGMOE_OK;
 }
