@@ -40,19 +40,18 @@ using namespace sm100;
 
 constexpr int I8_M = 128;          // weight rows per CTA tile (= TMEM lanes)
 constexpr int I8_BK = 128;         // codes per stage: one swizzled 128-byte row
-constexpr int I8_EPI_WARPS = 8;    // warps 0-7: TMEM lane quarter = warp & 3
-constexpr int I8_LOAD_WARP = 8;
-constexpr int I8_MMA_WARP = 9;
-constexpr int I8_THREADS = 10 * 32;
+// Warps 0 .. EPI_WARPS - 1 are the epilogue (TMEM lane quarter = warp & 3), then
+// the loading and the MMA-issuing warp.
 constexpr int I8_MAX_GROUPS = QG_MAX_EXPERTS;
 constexpr int I8_MAX_IN = 131071;  // 131071 * 128 * 128 < 2^31: exact int32 sums
 constexpr long long I8_WAIT_CYCLES = 4000000000LL;  // ~2 s
-// Epilogue staging of a warp: 32 rows of 32 16-bit channels, 80 bytes apart so
+// Epilogue staging of a warp: 16 rows of 32 16-bit channels, 80 bytes apart so
 // that the 8 rows a stmatrix writes fall into different banks; then the scales
-// of its rows, up to four runs of 32.
+// of its rows, up to two runs of 32.
 constexpr int I8_ROW_PITCH = 80;
-constexpr int I8_RUNS = 4;
-constexpr int I8_STAGING = 32 * I8_ROW_PITCH + I8_RUNS * 128;
+constexpr int I8_SCALES = 16 * I8_ROW_PITCH;
+constexpr int I8_STAGING = I8_SCALES + 2 * 128;
+constexpr int I8_SMEM = 232448;  // most shared memory of a CTA
 
 // NT: most rows of a tile.  Stages fill the shared memory that one CTA per SM
 // may use, so that as many loads as possible are in flight.
@@ -63,12 +62,14 @@ struct I8Cfg {
     static constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int BUF = NT < 32 ? 32 : NT;  // TMEM columns per accumulator buffer
     static constexpr int TMEM_COLS = 2 * BUF;
-    static constexpr int S = 192 * 1024 / STAGE_BYTES;
-    static constexpr int BAR_BYTES = 8 * (2 * S + 5) + 16;
+    // warps: a run of 32 rows per quarter each, up to two runs
+    static constexpr int EPI_WARPS = NT <= 32 ? 4 : NT <= 64 ? 8 : 16;
+    static constexpr int LOAD_WARP = EPI_WARPS, MMA_WARP = EPI_WARPS + 1;
+    static constexpr int THREADS = (EPI_WARPS + 2) * 32;
     static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12;
-    static constexpr int SMEM =
-        S * STAGE_BYTES + I8_EPI_WARPS * I8_STAGING + BAR_BYTES + TAB_BYTES + 1024;
-    static_assert(SMEM <= 232448, "shared memory budget");
+    static constexpr int REST = EPI_WARPS * I8_STAGING + 8 * 5 + 16 + TAB_BYTES + 1024;
+    static constexpr int S = (I8_SMEM - REST) / (STAGE_BYTES + 16);  // two barriers a stage
+    static constexpr int SMEM = S * (STAGE_BYTES + 16) + REST;
     static_assert(STAGE_BYTES % 1024 == 0, "1024-byte aligned tiles");
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0, "TMEM budget");
 };
@@ -302,10 +303,9 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 *, float a, float b) {
 }
 
 // One accumulator of n rows (TMEM columns) by this warp: lane quarter q = 32
-// weight rows of tile rt; the two warps of a quarter take alternate runs of 32
-// rows (half 0 / 1).  y = float(sum) * ws * xs, the row's scale last: it is as
-// large as the activations are, and the sum times it may overflow where y does
-// not.
+// weight rows of tile rt; the SUBS warps of a quarter take turns at runs of 32
+// rows.  y = float(sum) * ws * xs, the row's scale last: it is as large as the
+// activations are, and the sum times it may overflow where y does not.
 //   float32, plain: a lane is a channel, a store 32 neighbouring ones of a row.
 //   SwiGLU: of a quarter's 32 weight rows the first 16 are gate, the others
 //     the up rows of the same 16 channels (k_i8_layout); read 16 lanes at a
@@ -313,32 +313,32 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 *, float a, float b) {
 //   16-bit: pairs of rows packed in a thread, transposed through the warp's
 //     staging, written 16 bytes at a time.
 // The tile's scales are fetched before its accumulator is waited for
-// (prepare), and a run's TMEM columns while the run before is converted: with
-// two warps per quarter nothing else hides those latencies, and an epilogue
-// that took longer than the tile's MMAs held the whole kernel at 36 % of the
-// tensor pipe.
-template <typename TO, bool SWIGLU>
+// (prepare).  The epilogue is a chain of dependent instructions with little to
+// overlap inside a warp: eight warps took 1100 cycles a run and held a
+// 4096 x 2048 x 4096 product at 32 us, sixteen take half.
+template <typename TO, bool SWIGLU, int SUBS>
 struct I8Epilogue {
     static constexpr bool F32 = sizeof(TO) == 4;
     static constexpr bool LANES = F32 && !SWIGLU;  // a lane is a channel
     static constexpr int CH = SWIGLU ? 16 : 32;    // channels of this warp
     // 16-bit rows leave in 16-byte chunks, a store ROWS rows
     static constexpr int CHUNKS = CH / 8, ROWS = 32 / CHUNKS;
+    static constexpr int RUNS = SUBS == 4 ? 2 : 1;  // of an accumulator, per warp
 
     const I8Args &a;
-    int q, half, lane;
+    int q, first, lane;  // first row column of this warp's first run
     uint32_t staging;
     float sw[4];  // scales of the weight rows this thread converts
 
     __device__ __forceinline__ I8Epilogue(const I8Args &a, int warp, int lane, uint32_t staging)
-        : a(a), q(warp & 3), half(warp >> 2), lane(lane), staging(staging) {}
+        : a(a), q(warp & 3), first(warp / 4 * 32), lane(lane), staging(staging) {}
 
     // ws: the quarter's 32 channel scales
     __device__ __forceinline__ void prepare(const float *ws, int64_t row0, int n) {
-        float sx[I8_RUNS];
+        float sx[RUNS];
 #pragma unroll
-        for (int i = 0; i < I8_RUNS; i++) {
-            const int c = half * 32 + i * 64 + lane;
+        for (int i = 0; i < RUNS; i++) {
+            const int c = first + i * SUBS * 32 + lane;
             sx[i] = c < n ? *(const volatile float *)(a.xs + row0 + c) : 0.f;
         }
         if constexpr (LANES) {
@@ -348,8 +348,8 @@ struct I8Epilogue {
             for (int i = 0; i < 4; i++) sw[i] = ws[(lane >> 2) + 8 * i];
         }
 #pragma unroll
-        for (int i = 0; i < I8_RUNS; i++)
-            st_shared_f32(staging + 32 * I8_ROW_PITCH + i * 128 + lane * 4, sx[i]);
+        for (int i = 0; i < RUNS; i++)
+            st_shared_f32(staging + I8_SCALES + i * 128 + lane * 4, sx[i]);
         __syncwarp();
     }
 
@@ -361,6 +361,7 @@ struct I8Epilogue {
             tmem_ld_16x32(tmem, v[0]);
             tmem_ld_16x32(tmem + (16u << 16), v[1]);
         }
+        tmem_wait_ld();
     }
 
     // A run: 32 rows, nc of them real.  yp: this thread's place in the first
@@ -420,35 +421,39 @@ struct I8Epilogue {
                     for (int e = 0; e < (SWIGLU ? 2 : 4); e++)
                         p[e] = pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y);
                     if constexpr (SWIGLU)
-                        stmatrix2_trans(to + i * 8 * I8_ROW_PITCH, p[0], p[1]);
+                        stmatrix2_trans(to + (i & 1) * 8 * I8_ROW_PITCH, p[0], p[1]);
                     else
-                        stmatrix4_trans(to + i * 8 * I8_ROW_PITCH, p);
-                }
-            }
-            if constexpr (!F32) {
-                __syncwarp();
-                const uint32_t from =
-                    staging + (lane / CHUNKS) * I8_ROW_PITCH + (lane % CHUNKS) * 16;
-#pragma unroll
-                for (int p = 0; p < CHUNKS; p++) {
-                    const uint4 u = ld_shared_v4(from + p * ROWS * I8_ROW_PITCH);
-                    if (p * ROWS + lane / CHUNKS < nc) {
-                        const int o = o0 + lane % CHUNKS * 8;
-                        if (a.vec) {  // cols % 8 == 0: a chunk is inside or outside
-                            if (o < a.cols) *reinterpret_cast<uint4 *>(yp) = u;
-                        } else {
-                            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                            for (int e = 0; e < 8; e++)
-                                if (o + e < a.cols)
-                                    reinterpret_cast<uint16_t *>(yp)[e] =
-                                        (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
-                        }
+                        stmatrix4_trans(to + (i & 1) * 8 * I8_ROW_PITCH, p);
+                    if (i & 1) {  // 16 rows are staged
+                        __syncwarp();
+                        store16(yp, o0, nc - (i / 2) * 16);
+                        yp += 16 * pitch;
+                        __syncwarp();
                     }
-                    yp += ROWS * pitch;
                 }
-                __syncwarp();  // the staging is written again
             }
+        }
+    }
+    // The 16 staged rows, nc of them real, from yp on.
+    __device__ __forceinline__ void store16(TO *yp, int o0, int nc) {
+        const uint32_t from = staging + (lane / CHUNKS) * I8_ROW_PITCH + (lane % CHUNKS) * 16;
+        const int o = o0 + lane % CHUNKS * 8;
+#pragma unroll
+        for (int p = 0; p < 16 / ROWS; p++) {
+            const uint4 u = ld_shared_v4(from + p * ROWS * I8_ROW_PITCH);
+            if (p * ROWS + lane / CHUNKS < nc) {
+                if (a.vec) {  // cols % 8 == 0: a chunk is inside or outside
+                    if (o < a.cols) *reinterpret_cast<uint4 *>(yp) = u;
+                } else {
+                    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (o + e < a.cols)
+                            reinterpret_cast<uint16_t *>(yp)[e] =
+                                (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                }
+            }
+            yp += ROWS * (int64_t)a.cols;
         }
     }
     // Where this thread's first store of a run that starts at y row r0 goes.
@@ -473,17 +478,17 @@ struct I8Epilogue {
     template <typename F>
     __device__ __forceinline__ void drain(uint32_t tmem, int64_t row0, int n, int rt, F read) {
         const int o0 = (rt * 4 + q) * CH;
-        TO *yp = place(row0 + half * 32, o0);
-        int v[2][2][16];
-        if (half * 32 < n) fetch(tmem + half * 32, v[0]); else read();
+        TO *yp = place(row0 + first, o0);
+        if (first >= n) read();
 #pragma unroll
-        for (int i = 0; i < I8_RUNS; i++) {
-            const int c0 = half * 32 + i * 64;
+        for (int i = 0; i < RUNS; i++) {
+            const int c0 = first + i * SUBS * 32;
             if (c0 < n) {
-                tmem_wait_ld();
-                if (i + 1 < I8_RUNS && c0 + 64 < n) fetch(tmem + c0 + 64, v[(i + 1) & 1]); else read();
-                run(v[i & 1], staging + 32 * I8_ROW_PITCH + i * 128, yp, min(32, n - c0), o0);
-                yp += 64 * (int64_t)a.cols;
+                int v[2][16];
+                fetch(tmem + c0, v);
+                if (i + 1 == RUNS || c0 + SUBS * 32 >= n) read();
+                run(v, staging + I8_SCALES + i * 128, yp, min(32, n - c0), o0);
+                yp += SUBS * 32 * (int64_t)a.cols;
             }
         }
         __syncwarp();  // the scales are written again
@@ -492,7 +497,7 @@ struct I8Epilogue {
 
 // ---- one CTA per tile ---------------------------------------------------------------
 template <int NT, typename TO, bool SWIGLU>
-__global__ void __launch_bounds__(I8_THREADS, 1)
+__global__ void __launch_bounds__(I8Cfg<NT>::THREADS, 1)
 k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
      const I8Args a) {
     pdl_launch_dependents();
@@ -505,7 +510,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES +
-                                                  I8_EPI_WARPS * I8_STAGING);
+                                                  Cfg::EPI_WARPS * I8_STAGING);
     uint64_t *empty = full + S;
     uint64_t *accFull = empty + S;     // [2]
     uint64_t *accEmpty = accFull + 2;  // [2]
@@ -521,7 +526,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&accFull[b], 1);
-            mbar_init(&accEmpty[b], I8_EPI_WARPS);
+            mbar_init(&accEmpty[b], Cfg::EPI_WARPS);
         }
         mbar_init(drain, 1);
         st_volatile_shared(abort_addr, 0);
@@ -529,7 +534,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         prefetch_tmap(&tmap_w);
         prefetch_tmap(&tmap_x);
     }
-    if (warp == I8_MMA_WARP) {
+    if (warp == Cfg::MMA_WARP) {
         tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
         tmem_relinquish();
     }
@@ -548,9 +553,9 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         }
     };
 
-    if (warp < I8_EPI_WARPS) {
+    if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue: TMEM -> scaled rows ===============================
-        I8Epilogue<TO, SWIGLU> epi(a, warp, lane, staging + warp * I8_STAGING);
+        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane, staging + warp * I8_STAGING);
         int lt = 0;
         for (int u = blockIdx.x; u < n_units; u += gridDim.x, lt++) {
             const int buf = lt & 1;
@@ -569,7 +574,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
                 if (lane == 0) mbar_arrive(&accEmpty[buf]);
             });
         }
-    } else if (warp == I8_LOAD_WARP) {
+    } else if (warp == Cfg::LOAD_WARP) {
         // ============ loads: weight tile and row tile of each 128-code block ======
         if (lane == 0) {
             int g = 0;
@@ -636,7 +641,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     tc_fence_before();
     __syncthreads();
-    if (warp == I8_MMA_WARP) {
+    if (warp == Cfg::MMA_WARP) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::TMEM_COLS);
     }
@@ -658,7 +663,7 @@ __device__ __forceinline__ int i8p_first(int n) {  // rows of the first part
 }
 
 template <typename TO, bool SWIGLU>
-__global__ void __launch_bounds__(I8_THREADS, 1)
+__global__ void __launch_bounds__(I8Pair::THREADS, 1)
 k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
           const I8Args a) {
     pdl_launch_dependents();
@@ -673,7 +678,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
     uint64_t *full = reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES +
-                                                  I8_EPI_WARPS * I8_STAGING);
+                                                  Cfg::EPI_WARPS * I8_STAGING);
     uint64_t *empty = full + S;
     uint64_t *accFull = empty + S;     // [2]
     uint64_t *accEmpty = accFull + 2;  // [2]
@@ -689,7 +694,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         }
         for (int b = 0; b < 2; b++) {
             mbar_init(&accFull[b], 1);
-            mbar_init(&accEmpty[b], 2 * I8_EPI_WARPS);  // both CTAs' epilogues
+            mbar_init(&accEmpty[b], 2 * Cfg::EPI_WARPS);  // both CTAs' epilogues
         }
         mbar_init(drain, 1);
         st_volatile_shared(abort_addr, 0);
@@ -697,7 +702,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         prefetch_tmap(&tmap_w);
         prefetch_tmap(&tmap_x);
     }
-    if (warp == I8_MMA_WARP) tmem_alloc2(tmem_slot, 512);
+    if (warp == Cfg::MMA_WARP) tmem_alloc2(tmem_slot, 512);
     pdl_wait();
     if (warp == 0) i8_prefix(a, prefix, lane);
     tc_fence_before();
@@ -714,9 +719,9 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         }
     };
 
-    if (warp < I8_EPI_WARPS) {
+    if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue of this CTA's 128 channels =========================
-        I8Epilogue<TO, SWIGLU> epi(a, warp, lane, staging + warp * I8_STAGING);
+        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane, staging + warp * I8_STAGING);
         int sc = 0;  // accumulators used so far
         bool ok = true;
         for (int u = first_unit; u < n_units && ok; u += unit_step) {
@@ -746,7 +751,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                 sc++;
             }
         }
-    } else if (warp == I8_LOAD_WARP) {
+    } else if (warp == Cfg::LOAD_WARP) {
         // ============ this CTA's half of the loads ================================
         if (lane == 0) {
             int g = 0;
@@ -878,7 +883,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     __syncthreads();
     cluster_sync();
     tc_fence_after();
-    if (warp == I8_MMA_WARP) tmem_dealloc2(tmem, 512);
+    if (warp == Cfg::MMA_WARP) tmem_dealloc2(tmem, 512);
     cluster_sync();
 }
 
@@ -1006,7 +1011,7 @@ static int launch_i8_pair_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &
     at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_pdl
     at[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(I8_THREADS);
+    cfg.blockDim = dim3(I8Pair::THREADS);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
     cfg.attrs = at;
@@ -1039,7 +1044,7 @@ static int launch_i8_cta_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a
     }
     int64_t grid = num_sms(h->device);
     if (max_units < grid) grid = max_units;
-    QG_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8_THREADS), smem, s, 1, h->tmap_w, tx, a));
+    QG_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8Cfg<NT>::THREADS), smem, s, 1, h->tmap_w, tx, a));
     return QGMOE_OK;
 }
 

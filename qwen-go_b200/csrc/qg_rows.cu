@@ -127,15 +127,16 @@ template <> struct Vec8<float> {  // two 16-byte loads
 // ---- sort -------------------------------------------------------------------
 // One cluster of up to eight CTAs, no workspace, one launch.  Each warp owns a
 // contiguous range of pairs and takes it 32 at a time: lanes with the same
-// expert find each other (match), rank themselves in lane order on top of the
-// warp's count of that expert so far, and the first adds their number to the
-// count.  The counts of the CTA's warps, then of the cluster's CTAs
+// expert find each other (a ballot per bit of the id; match.any is several
+// times slower), rank themselves in lane order on top of the warp's count of
+// that expert so far, and the first adds their number to the count.  The counts of the CTA's warps, then of the cluster's CTAs
 // (distributed shared memory), then of the experts are summed in order; a
 // pair's row is the three prefixes and its rank.  The order within an expert
 // is the pairs' own by construction; no atomics.
 // Every id is handled once: 32768 pairs over 128 experts take 5 us, where one
 // CTA per expert, each counting all pairs, took 12.
 constexpr int SORT_MAX_WARPS = 32;
+constexpr int SORT_MAX_CTAS = 8;
 constexpr int SORT_STEPS = 4;  // steps of 32 whose loads are in flight together
 
 __device__ __forceinline__ int ld_i32_if(bool on, const int32_t *p, int other) {
@@ -154,22 +155,35 @@ __device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
     return v;
 }
 
+// Lanes whose v (below 2^bits) equals this lane's.
+__device__ __forceinline__ unsigned same_lanes(int v, int bits) {
+    unsigned m = ~0u;
+    for (int b = 0; b < bits; b++) {
+        const bool on = (v >> b) & 1;
+        const unsigned w = __ballot_sync(~0u, on);
+        m &= on ? w : ~w;
+    }
+    return m;
+}
+
 __global__ void __launch_bounds__(SORT_MAX_WARPS * 32)
 k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_row,
               int32_t *row_pair) {
     extern __shared__ int sort_smem[];
+    __shared__ int s_sum[SORT_MAX_WARPS];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
     const int C = gridDim.z, rank = blockIdx.z;  // the grid is the cluster
     int *hist = sort_smem;        // [nw][E]: counts, then the warps before
     int *tot = hist + nw * E;     // [E] this CTA's counts
-    int *base = tot + E;          // [E + 1] counts of all, then first rows
+    int *base = tot + E;          // [E] first rows
     int *mine = hist + warp * E;
     int64_t per = ((int64_t)N + C * nw - 1) / (C * nw);
     per = (per + 31) & ~int64_t(31);
     const int64_t lo = min((int64_t)N, per * (rank * nw + warp)), hi = min((int64_t)N, lo + per);
     const bool kept = per <= SORT_STEPS * 32;  // one round: ids and ranks stay in registers
     const unsigned below = (1u << lane) - 1;
+    const int bits = 32 - __clz(E);
     for (int e = lane; e < E; e += 32) mine[e] = 0;
     __syncwarp();
 
@@ -184,7 +198,7 @@ k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_
         for (int b = 0; b < SORT_STEPS; b++) {
             const int64_t i = i0 + b * 32 + lane;
             const bool valid = (unsigned)id[b] < (unsigned)E;
-            const unsigned peers = __match_any_sync(~0u, valid ? id[b] : -1);
+            const unsigned peers = same_lanes(valid ? id[b] : E, bits);
             const int ahead = __popc(peers & below);
             const int so_far = valid ? mine[id[b]] : 0;
             __syncwarp();
@@ -197,46 +211,61 @@ k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_
     __syncthreads();
     for (int e = threadIdx.x; e < E; e += blockDim.x) {
         int sum = 0;
-#pragma unroll 8
-        for (int w = 0; w < nw; w++) {
-            const int v = hist[w * E + e];
-            hist[w * E + e] = sum;
-            sum += v;
+        for (int w0 = 0; w0 < nw; w0 += 8) {
+            int v[8];
+#pragma unroll
+            for (int w = 0; w < 8; w++) v[w] = w0 + w < nw ? hist[(w0 + w) * E + e] : 0;
+#pragma unroll
+            for (int w = 0; w < 8; w++) {
+                if (w0 + w < nw) hist[(w0 + w) * E + e] = sum;
+                sum += v[w];
+            }
         }
         tot[e] = sum;
     }
     if (C > 1) sm100::cluster_sync(); else __syncthreads();
-    // counts of all CTAs to base, those of the CTAs before this one to tot
-    for (int e = threadIdx.x; e < E; e += blockDim.x) {
+    // first rows of the experts: a scan over the counts of all CTAs; hist's
+    // first row, whose values are all zero, takes those of the CTAs before
+    // this one (tot itself is still read by the others)
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += blockDim.x) {
+        const int e = e0 + threadIdx.x;
         int before = 0, all = 0;
-        for (int c = 0; c < C; c++) {
-            const int v =
-                C > 1 ? ld_cluster_i32(sm100::mapa_shared(sm100::smem_u32(tot + e), c)) : tot[e];
-            if (c == rank) before = all;
-            all += v;
-        }
-        base[e] = all;
-        // tot itself is still read by the other CTAs: hist's first row, whose
-        // values are all zero, takes the sum
-        hist[e] = before;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int sum = 0;
-        for (int e0 = 0; e0 < E; e0 += 32) {
-            const int e = e0 + lane, v = e < E ? base[e] : 0;
-            int x = v;
+        if (e < E) {
+            int v[SORT_MAX_CTAS];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(~0u, x, o);
-                if (lane >= o) x += y;
+            for (int c = 0; c < SORT_MAX_CTAS; c++) {
+                v[c] = 0;
+                if (c < C)
+                    v[c] = C > 1 ? ld_cluster_i32(sm100::mapa_shared(sm100::smem_u32(tot + e), c))
+                                 : tot[e];
             }
-            if (e < E) base[e] = sum + x - v;
-            sum += __shfl_sync(~0u, x, 31);
+#pragma unroll
+            for (int c = 0; c < SORT_MAX_CTAS; c++) {
+                if (c < rank) before += v[c];
+                all += v[c];
+            }
         }
-        if (lane == 0) base[E] = sum;
+        int x = all;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(~0u, x, o);
+            if (lane >= o) x += y;
+        }
+        if (lane == 31) s_sum[warp] = x;
+        __syncthreads();
+        const int w = lane < nw ? s_sum[lane] : 0;
+        const int ahead = __reduce_add_sync(~0u, lane < warp ? w : 0);
+        if (e < E) {
+            base[e] = carry + ahead + x - all;
+            hist[e] = before;
+        }
+        carry += __reduce_add_sync(~0u, w);
+        __syncthreads();
     }
-    __syncthreads();
+    const int total = carry;
+    // the other CTAs' counts are read; nobody waits for this CTA's stores
+    if (C > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     for (int64_t i0 = lo; i0 < hi; i0 += SORT_STEPS * 32) {
         if (!kept) {
 #pragma unroll
@@ -258,13 +287,13 @@ k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_
             pair_row[i] = row;
         }
     }
-    const int total = base[E];
     const int64_t t0 = (int64_t)rank * blockDim.x + threadIdx.x;
     if (rank == 0)
-        for (int e = threadIdx.x; e <= E; e += blockDim.x) offsets[e] = base[e];
+        for (int e = threadIdx.x; e <= E; e += blockDim.x) offsets[e] = e < E ? base[e] : total;
     if (row_pair)  // rows without a pair
         for (int64_t i = total + t0; i < N; i += (int64_t)C * blockDim.x) row_pair[i] = -1;
-    if (C > 1) sm100::cluster_sync();  // the other CTAs have read tot
+    // this CTA's counts stay until all have read them
+    if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // ---- gather -------------------------------------------------------------------
@@ -422,12 +451,13 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
 // scale NaN and codes 0, so that what is computed from it is NaN.  With
 // pair_row, row t goes to the k rows of its pairs.
 //
-// The quotient is formed as x * (1 / scale), within 2^-22 |q| < 4e-5 of the
-// exact one, and rounded by adding 1.5 * 2^23, which leaves the code in the
-// low byte.  Only where that lands within 1e-4 of a half, where the exact
-// quotient might round the other way, the eight values are divided (the test
-// is one maximum over them).  Five operations a value instead of some twenty:
-// 4096 rows of 2048 went from 14.8 us to the time of their bytes.
+// The quotient is Markstein's: with y the rounded reciprocal of the scale and
+// t = x y, the remainder r = x - t s is exact in one fused operation and
+// t + r y is the correctly rounded x / s (Markstein 1990; a scale whose
+// mantissa is all ones is the theorem's exception and is divided by).  Adding
+// 1.5 * 2^23 rounds it, halves to even, and leaves the code in the low byte;
+// halves are then moved away from zero, which only vectors that hold one pay
+// for.  Seven operations a value instead of some twenty.
 //
 // A row belongs to `wpr` warps of a CTA.  It is copied to shared memory
 // asynchronously and read there twice, each thread the vectors it copied
@@ -438,41 +468,111 @@ constexpr int QR_WARPS = 8;
 constexpr int QR_THREADS = QR_WARPS * 32;
 constexpr int QR_ROW_BYTES = 32 * 1024;
 
-__device__ __forceinline__ uint32_t code_of(float v, float s) {
-    const float q = fminf(fmaxf(roundf(__fdiv_rn(v, s)), -127.f), 127.f);
-    return (uint32_t)(int)q & 0xFFu;
-}
 __device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
-__device__ __noinline__ uint32_t codes_exact(float a, float b, float c, float d, float s) {
-    return pack4(code_of(a, s), code_of(b, s), code_of(c, s), code_of(d, s));
-}
-// Largest magnitude as float bits (exponent all ones: infinity or NaN).
-__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7FFFFFFFu; }
-template <typename T> __device__ __forceinline__ void fold_max(uint32_t &m, const Vec8<T> &x) {
-    float v[8];
-    x.get(v);
+// Largest magnitude of a row.  float32: a maximum that keeps NaN; 16 bits: the
+// two halves of a word at once, as integers, which order magnitudes and put
+// infinity and NaN above every number.
+template <typename T> struct AbsMax {
+    uint32_t m = 0;
+    __device__ __forceinline__ void fold(const Vec8<T> &x) {
+        const uint32_t w[4] = {x.r.x, x.r.y, x.r.z, x.r.w};
 #pragma unroll
-    for (int q = 0; q < 8; q++) m = max(m, abs_bits(v[q]));
-}
+        for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
+    __device__ __forceinline__ void fold1(float v) {  // one widened value
+        if constexpr (__is_same(T, __half))
+            m = __vmaxu2(m, (uint32_t)__half_as_ushort(__float2half_rn(fabsf(v))));
+        else
+            m = __vmaxu2(m, __float_as_uint(fabsf(v)) >> 16);
+    }
+    // as float32 bits, exponent all ones for infinity or NaN
+    __device__ __forceinline__ uint32_t bits() const {
+        const uint32_t h = max(m & 0xFFFFu, m >> 16);
+        if constexpr (__is_same(T, __half)) {
+            if (h >= 0x7C00u) return 0x7F800000u;
+            return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+        }
+        return h << 16;
+    }
+};
+template <> struct AbsMax<float> {
+    float m = 0.f;
+    __device__ __forceinline__ void fold1(float v) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
+    }
+    __device__ __forceinline__ void fold(const Vec8<float> &x) {
+        float v[8];
+        x.get(v);
+#pragma unroll
+        for (int q = 0; q < 8; q++) fold1(v[q]);
+    }
+    __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(m); }
+};
 __device__ __forceinline__ float scale_of(uint32_t m) {
     return fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), 1e-8f);
 }
+// inv: __frcp_rn(s), or 0 where the quotient has to be divided.
+__device__ __forceinline__ float inverse_of(float s) {
+    return (__float_as_uint(s) & 0x7FFFFFu) == 0x7FFFFFu ? 0.f : __frcp_rn(s);
+}
+// Pairs of float32 in a register pair, two operations per instruction.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unf2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
 __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
     constexpr float MAGIC = 12582912.f;
+    const uint64_t minus_s = f2(-s, -s), y = f2(inv, inv);
+    const uint64_t magic = f2(MAGIC, MAGIC), minus_magic = f2(-MAGIC, -MAGIC);
+    const uint64_t minus_one = f2(-1.f, -1.f);
+    float2 q[4], e[4];
     uint32_t c[8];
     float far = 0.f;
 #pragma unroll
-    for (int q = 0; q < 8; q++) {
-        const float t = __fmul_rn(v[q], inv);
-        const float r = __fadd_rn(t, MAGIC);
-        far = fmaxf(far, fabsf(__fsub_rn(t, __fsub_rn(r, MAGIC))));
-        c[q] = __float_as_uint(r);
+    for (int i = 0; i < 4; i++) {
+        const uint64_t x = f2(v[2 * i], v[2 * i + 1]);
+        const uint64_t t = mul2(x, y);
+        uint64_t z = fma2(fma2(t, minus_s, x), y, t);
+        if (inv == 0.f) z = f2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
+        const uint64_t r = add2(z, magic);
+        q[i] = unf2(z);
+        e[i] = unf2(fma2(add2(r, minus_magic), minus_one, z));  // z - round(z), exact
+        const float2 rf = unf2(r);
+        c[2 * i] = __float_as_uint(rf.x);
+        c[2 * i + 1] = __float_as_uint(rf.y);
+        far = fmaxf(far, fmaxf(fabsf(e[i].x), fabsf(e[i].y)));
     }
-    if (far > 0.4999f)
-        return make_uint2(codes_exact(v[0], v[1], v[2], v[3], s),
-                          codes_exact(v[4], v[5], v[6], v[7], s));
+    if (far == 0.5f) {  // some q is a half: away from zero, not to the even side
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float z = i & 1 ? q[i >> 1].y : q[i >> 1].x, d = i & 1 ? e[i >> 1].y : e[i >> 1].x;
+            if (fabsf(d) == 0.5f)
+                c[i] = __float_as_uint(__fadd_rn(__fadd_rn(z, copysignf(0.5f, z)), MAGIC));
+        }
+    }
     return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
 }
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
@@ -487,7 +587,7 @@ template <typename T> __device__ __forceinline__ void ld_shared_vec8(uint32_t ad
     }
 }
 
-template <typename TI>
+template <typename TI, bool GATHER>
 __global__ void __launch_bounds__(QR_THREADS)
 k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t *pair_row,
                 int8_t *codes, int64_t ld, float *scale) {
@@ -507,19 +607,18 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t 
             if (sizeof(TI) == 4) cp_async16(row + c * sizeof(TI) + 16, src + c + 4);
         }
     // destination rows, lane j the j-th of this run of up to 32
-    const int n_dst = pair_row ? k : 1;
     int dst = -1;
-    if (on && lane < n_dst) dst = pair_row ? ld_i32(pair_row + t * k + lane) : (int)t;
+    if (GATHER && on && lane < k) dst = ld_i32(pair_row + t * k + lane);
     asm volatile("cp.async.wait_all;" ::: "memory");
-    uint32_t m = 0;
+    AbsMax<TI> top;
     if (on)
-#pragma unroll 2
+#pragma unroll 4
         for (int c = c0; c < K; c += span) {
             Vec8<TI> in;
             ld_shared_vec8(row + c * (int)sizeof(TI), in);
-            fold_max(m, in);
+            top.fold(in);
         }
-    m = __reduce_max_sync(~0u, m);
+    uint32_t m = __reduce_max_sync(~0u, top.bits());
     if (wpr > 1) {
         if (lane == 0) s_max[warp] = m;
         __syncthreads();
@@ -527,26 +626,41 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t 
     }
     if (!on) return;
     const bool bad = m >= 0x7F800000u;
-    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
-    for (int j0 = 0; j0 < n_dst; j0 += 32) {
-        if (j0) dst = j0 + lane < n_dst ? ld_i32(pair_row + t * k + j0 + lane) : -1;
-        const int n = min(32, n_dst - j0);
-        if (part == 0 && lane < n && (unsigned)dst < (unsigned)N)
-            scale[dst] = bad ? CUDART_NAN_F : s;
-        for (int c = c0; c - lane * 8 < K; c += span) {  // whole warps: the rows are shuffled
-            uint2 u = make_uint2(0, 0);
-            if (c < K && !bad) {
-                Vec8<TI> in;
-                float v[8];
-                ld_shared_vec8(row + c * (int)sizeof(TI), in);
-                in.get(v);
-                u = codes_of(v, s, inv);
-            }
+    const float s = bad ? 1.f : scale_of(m), inv = inverse_of(s);
+    if constexpr (!GATHER) {
+        if (part == 0 && lane == 0) scale[t] = bad ? CUDART_NAN_F : s;
+        int8_t *out = codes + t * ld;
+#pragma unroll 2
+        for (int c = c0; c < K; c += span) {
+            Vec8<TI> in;
+            float v[8];
+            ld_shared_vec8(row + c * (int)sizeof(TI), in);
+            in.get(v);
+            uint2 u = codes_of(v, s, inv);
+            if (bad) u = make_uint2(0, 0);
+            *reinterpret_cast<uint2 *>(out + c) = u;
+        }
+    } else {
+        for (int j0 = 0; j0 < k; j0 += 32) {
+            if (j0) dst = j0 + lane < k ? ld_i32(pair_row + t * k + j0 + lane) : -1;
+            const int n = min(32, k - j0);
+            if (part == 0 && lane < n && (unsigned)dst < (unsigned)N)
+                scale[dst] = bad ? CUDART_NAN_F : s;
+            for (int c = c0; c - lane * 8 < K; c += span) {  // whole warps: the rows are shuffled
+                uint2 u = make_uint2(0, 0);
+                if (c < K && !bad) {
+                    Vec8<TI> in;
+                    float v[8];
+                    ld_shared_vec8(row + c * (int)sizeof(TI), in);
+                    in.get(v);
+                    u = codes_of(v, s, inv);
+                }
 #pragma unroll 4
-            for (int j = 0; j < n; j++) {
-                const int r = __shfl_sync(~0u, dst, j);
-                if ((unsigned)r < (unsigned)N && c < K)
-                    *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = u;
+                for (int j = 0; j < n; j++) {
+                    const int r = __shfl_sync(~0u, dst, j);
+                    if ((unsigned)r < (unsigned)N && c < K)
+                        *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = u;
+                }
             }
         }
     }
@@ -563,24 +677,24 @@ k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_
     const int64_t t = blockIdx.x;
     const int tid = threadIdx.x, nt = blockDim.x;
     const TI *src = x + t * K;
-    uint32_t m = 0;
+    AbsMax<TI> top;
     if constexpr (VEC) {
 #pragma unroll 4
         for (int c = tid * 8; c < K; c += nt * 8) {
             Vec8<TI> in;
             in.load(src + c);
-            fold_max(m, in);
+            top.fold(in);
         }
     } else {
 #pragma unroll 4
-        for (int c = tid; c < K; c += nt) m = max(m, abs_bits(Elem<TI>::load(src + c)));
+        for (int c = tid; c < K; c += nt) top.fold1(Elem<TI>::load(src + c));
     }
-    m = __reduce_max_sync(~0u, m);
+    uint32_t m = __reduce_max_sync(~0u, top.bits());
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
     for (int w = 0; w < nt >> 5; w++) m = max(m, s_max[w]);
     const bool bad = m >= 0x7F800000u;
-    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
+    const float s = bad ? 1.f : scale_of(m), inv = inverse_of(s);
     const int n_dst = pair_row ? k : 1;
     auto dst_row = [&](int j) { return pair_row ? ld_i32(pair_row + t * k + j) : (int)t; };
     for (int j = tid; j < n_dst; j += nt) {
@@ -671,10 +785,11 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
     const bool vec = K % 8 == 0 && aligned16(x);
     const int N = pair_row ? T * k : T;
     const int row_bytes = K * (dt == QGMOE_DT_F32 ? 4 : 2);
-    // Many rows: a warp per row (no barrier); few rows: up to eight warps, for
-    // latency.
-    int wpr = T < 1024 ? QR_WARPS : 1;
-    while (wpr > 1 && K <= wpr / 2 * 256) wpr /= 2;
+    // As many warps for a row as fill the device about once (8192 warps): 4096
+    // bf16 rows of 2048 take 8.8 us with one or two warps each and 14.3 with
+    // eight, 1024 rows 6.0, 5.4, 4.3 and 4.5 us with one, two, four and eight.
+    int wpr = 1;
+    while (wpr < QR_WARPS && (int64_t)T * wpr < 8192 && K > wpr * 256) wpr *= 2;
     while (wpr < QR_WARPS && QR_WARPS / wpr * (int64_t)row_bytes > QR_ROW_BYTES) wpr *= 2;
     const int rows = QR_WARPS / wpr;
     return with_dtype(dt, [&](auto *ip) {
@@ -687,7 +802,8 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
                                static_cast<const TI *>(x), k, K, N, pair_row, codes, ld, scale));
             return (int)QGMOE_OK;
         }
-        QG_CUDA(launch_pdl(k_quantize_rows<TI>, dim3((unsigned)((T + (int64_t)rows - 1) / rows)),
+        auto kern = pair_row ? k_quantize_rows<TI, true> : k_quantize_rows<TI, false>;
+        QG_CUDA(launch_pdl(kern, dim3((unsigned)((T + (int64_t)rows - 1) / rows)),
                            dim3(QR_THREADS), (size_t)(rows * row_bytes), s, 1,
                            static_cast<const TI *>(x), T, k, K, N, wpr, pair_row, codes, ld,
                            scale));
@@ -733,10 +849,11 @@ int qgmoe_sort_tokens(const int32_t *sel_idx, int32_t T, int32_t k, int32_t E, i
     int64_t warps = ((int64_t)N + SORT_STEPS * 32 - 1) / (SORT_STEPS * 32);
     warps = warps < 1 ? 1 : warps;
     int C = 1;
-    while (C < 8 && warps > C * SORT_MAX_WARPS) C *= 2;
+    while (C < SORT_MAX_CTAS && warps > C * SORT_MAX_WARPS) C *= 2;
     int nw = (int)((warps + C - 1) / C);
+    if (nw < (E + 31) / 32) nw = (E + 31) / 32;  // a thread per expert for the scans
     if (nw > SORT_MAX_WARPS) nw = SORT_MAX_WARPS;
-    const size_t smem = sizeof(int) * ((size_t)(nw + 2) * E + 1);
+    const size_t smem = sizeof(int) * (size_t)(nw + 2) * E;
     if (smem > 48 * 1024)
         QG_CUDA(cudaFuncSetAttribute(k_sort_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)smem));
