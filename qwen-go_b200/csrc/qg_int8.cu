@@ -581,7 +581,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
             bool ok = true;
             for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
                 const I8Unit w = i8_unit(a, prefix, u);
-                const int wrow = (w.g * a.RT + w.ct) * I8_M;
+                const int wrow = (w.g * a.RT + w.ct) * a.KB * I8_M;
                 for (int kb = 0; kb < a.KB; kb++, g++) {
                     const int s = g % S;
                     if (!mbar_wait(&empty[s], ((g / S) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
@@ -591,7 +591,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
                     }
                     uint8_t *dst = base + s * Cfg::STAGE_BYTES;
                     mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
-                    tma_load_2d(dst, &tmap_w, kb * I8_BK, wrow, &full[s]);
+                    tma_load_2d(dst, &tmap_w, 0, wrow + kb * I8_M, &full[s]);
                     tma_load_2d(dst + Cfg::A_BYTES, &tmap_x, kb * I8_BK, w.row0, &full[s]);
                 }
             }
@@ -758,7 +758,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
             bool ok = true;
             for (int u = first_unit; u < n_units && ok; u += unit_step) {
                 const I8Unit w = i8_unit(a, prefix, u);
-                const int wrow = (w.g * a.RT + w.ct * 2 + rank) * I8_M;
+                const int wrow = (w.g * a.RT + w.ct * 2 + rank) * a.KB * I8_M;
                 const int n0 = i8p_first(w.n), n1 = w.n - n0;
                 // half of each part's rows, and the boxes that cover them
                 const int h0 = ((n0 + 31) & ~31) / 2, h1 = ((n1 + 31) & ~31) / 2;
@@ -776,7 +776,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                     if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
                     const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
                     const int x = kb * I8_BK;
-                    tma_load_2d_pair(dst, &tmap_w, x, wrow, bar);
+                    tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
                     for (int b = 0; b < b0; b++)
                         tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x, r0 + b * I8P_BOX,
                                          bar);
@@ -888,14 +888,16 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 }
 
 // ---- weight layout -------------------------------------------------------------
-// Rows of `groups` groups in tile order, pitch ldw, zeros past the group's
-// rows and past I; scales alike.  With SwiGLU, tile rt holds output columns
-// [rt*64, rt*64 + 64): of each 32 tile rows the first 16 are gate rows of 16
-// columns, the others the up rows of the same columns.
-__global__ void k_i8_layout(const int8_t *q, const float *scale, int groups, int O, int I,
-                            int swiglu, int RT, int64_t ldw, int8_t *dst, float *dscale) {
-    const int64_t row = blockIdx.x;  // of groups * RT * 128
-    const int g = (int)(row / ((int64_t)RT * I8_M));
+// Tiles of 128 rows x 128 codes, each 16 KB in one piece, a row tile's blocks
+// after one another: read as a box of a plain [rows, in] matrix a tile is 128
+// pieces of 128 bytes, of which HBM gave 3.9 TB/s.  Zeros past a group's rows
+// and past I; scales [groups * RT * 128] alike.  With SwiGLU, tile rt holds
+// output columns [rt*64, rt*64 + 64): of each 32 tile rows the first 16 are
+// gate rows of 16 columns, the others the up rows of the same columns.
+__global__ void k_i8_layout(const int8_t *q, const float *scale, int O, int I, int swiglu, int RT,
+                            int KB, int8_t *dst, float *dscale) {
+    const int64_t row = blockIdx.x, tile = row / I8_M;  // of groups * RT * 128
+    const int g = (int)(tile / RT);
     const int l = (int)(row - (int64_t)g * RT * I8_M);
     int o = l;
     bool live = l < O;
@@ -906,8 +908,10 @@ __global__ void k_i8_layout(const int8_t *q, const float *scale, int groups, int
         o = (r & 16) ? cols + c : c;
     }
     const int8_t *src = q + ((int64_t)g * O + o) * I;
-    for (int64_t i = threadIdx.x; i < ldw; i += blockDim.x)
-        dst[row * ldw + i] = live && i < I ? src[i] : (int8_t)0;
+    int8_t *d = dst + (tile * KB * I8_M + row % I8_M) * I8_BK;
+    for (int i = threadIdx.x; i < KB * I8_BK; i += blockDim.x)
+        d[(int64_t)(i / I8_BK) * (I8_M * I8_BK) + i % I8_BK] =
+            live && i < I ? src[i] : (int8_t)0;
     if (threadIdx.x == 0) dscale[row] = live ? scale[(int64_t)g * O + o] : 0.f;
 }
 
@@ -978,7 +982,7 @@ struct qgq8 {
     int RT = 0, live = 0;  // 128-row weight tiles per group, and those that hold channels
     bool swiglu = false;
     cudaStream_t stream = nullptr;
-    int8_t *w = nullptr;   // [G * RT * 128, ldw]
+    int8_t *w = nullptr;   // [G * RT, KB, 128, 128]
     float *ws = nullptr;   // [G * RT * 128]
     int *err_dev = nullptr;
     CUtensorMap tmap_w{};
@@ -1140,19 +1144,19 @@ static int i8_alloc(void **p, size_t bytes) {
 // Device copies of the weights in tile order.  Host weights travel through a
 // staging buffer of whole groups, 64 MB or one group.
 static int i8_build(qgq8 *h, const int8_t *q, const float *scale, bool on_device) {
-    const int64_t rows = (int64_t)h->G * h->RT * I8_M, ldw = i8_pitch(h->I);
-    int rc = i8_alloc(reinterpret_cast<void **>(&h->w), (size_t)rows * ldw);
+    const int64_t rows = (int64_t)h->G * h->RT * I8_M, row_bytes = (int64_t)h->KB * I8_BK;
+    int rc = i8_alloc(reinterpret_cast<void **>(&h->w), (size_t)(rows * row_bytes));
     if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->ws), sizeof(float) * rows);
     if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->err_dev), sizeof(int));
-    if (!rc) rc = i8_encode_map(&h->tmap_w, h->w, rows, h->I, ldw, I8_M);
+    if (!rc) rc = i8_encode_map(&h->tmap_w, h->w, rows * h->KB, I8_BK, I8_BK, I8_M);
     if (rc) return rc;
     QG_CUDA(cudaMemsetAsync(h->err_dev, 0, sizeof(int), h->stream));
     const int64_t gbytes = (int64_t)h->O * h->I;
     if (on_device) {
         // whatever stream the caller wrote the weights on
         QG_CUDA(cudaDeviceSynchronize());
-        k_i8_layout<<<(unsigned)rows, 256, 0, h->stream>>>(q, scale, h->G, h->O, h->I, h->swiglu,
-                                                           h->RT, ldw, h->w, h->ws);
+        k_i8_layout<<<(unsigned)rows, 256, 0, h->stream>>>(q, scale, h->O, h->I, h->swiglu, h->RT,
+                                                           h->KB, h->w, h->ws);
         QG_CUDA(cudaGetLastError());
         QG_CUDA(cudaStreamSynchronize(h->stream));
         return QGMOE_OK;
@@ -1173,7 +1177,7 @@ static int i8_build(qgq8 *h, const int8_t *q, const float *scale, bool on_device
         if (e != cudaSuccess) break;
         const int64_t r0 = g * h->RT * I8_M;
         k_i8_layout<<<(unsigned)(n * h->RT * I8_M), 256, 0, h->stream>>>(
-            tq, ts, (int)n, h->O, h->I, h->swiglu, h->RT, ldw, h->w + r0 * ldw, h->ws + r0);
+            tq, ts, h->O, h->I, h->swiglu, h->RT, h->KB, h->w + r0 * row_bytes, h->ws + r0);
         e = cudaGetLastError();
         if (e == cudaSuccess) e = cudaStreamSynchronize(h->stream);  // tq is reused
     }
@@ -1199,7 +1203,8 @@ int qgq8_create(int32_t groups, int32_t O, int32_t I, const int8_t *q, const flo
         return set_error(QGMOE_ERR_INVALID_ARG, "SwiGLU needs gate and up rows: out=%d is odd", O);
     const int64_t cols = swiglu ? O / 2 : O, per = swiglu ? 64 : I8_M;
     const int64_t RT = (cols + 2 * per - 1) / (2 * per) * 2;  // whole CTA pairs
-    if (RT * groups * I8_M > INT32_MAX)
+    const int64_t KB = (I + I8_BK - 1) / I8_BK;
+    if (RT * groups * I8_M * KB > INT32_MAX)
         return set_error(QGMOE_ERR_INVALID_ARG, "groups=%d x out=%d is too many rows", groups, O);
     if (!q || !scale) return set_error(QGMOE_ERR_INVALID_ARG, "null weights");
     if (!qgmoe_device_ok(device))
@@ -1214,7 +1219,7 @@ int qgq8_create(int32_t groups, int32_t O, int32_t I, const int8_t *q, const flo
     h->cols = (int)cols;
     h->RT = (int)RT;
     h->live = (int)((cols + per - 1) / per);
-    h->KB = (I + I8_BK - 1) / I8_BK;
+    h->KB = (int)KB;
     h->swiglu = swiglu != 0;
     int rc = QGMOE_OK;
     cudaError_t e = cudaStreamCreateWithFlags(&h->stream, cudaStreamNonBlocking);
