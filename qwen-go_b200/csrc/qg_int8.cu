@@ -43,6 +43,7 @@ constexpr int I8_BK = 128;         // codes per stage: one swizzled 128-byte row
 // Warps 0 .. EPI_WARPS - 1 are the epilogue (TMEM lane quarter = warp & 3), then
 // the loading and the MMA-issuing warp.
 constexpr int I8_MAX_GROUPS = QG_MAX_EXPERTS;
+constexpr int I8_UNITS = 64;       // units of a CTA decoded once, into shared memory
 constexpr int I8_MAX_IN = 131071;  // 131071 * 128 * 128 < 2^31: exact int32 sums
 constexpr long long I8_WAIT_CYCLES = 4000000000LL;  // ~2 s
 // Epilogue staging of a warp: 16 rows of 32 16-bit channels, 80 bytes apart so
@@ -66,7 +67,7 @@ struct I8Cfg {
     static constexpr int EPI_WARPS = NT <= 32 ? 4 : NT <= 64 ? 8 : 16;
     static constexpr int LOAD_WARP = EPI_WARPS, MMA_WARP = EPI_WARPS + 1;
     static constexpr int THREADS = (EPI_WARPS + 2) * 32;
-    static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12;
+    static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12 + I8_UNITS * 16;
     static constexpr int REST = EPI_WARPS * I8_STAGING + 8 * 5 + 16 + TAB_BYTES + 1024;
     static constexpr int S = (I8_SMEM - REST) / (STAGE_BYTES + 16);  // two barriers a stage
     static constexpr int SMEM = S * (STAGE_BYTES + 16) + REST;
@@ -223,6 +224,36 @@ __device__ __forceinline__ I8Unit i8_unit(const I8Args &a, const int *prefix, in
     return w;
 }
 
+// A CTA's (a pair's) units in order: first, first + step, ...  The first
+// I8_UNITS of them are decoded together at the start (fill, all threads, then
+// a barrier): a role that looks its next unit up pays a search and two loads
+// of offsets, some 1500 cycles in which it does nothing else.
+struct I8Units {
+    const I8Args &a;
+    const int *prefix;
+    uint32_t table;  // [I8_UNITS] x 16 bytes
+    int first, step, count;
+    __device__ __forceinline__ I8Units(const I8Args &a, const int *prefix, int first, int step)
+        : a(a), prefix(prefix),
+          table((smem_u32(prefix + a.G + 1) + 15) & ~15u), first(first), step(step) {
+        const int n = prefix[a.G] * a.CT;
+        count = first < n ? (n - first + step - 1) / step : 0;
+    }
+    __device__ __forceinline__ void fill(int tid, int threads) const {
+        for (int i = tid; i < min(count, I8_UNITS); i += threads) {
+            const I8Unit w = i8_unit(a, prefix, first + i * step);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(table + i * 16), "r"(w.g),
+                         "r"(w.ct), "r"(w.row0), "r"(w.n)
+                         : "memory");
+        }
+    }
+    __device__ __forceinline__ I8Unit operator[](int i) const {
+        if (i >= I8_UNITS) return i8_unit(a, prefix, first + i * step);
+        const uint4 v = ld_shared_v4(table + i * 16);
+        return I8Unit{(int)v.x, (int)v.y, (int)v.z, (int)v.w};
+    }
+};
+
 // ---- epilogue --------------------------------------------------------------------
 // silu(g) * u = g / (1 + e^-g) * u in float32.  e^-g may overflow to infinity,
 // where the quotient is the right limit, -0.
@@ -312,8 +343,8 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 *, float a, float b) {
 //     time, both land in the same thread.
 //   16-bit: pairs of rows packed in a thread, transposed through the warp's
 //     staging, written 16 bytes at a time.
-// The tile's scales are fetched before its accumulator is waited for
-// (prepare).  The epilogue is a chain of dependent instructions with little to
+// An accumulator's scales are requested while the one before it is waited for
+// and converted.  The epilogue is a chain of dependent instructions with little to
 // overlap inside a warp: eight warps took 1100 cycles a run and held a
 // 4096 x 2048 x 4096 product at 32 us, sixteen take half.
 template <typename TO, bool SWIGLU, int SUBS>
@@ -328,28 +359,33 @@ struct I8Epilogue {
     const I8Args &a;
     int q, first, lane;  // first row column of this warp's first run
     uint32_t staging;
-    float sw[4];  // scales of the weight rows this thread converts
+    float sw[4], next_sw[4];  // scales of the weight rows this thread converts
+    float next_sx[RUNS];
 
     __device__ __forceinline__ I8Epilogue(const I8Args &a, int warp, int lane, uint32_t staging)
         : a(a), q(warp & 3), first(warp / 4 * 32), lane(lane), staging(staging) {}
 
-    // ws: the quarter's 32 channel scales
-    __device__ __forceinline__ void prepare(const float *ws, int64_t row0, int n) {
-        float sx[RUNS];
+    // The scales of an accumulator's rows (xs) and of this quarter's 32
+    // channels (ws), in flight until begin() of that accumulator.
+    __device__ __forceinline__ void request(const float *ws, int64_t row0, int n) {
 #pragma unroll
         for (int i = 0; i < RUNS; i++) {
             const int c = first + i * SUBS * 32 + lane;
-            sx[i] = c < n ? *(const volatile float *)(a.xs + row0 + c) : 0.f;
+            next_sx[i] = c < n ? *(const volatile float *)(a.xs + row0 + c) : 0.f;
         }
         if constexpr (LANES) {
-            sw[0] = ws[lane];
+            next_sw[0] = ws[lane];
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) sw[i] = ws[(lane >> 2) + 8 * i];
+            for (int i = 0; i < 4; i++) next_sw[i] = ws[(lane >> 2) + 8 * i];
         }
+    }
+    __device__ __forceinline__ void begin() {
+#pragma unroll
+        for (int i = 0; i < (LANES ? 1 : 4); i++) sw[i] = next_sw[i];
 #pragma unroll
         for (int i = 0; i < RUNS; i++)
-            st_shared_f32(staging + I8_SCALES + i * 128 + lane * 4, sx[i]);
+            st_shared_f32(staging + I8_SCALES + i * 128 + lane * 4, next_sx[i]);
         __syncwarp();
     }
 
@@ -544,7 +580,9 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int n_units = prefix[a.G] * a.CT;
+    const I8Units units(a, prefix, blockIdx.x, gridDim.x);
+    units.fill(tid, Cfg::THREADS);
+    __syncthreads();
 
     auto fail = [&]() {
         if (!ld_volatile_shared(abort_addr)) {
@@ -556,11 +594,17 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue: TMEM -> scaled rows ===============================
         I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane, staging + warp * I8_STAGING);
-        int lt = 0;
-        for (int u = blockIdx.x; u < n_units; u += gridDim.x, lt++) {
+        auto request = [&](int i) {
+            if (i >= units.count) return;
+            const I8Unit w = units[i];
+            epi.request(a.ws + ((size_t)w.g * a.RT + w.ct) * I8_M + epi.q * 32, w.row0, w.n);
+        };
+        request(0);
+        for (int lt = 0; lt < units.count; lt++) {
             const int buf = lt & 1;
-            const I8Unit w = i8_unit(a, prefix, u);
-            epi.prepare(a.ws + ((size_t)w.g * a.RT + w.ct) * I8_M + epi.q * 32, w.row0, w.n);
+            const I8Unit w = units[lt];
+            epi.begin();
+            request(lt + 1);
             // the lanes wait one by one and must leave the loop together
             if (!__all_sync(~0u, mbar_wait(&accFull[buf], (lt >> 1) & 1, abort_addr,
                                            I8_WAIT_CYCLES))) {
@@ -579,8 +623,8 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         if (lane == 0) {
             int g = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x) {
-                const I8Unit w = i8_unit(a, prefix, u);
+            for (int i = 0; i < units.count && ok; i++) {
+                const I8Unit w = units[i];
                 const int wrow = (w.g * a.RT + w.ct) * a.KB * I8_M;
                 for (int kb = 0; kb < a.KB; kb++, g++) {
                     const int s = g % S;
@@ -606,8 +650,8 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         if (lane == 0) {
             int g = 0, lt = 0;
             bool ok = true;
-            for (int u = blockIdx.x; u < n_units && ok; u += gridDim.x, lt++) {
-                const I8Unit w = i8_unit(a, prefix, u);
+            for (; lt < units.count && ok; lt++) {
+                const I8Unit w = units[lt];
                 const uint32_t idesc = idesc_i8(I8_M, (w.n + 15) & ~15);
                 const int buf = lt & 1;
                 if (!mbar_wait(&accEmpty[buf], ((lt >> 1) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
@@ -672,7 +716,6 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     extern __shared__ uint8_t smem_raw[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_ctarank();
-    const int first_unit = blockIdx.x >> 1, unit_step = gridDim.x >> 1;
 
     uint8_t *base = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -710,7 +753,9 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     cluster_sync();  // the other CTA's barriers are initialised
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int n_units = prefix[a.G] * a.CT;
+    const I8Units units(a, prefix, blockIdx.x >> 1, gridDim.x >> 1);
+    units.fill(tid, Cfg::THREADS);
+    __syncthreads();
 
     auto fail = [&]() {
         if (!ld_volatile_shared(abort_addr)) {
@@ -722,42 +767,64 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue of this CTA's 128 channels =========================
         I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane, staging + warp * I8_STAGING);
-        int sc = 0;  // accumulators used so far
-        bool ok = true;
-        for (int u = first_unit; u < n_units && ok; u += unit_step) {
-            const I8Unit w = i8_unit(a, prefix, u);
-            const int rt = w.ct * 2 + rank, n0 = i8p_first(w.n);
-            for (int p = 0; p < 2; p++) {
-                const int n = p ? w.n - n0 : n0;
-                if (n == 0) break;
-                const int buf = sc & 1;
-                const int64_t row0 = (int64_t)w.row0 + (p ? n0 : 0);
-                epi.prepare(a.ws + ((size_t)w.g * a.RT + rt) * I8_M + epi.q * 32, row0, n);
-                // the lanes wait one by one and must leave the loop together
-                if (!__all_sync(~0u, mbar_wait(&accFull[buf], (sc >> 1) & 1, abort_addr,
-                                               I8_WAIT_CYCLES))) {
-                    fail();
-                    ok = false;
-                    break;
-                }
-                tc_fence_after();
-                epi.drain(tmem + buf * I8P_PART + ((uint32_t)(epi.q * 32) << 16), row0, n, rt,
-                          [&] {
-                              tc_fence_before();
-                              __syncwarp();
-                              if (lane == 0)
-                                  mbar_arrive_cluster(mapa_shared(smem_u32(&accEmpty[buf]), 0));
-                          });
-                sc++;
+        // parts of units in order; sc: accumulators used so far
+        struct Part {
+            I8Unit w;
+            int64_t row0;
+            int i, p, n;
+        };
+        auto first_part = [&](int i) {
+            Part r{};
+            r.i = i;
+            if (i < units.count) {
+                r.w = units[i];
+                r.row0 = r.w.row0;
+                r.n = i8p_first(r.w.n);
             }
+            return r;
+        };
+        auto request = [&](const Part &r) {
+            if (r.i < units.count)
+                epi.request(a.ws + ((size_t)r.w.g * a.RT + r.w.ct * 2 + rank) * I8_M + epi.q * 32,
+                            r.row0, r.n);
+        };
+        Part cur = first_part(0);
+        request(cur);
+        for (int sc = 0; cur.i < units.count; sc++) {
+            Part next = cur;
+            if (cur.p == 0 && cur.w.n > cur.n) {
+                next.p = 1;
+                next.row0 += cur.n;
+                next.n = cur.w.n - cur.n;
+            } else {
+                next = first_part(cur.i + 1);
+            }
+            const int buf = sc & 1;
+            epi.begin();
+            request(next);
+            // the lanes wait one by one and must leave the loop together
+            if (!__all_sync(~0u, mbar_wait(&accFull[buf], (sc >> 1) & 1, abort_addr,
+                                           I8_WAIT_CYCLES))) {
+                fail();
+                break;
+            }
+            tc_fence_after();
+            epi.drain(tmem + buf * I8P_PART + ((uint32_t)(epi.q * 32) << 16), cur.row0, cur.n,
+                      cur.w.ct * 2 + rank, [&] {
+                          tc_fence_before();
+                          __syncwarp();
+                          if (lane == 0)
+                              mbar_arrive_cluster(mapa_shared(smem_u32(&accEmpty[buf]), 0));
+                      });
+            cur = next;
         }
     } else if (warp == Cfg::LOAD_WARP) {
         // ============ this CTA's half of the loads ================================
         if (lane == 0) {
             int g = 0;
             bool ok = true;
-            for (int u = first_unit; u < n_units && ok; u += unit_step) {
-                const I8Unit w = i8_unit(a, prefix, u);
+            for (int i = 0; i < units.count && ok; i++) {
+                const I8Unit w = units[i];
                 const int wrow = (w.g * a.RT + w.ct * 2 + rank) * a.KB * I8_M;
                 const int n0 = i8p_first(w.n), n1 = w.n - n0;
                 // half of each part's rows, and the boxes that cover them
@@ -818,8 +885,8 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                 }
                 return false;
             };
-            for (int u = first_unit; u < n_units && ok; u += unit_step) {
-                const I8Unit w = i8_unit(a, prefix, u);
+            for (int i = 0; i < units.count && ok; i++) {
+                const I8Unit w = units[i];
                 const int n0 = i8p_first(w.n), n1 = w.n - n0;
                 const uint32_t id0 = idesc_i8(2 * I8_M, (n0 + 31) & ~31);
                 const uint32_t id1 = idesc_i8(2 * I8_M, (n1 + 31) & ~31);
