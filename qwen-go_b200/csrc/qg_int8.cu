@@ -404,12 +404,13 @@ struct I8Epilogue {
     // one (place()).  Two values at a time: mul.f32x2 halves the products, and
     // walking the rows by their pitch instead of multiplying for each halves
     // the rest; the epilogue is bound by its instructions.
+    template <bool WHOLE>
     __device__ __forceinline__ void run(const int (&v)[2][16], uint32_t scales, TO *yp, int nc,
                                         int o0) {
         const int64_t pitch = a.cols;
         if constexpr (LANES) {
             const uint64_t s2 = pack_f32x2(sw[0], sw[0]);
-            const bool mine = o0 + lane < a.cols, whole = nc == 32;
+            const bool mine = o0 + lane < a.cols;
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
                 const ulonglong2 sx = ld_shared_u64x2(scales + c * 4);
@@ -418,7 +419,7 @@ struct I8Epilogue {
                 const float f[4] = {f0.x, f0.y, f1.x, f1.y};
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    if (mine && (whole || c + b < nc)) *yp = f[b];
+                    if (WHOLE || (mine && c + b < nc)) *yp = f[b];
                     yp += pitch;
                 }
             }
@@ -446,9 +447,9 @@ struct I8Epilogue {
                     const int c = i * 8 + co;
 #pragma unroll
                     for (int e = 0; e < 2; e++)
-                        if (o0 + ro + 8 * e < a.cols) {
-                            if (c < nc) yp[8 * e] = f[e].x;
-                            if (c + 1 < nc) yp[pitch + 8 * e] = f[e].y;
+                        if (WHOLE || o0 + ro + 8 * e < a.cols) {
+                            if (WHOLE || c < nc) yp[8 * e] = f[e].x;
+                            if (WHOLE || c + 1 < nc) yp[pitch + 8 * e] = f[e].y;
                         }
                     yp += 8 * pitch;
                 } else {
@@ -462,7 +463,7 @@ struct I8Epilogue {
                         stmatrix4_trans(to + (i & 1) * 8 * I8_ROW_PITCH, p);
                     if (i & 1) {  // 16 rows are staged
                         __syncwarp();
-                        store16(yp, o0, nc - (i / 2) * 16);
+                        store16<WHOLE>(yp, o0, nc - (i / 2) * 16);
                         yp += 16 * pitch;
                         __syncwarp();
                     }
@@ -471,13 +472,16 @@ struct I8Epilogue {
         }
     }
     // The 16 staged rows, nc of them real, from yp on.
+    template <bool WHOLE>
     __device__ __forceinline__ void store16(TO *yp, int o0, int nc) {
         const uint32_t from = staging + (lane / CHUNKS) * I8_ROW_PITCH + (lane % CHUNKS) * 16;
         const int o = o0 + lane % CHUNKS * 8;
 #pragma unroll
         for (int p = 0; p < 16 / ROWS; p++) {
             const uint4 u = ld_shared_v4(from + p * ROWS * I8_ROW_PITCH);
-            if (p * ROWS + lane / CHUNKS < nc) {
+            if constexpr (WHOLE) {
+                *reinterpret_cast<uint4 *>(yp) = u;
+            } else if (p * ROWS + lane / CHUNKS < nc) {
                 if (a.vec) {  // cols % 8 == 0: a chunk is inside or outside
                     if (o < a.cols) *reinterpret_cast<uint4 *>(yp) = u;
                 } else {
@@ -515,6 +519,8 @@ struct I8Epilogue {
     __device__ __forceinline__ void drain(uint32_t tmem, int64_t row0, int n, int rt, F read) {
         const int o0 = (rt * 4 + q) * CH;
         TO *yp = place(row0 + first, o0);
+        // all channels exist (and 16-bit rows are aligned): nothing to check
+        const bool whole = o0 + CH <= a.cols && (F32 || a.vec);
         if (first >= n) read();
 #pragma unroll
         for (int i = 0; i < RUNS; i++) {
@@ -523,7 +529,11 @@ struct I8Epilogue {
                 int v[2][16];
                 fetch(tmem + c0, v);
                 if (i + 1 == RUNS || c0 + SUBS * 32 >= n) read();
-                run(v, staging + I8_SCALES + i * 128, yp, min(32, n - c0), o0);
+                const uint32_t scales = staging + I8_SCALES + i * 128;
+                if (whole && c0 + 32 <= n)
+                    run<true>(v, scales, yp, 32, o0);
+                else
+                    run<false>(v, scales, yp, min(32, n - c0), o0);
                 yp += SUBS * 32 * (int64_t)a.cols;
             }
         }
