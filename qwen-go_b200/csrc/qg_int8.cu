@@ -46,13 +46,7 @@ constexpr int I8_MAX_GROUPS = QG_MAX_EXPERTS;
 constexpr int I8_UNITS = 64;       // units of a CTA decoded once, into shared memory
 constexpr int I8_MAX_IN = 131071;  // 131071 * 128 * 128 < 2^31: exact int32 sums
 constexpr long long I8_WAIT_CYCLES = 4000000000LL;  // ~2 s
-// Epilogue staging of the four warps that share a run of rows (a "sub"): 16
-// rows x 128 16-bit channels as two boxes of 64 channels in the 128B swizzle
-// (so that neither the matrix stores nor the TMA store meet bank conflicts),
-// or one box with SwiGLU.  Then each warp's row scales, up to two runs of 32.
-constexpr int I8_BOX_BYTES = 16 * 128;
-constexpr int I8_SUB_BYTES = 2 * I8_BOX_BYTES;
-constexpr int I8_SCALE_BYTES = 2 * 128;  // per warp
+constexpr int I8_SCALE_BYTES = 2 * 128;  // an epilogue warp's row scales: two runs of 32
 constexpr int I8_SMEM = 232448;  // most shared memory of a CTA
 
 // NT: most rows of a tile.  Stages fill the shared memory that one CTA per SM
@@ -69,7 +63,7 @@ struct I8Cfg {
     static constexpr int LOAD_WARP = EPI_WARPS, MMA_WARP = EPI_WARPS + 1;
     static constexpr int THREADS = (EPI_WARPS + 2) * 32;
     static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12 + I8_UNITS * 16;
-    static constexpr int EPI_BYTES = EPI_WARPS / 4 * I8_SUB_BYTES + EPI_WARPS * I8_SCALE_BYTES;
+    static constexpr int EPI_BYTES = EPI_WARPS * I8_SCALE_BYTES;
     static constexpr int REST = EPI_BYTES + 8 * 5 + 16 + TAB_BYTES + 1024;
     static constexpr int S = (I8_SMEM - REST) / (STAGE_BYTES + 16);  // two barriers a stage
     static constexpr int SMEM = S * (STAGE_BYTES + 16) + REST;
@@ -286,20 +280,12 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, int (&v)[16]) {
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// Four 8x8 matrices of 16-bit pairs, stored transposed: lane l gives the
-// address of stored row l % 8 of matrix l / 8.
-__device__ __forceinline__ void stmatrix4_trans(uint32_t addr, const uint32_t (&r)[4]) {
-    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(
-                     addr),
-                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
-                 : "memory");
-}
-// A box of shared memory to its place in global memory; bulk_group ordering.
-__device__ __forceinline__ void tma_store_2d(const CUtensorMap *map, uint32_t src, int x, int y) {
-    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                     reinterpret_cast<uint64_t>(map)),
-                 "r"(x), "r"(y), "r"(src)
-                 : "memory");
+// Transposes an 8x8 matrix of 16-bit values across the warp: thread l gives
+// the pair (row l/4, columns 2(l%4), + 1) and gets (row 2(l%4), + 1, column
+// l/4).
+__device__ __forceinline__ uint32_t movmatrix(uint32_t v) {
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
+    return v;
 }
 // Two float32 in a register pair: (float(a), float(b)) * s * t.
 __device__ __forceinline__ uint64_t pack_f32x2(float a, float b) {
@@ -348,55 +334,36 @@ __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 *, float a, float b) {
 // activations are, and the sum times it may overflow where y does not.
 //   float32, plain: a lane is a channel, a store 32 neighbouring ones of a row.
 //   SwiGLU: of a quarter's 32 weight rows the first 16 are gate, the others
-//     the up rows of the same 16 channels (k_i8_layout); read 16 lanes at a
-//     time, both land in the same thread.
-//   16-bit: pairs of rows packed in a thread, transposed into the staging that
-//     the four quarters' warps of a run share, 16 rows at a time; these leave
-//     as TMA stores, which the warps do not wait for (their own 16-byte stores
-//     held them for half of the epilogue), or, where the run ends inside the
-//     32 rows or y is not 16-byte aligned, row by row.
+//     the up rows of the same 16 channels; read 16 lanes at a time, both land
+//     in the same thread.
+//   16-bit: pairs of rows packed in a thread and transposed across the warp
+//     (movmatrix), so that a thread has pairs of channels of one row; the order
+//     of the weight rows (i8_channel) makes a thread's pairs neighbours, which
+//     leave as one 16-byte store (8 bytes with SwiGLU).  Staged in shared
+//     memory instead, the barriers and the waits for the staging to be read
+//     cost as much as the conversion: 4096 x 128 x 4096, mostly epilogue, took
+//     12.7 us with TMA stores and takes 10.3.
 // An accumulator's scales are requested while the one before it is waited for
 // and converted.
+__host__ __device__ __forceinline__ int i8_channel(int row, bool swiglu) {  // of 32 (16) rows
+    const int m = row / 8, j = row % 8 / 2, b = row & 1;
+    return (swiglu ? 4 : 8) * j + 2 * m + b;
+}
 template <typename TO, bool SWIGLU, int SUBS>
 struct I8Epilogue {
     static constexpr bool F32 = sizeof(TO) == 4;
     static constexpr bool LANES = F32 && !SWIGLU;  // a lane is a channel
     static constexpr int CH = SWIGLU ? 16 : 32;    // channels of this warp
-    static constexpr int CHUNKS = CH / 2;  // 16-byte chunks of a staged row: four quarters
     static constexpr int RUNS = SUBS == 4 ? 2 : 1;  // of an accumulator, per warp
 
     const I8Args &a;
-    const CUtensorMap *tmap_y;
-    int q, sub, first, lane;  // first: row column of this warp's first run
-    uint32_t box, scales;
+    int q, first, lane;  // first: row column of this warp's first run
+    uint32_t scales;
     float sw[4], next_sw[4];  // scales of the weight rows this thread converts
     float next_sx[RUNS];
 
-    // staging: the subs' boxes, then the warps' scales
-    __device__ __forceinline__ I8Epilogue(const I8Args &a, const CUtensorMap *tmap_y, int warp,
-                                          int lane, uint32_t staging)
-        : a(a), tmap_y(tmap_y), q(warp & 3), sub(warp >> 2), first(sub * 32), lane(lane),
-          box(staging + sub * I8_SUB_BYTES),
-          scales(staging + SUBS * I8_SUB_BYTES + warp * I8_SCALE_BYTES) {}
-    __device__ __forceinline__ bool issuer() const { return q == 0 && lane == 0; }
-    // the four warps of this sub
-    __device__ __forceinline__ void sync_sub() const {
-        asm volatile("bar.sync %0, 128;" ::"r"(sub + 1) : "memory");
-    }
-
-    // Whether all of them, or this warp alone, may go on: a run has barriers of
-    // the sub's warps, which must leave together or not at all.
-    __device__ __forceinline__ bool agree(bool ok) const {
-        if constexpr (F32) return __all_sync(~0u, ok);
-        uint32_t r;
-        asm volatile(
-            "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %2, 0;\n\t"
-            "barrier.cta.red.and.pred p, %1, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(r)
-            : "r"(sub + 1), "r"((uint32_t)ok)
-            : "memory");
-        return r != 0;
-    }
+    __device__ __forceinline__ I8Epilogue(const I8Args &a, int warp, int lane, uint32_t scales)
+        : a(a), q(warp & 3), first(warp / 4 * 32), lane(lane), scales(scales) {}
 
     // The scales of an accumulator's rows (xs) and of this quarter's 32
     // channels (ws), in flight until begin() of that accumulator.
@@ -437,13 +404,12 @@ struct I8Epilogue {
     // values at a time: mul.f32x2 halves the instructions of the products.
     template <bool WHOLE>
     __device__ __forceinline__ void run(const int (&v)[2][16], uint32_t sx_at, int64_t r0, int nc,
-                                        int rt) {
-        const int o0 = (rt * 4 + q) * CH;
+                                        int o0) {
         const int64_t pitch = a.cols;
         if constexpr (LANES) {
             const uint64_t s2 = pack_f32x2(sw[0], sw[0]);
-            const bool mine = o0 + lane < a.cols;
-            TO *yp = static_cast<TO *>(a.y) + r0 * pitch + o0 + lane;
+            const int o = o0 + i8_channel(lane, false);
+            TO *yp = static_cast<TO *>(a.y) + r0 * pitch + o;
 #pragma unroll
             for (int c = 0; c < 32; c += 4) {
                 const ulonglong2 sx = ld_shared_u64x2(sx_at + c * 4);
@@ -452,103 +418,58 @@ struct I8Epilogue {
                 const float f[4] = {f0.x, f0.y, f1.x, f1.y};
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    if (WHOLE || (mine && c + b < nc)) *yp = f[b];
+                    if (WHOLE || (o < a.cols && c + b < nc)) *yp = f[b];
                     yp += pitch;
                 }
             }
         } else {
             const int ro = lane >> 2, co = (lane & 3) * 2;
-            // this lane's row address for the matrix stores: 16-byte chunk
-            // q * CH / 8 + (matrix) of a staged row
-            const int chunk = SWIGLU ? q * 2 + ((lane >> 3) & 1) : (q & 1) * 4 + (lane >> 3);
-            const uint32_t to = box + (SWIGLU ? 0 : (q >> 1) * I8_BOX_BYTES) + (lane & 7) * 128 +
-                                ((chunk ^ (lane & 7)) << 4);
-            TO *yp = static_cast<TO *>(a.y) + (r0 + co) * pitch + o0 + ro;  // float32 SwiGLU
+            constexpr int N = SWIGLU ? 4 : 8;  // channels of a thread's store
+            const int o = F32 ? o0 + i8_channel(ro, true) : o0 + (lane & 3) * N;
+            TO *yp = static_cast<TO *>(a.y) + (r0 + (F32 ? co : ro)) * pitch + o;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {  // 16 rows
-                uint32_t p[2][4];
+            for (int i = 0; i < 4; i++) {
+                const uint64_t sx = ld_shared_u64(sx_at + (i * 8 + co) * 4);
+                float2 f[4];  // weight rows ro + 8e, a pair of rows each
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int i = h * 2 + k;
-                    const uint64_t sx = ld_shared_u64(sx_at + (i * 8 + co) * 4);
-                    float2 f[4];  // weight rows ro + 8e, a pair of rows each
+                for (int e = 0; e < 4; e++) {
+                    const int *x = &v[e >> 1][i * 4 + (e & 1) * 2];
+                    f[e] = scaled(x[0], x[1], pack_f32x2(sw[e], sw[e]), sx);
+                }
+                if constexpr (SWIGLU) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int *x = &v[e >> 1][i * 4 + (e & 1) * 2];
-                        f[e] = scaled(x[0], x[1], pack_f32x2(sw[e], sw[e]), sx);
-                    }
-                    if constexpr (SWIGLU) {
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            f[e].x = swiglu(f[e].x, f[2 + e].x);
-                            f[e].y = swiglu(f[e].y, f[2 + e].y);
-                        }
-                    }
-                    if constexpr (F32) {  // eight neighbouring channels of four rows per store
-                        const int c = i * 8 + co;
-#pragma unroll
-                        for (int e = 0; e < 2; e++)
-                            if (WHOLE || o0 + ro + 8 * e < a.cols) {
-                                if (WHOLE || c < nc) yp[8 * e] = f[e].x;
-                                if (WHOLE || c + 1 < nc) yp[pitch + 8 * e] = f[e].y;
-                            }
-                        yp += 8 * pitch;
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < (SWIGLU ? 2 : 4); e++)
-                            p[k][e] = pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y);
+                    for (int e = 0; e < 2; e++) {
+                        f[e].x = swiglu(f[e].x, f[2 + e].x);
+                        f[e].y = swiglu(f[e].y, f[2 + e].y);
                     }
                 }
-                if constexpr (!F32) {
-                    // the staging is free once the last TMA store has read it
-                    if (issuer()) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-                    sync_sub();
+                if constexpr (F32) {  // pairs of channels of four rows per store
+                    const int c = i * 8 + co;
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
+                    for (int e = 0; e < 2; e++)
+                        if (WHOLE || o + 2 * e < a.cols) {
+                            if (WHOLE || c < nc) yp[2 * e] = f[e].x;
+                            if (WHOLE || c + 1 < nc) yp[pitch + 2 * e] = f[e].y;
+                        }
+                } else {
+                    uint32_t p[N / 2];
+#pragma unroll
+                    for (int e = 0; e < N / 2; e++)
+                        p[e] = movmatrix(pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y));
+                    if (WHOLE || (a.vec && i * 8 + ro < nc && o < a.cols)) {
                         if constexpr (SWIGLU)
-                            stmatrix2_trans(to + k * 1024, p[k][0], p[k][1]);
+                            *reinterpret_cast<uint2 *>(yp) = make_uint2(p[0], p[1]);
                         else
-                            stmatrix4_trans(to + k * 1024, p[k]);
-                    }
-                    if (WHOLE) fence_proxy_async_smem();
-                    sync_sub();
-                    if constexpr (WHOLE) {
-                        if (issuer()) {
+                            *reinterpret_cast<uint4 *>(yp) = make_uint4(p[0], p[1], p[2], p[3]);
+                    } else if (!a.vec && i * 8 + ro < nc) {
 #pragma unroll
-                            for (int b = 0; b < (SWIGLU ? 1 : 2); b++) {
-                                const int x = rt * 4 * CH + b * 64;
-                                if (x < a.cols)
-                                    tma_store_2d(tmap_y, box + b * I8_BOX_BYTES, x,
-                                                 (int)r0 + h * 16);
-                            }
-                            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-                        }
-                    } else {
-                        store16(r0 + h * 16, nc - h * 16, rt);
+                        for (int e = 0; e < N; e++)
+                            if (o + e < a.cols)
+                                reinterpret_cast<uint16_t *>(yp)[e] =
+                                    (uint16_t)(p[e >> 1] >> (16 * (e & 1)));
                     }
                 }
-            }
-        }
-    }
-    // The 16 staged rows of all four quarters, nc of them real, by this
-    // sub's 128 threads.
-    __device__ __forceinline__ void store16(int64_t r0, int nc, int rt) {
-#pragma unroll
-        for (int i = q * 32 + lane; i < 16 * CHUNKS; i += 128) {
-            const int c = i / CHUNKS, ch = i % CHUNKS, o = rt * 4 * CH + ch * 8;
-            if (c >= nc) break;  // rows ascend with i
-            const uint4 u = ld_shared_v4(box + ch / 8 * I8_BOX_BYTES + c * 128 +
-                                         (((ch & 7) ^ (c & 7)) << 4));
-            TO *yp = static_cast<TO *>(a.y) + (r0 + c) * a.cols + o;
-            if (a.vec) {  // cols % 8 == 0: a chunk is inside or outside
-                if (o < a.cols) *reinterpret_cast<uint4 *>(yp) = u;
-            } else {
-                const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (o + e < a.cols)
-                        reinterpret_cast<uint16_t *>(yp)[e] =
-                            (uint16_t)(w[e >> 1] >> (16 * (e & 1)));
+                yp += 8 * pitch;
             }
         }
     }
@@ -558,9 +479,9 @@ struct I8Epilogue {
     // of them are converted.
     template <typename F>
     __device__ __forceinline__ void drain(uint32_t tmem, int64_t row0, int n, int rt, F read) {
-        // nothing to check per value: float32, all channels exist; 16 bits,
-        // the TMA store leaves out those that do not
-        const bool whole = F32 ? (rt * 4 + q + 1) * CH <= a.cols : a.vec;
+        const int o0 = (rt * 4 + q) * CH;
+        // all channels exist (and 16-bit rows are aligned): nothing to check
+        const bool whole = o0 + CH <= a.cols && (F32 || a.vec);
         if (first >= n) read();
 #pragma unroll
         for (int i = 0; i < RUNS; i++) {
@@ -570,17 +491,12 @@ struct I8Epilogue {
                 fetch(tmem + c0, v);
                 if (i + 1 == RUNS || c0 + SUBS * 32 >= n) read();
                 if (whole && c0 + 32 <= n)
-                    run<true>(v, scales + i * 128, row0 + c0, 32, rt);
+                    run<true>(v, scales + i * 128, row0 + c0, 32, o0);
                 else
-                    run<false>(v, scales + i * 128, row0 + c0, min(32, n - c0), rt);
+                    run<false>(v, scales + i * 128, row0 + c0, min(32, n - c0), o0);
             }
         }
         __syncwarp();  // the scales are written again
-    }
-    // The TMA stores have been made, before the shared memory goes.
-    __device__ __forceinline__ void finish() const {
-        if (!F32 && issuer()) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-        __syncwarp();
     }
 };
 
@@ -588,7 +504,7 @@ struct I8Epilogue {
 template <int NT, typename TO, bool SWIGLU>
 __global__ void __launch_bounds__(I8Cfg<NT>::THREADS, 1)
 k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-     const __grid_constant__ CUtensorMap tmap_y, const I8Args a) {
+     const I8Args a) {
     pdl_launch_dependents();
     using Cfg = I8Cfg<NT>;
     constexpr int S = Cfg::S;
@@ -597,7 +513,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     uint8_t *base = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
+    const uint32_t scales = smem_u32(base + S * Cfg::STAGE_BYTES);
     uint64_t *full =
         reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES + Cfg::EPI_BYTES);
     uint64_t *empty = full + S;
@@ -646,7 +562,8 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue: TMEM -> scaled rows ===============================
-        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, &tmap_y, warp, lane, staging);
+        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane,
+                                                       scales + warp * I8_SCALE_BYTES);
         auto request = [&](int i) {
             if (i >= units.count) return;
             const I8Unit w = units[i];
@@ -658,7 +575,9 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
             const I8Unit w = units[lt];
             epi.begin();
             request(lt + 1);
-            if (!epi.agree(mbar_wait(&accFull[buf], (lt >> 1) & 1, abort_addr, I8_WAIT_CYCLES))) {
+            // the lanes wait one by one and must leave the loop together
+            if (!__all_sync(~0u, mbar_wait(&accFull[buf], (lt >> 1) & 1, abort_addr,
+                                           I8_WAIT_CYCLES))) {
                 fail();
                 break;
             }
@@ -669,7 +588,6 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
                 if (lane == 0) mbar_arrive(&accEmpty[buf]);
             });
         }
-        epi.finish();
     } else if (warp == Cfg::LOAD_WARP) {
         // ============ loads: weight tile and row tile of each 128-code block ======
         if (lane == 0) {
@@ -761,7 +679,7 @@ __device__ __forceinline__ int i8p_first(int n) {  // rows of the first part
 template <typename TO, bool SWIGLU>
 __global__ void __launch_bounds__(I8Pair::THREADS, 1)
 k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtensorMap tmap_x,
-          const __grid_constant__ CUtensorMap tmap_y, const I8Args a) {
+          const I8Args a) {
     pdl_launch_dependents();
     using Cfg = I8Pair;
     constexpr int S = Cfg::S;
@@ -771,7 +689,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 
     uint8_t *base = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t staging = smem_u32(base + S * Cfg::STAGE_BYTES);
+    const uint32_t scales = smem_u32(base + S * Cfg::STAGE_BYTES);
     uint64_t *full =
         reinterpret_cast<uint64_t *>(base + S * Cfg::STAGE_BYTES + Cfg::EPI_BYTES);
     uint64_t *empty = full + S;
@@ -818,7 +736,8 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue of this CTA's 128 channels =========================
-        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, &tmap_y, warp, lane, staging);
+        I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane,
+                                                       scales + warp * I8_SCALE_BYTES);
         // parts of units in order; sc: accumulators used so far
         struct Part {
             I8Unit w;
@@ -854,7 +773,9 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
             const int buf = sc & 1;
             epi.begin();
             request(next);
-            if (!epi.agree(mbar_wait(&accFull[buf], (sc >> 1) & 1, abort_addr, I8_WAIT_CYCLES))) {
+            // the lanes wait one by one and must leave the loop together
+            if (!__all_sync(~0u, mbar_wait(&accFull[buf], (sc >> 1) & 1, abort_addr,
+                                           I8_WAIT_CYCLES))) {
                 fail();
                 break;
             }
@@ -868,7 +789,6 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                       });
             cur = next;
         }
-        epi.finish();
     } else if (warp == Cfg::LOAD_WARP) {
         // ============ this CTA's half of the loads ================================
         if (lane == 0) {
@@ -1017,13 +937,16 @@ __global__ void k_i8_layout(const int8_t *q, const float *scale, int O, int I, i
     const int64_t row = blockIdx.x, tile = row / I8_M;  // of groups * RT * 128
     const int g = (int)(tile / RT);
     const int l = (int)(row - (int64_t)g * RT * I8_M);
-    int o = l;
-    bool live = l < O;
+    const int rt = l / I8_M, quarter = l % I8_M / 32, r = l % 32;
+    int o;
+    bool live;
     if (swiglu) {
-        const int rt = l / I8_M, r = l % I8_M, cols = O / 2;
-        const int c = rt * 64 + (r / 32) * 16 + (r & 15);
+        const int cols = O / 2, c = rt * 64 + quarter * 16 + i8_channel(r & 15, true);
         live = c < cols;
         o = (r & 16) ? cols + c : c;
+    } else {
+        o = rt * I8_M + quarter * 32 + i8_channel(r, false);
+        live = o < O;
     }
     const int8_t *src = q + ((int64_t)g * O + o) * I;
     int8_t *d = dst + (tile * KB * I8_M + row % I8_M) * I8_BK;
@@ -1053,26 +976,22 @@ static PFN_cuTensorMapEncodeTiled_v12000 i8_encode_fn() {
     return fn;
 }
 
-// 2-D [rows, cols] with row pitch ld bytes, boxes of 128-byte rows, 128B
-// swizzle, zeros beyond the edges.
-static int i8_encode(CUtensorMap *map, CUtensorMapDataType type, const void *ptr, int64_t rows,
-                     int64_t cols, int64_t ld, int box_cols, int box_rows) {
+// 2-D int8 [rows, cols] with row pitch ld bytes, boxes of 128 codes x box_rows
+// rows, 128B swizzle, zeros beyond the edges.
+static int i8_encode_map(CUtensorMap *map, const int8_t *ptr, int64_t rows, int cols, int64_t ld,
+                         int box_rows) {
     auto fn = i8_encode_fn();
     if (!fn) return set_error(QGMOE_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
     cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
     cuuint64_t strides[1] = {(cuuint64_t)ld};
-    cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    cuuint32_t box[2] = {I8_BK, (cuuint32_t)box_rows};
     cuuint32_t estr[2] = {1, 1};
-    CUresult r = fn(map, type, 2, const_cast<void *>(ptr), dims, strides, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+    CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<int8_t *>(ptr), dims, strides,
+                    box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS)
         return set_error(QGMOE_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return QGMOE_OK;
-}
-static int i8_encode_codes(CUtensorMap *map, const int8_t *ptr, int64_t rows, int cols, int64_t ld,
-                           int box_rows) {
-    return i8_encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, ptr, rows, cols, ld, I8_BK, box_rows);
 }
 
 // Makes `device` current for a call and puts the caller's device back.
@@ -1124,12 +1043,8 @@ static int i8_tile(int64_t rows_per_group) {
     return rows_per_group <= 16 ? 16 : rows_per_group <= 64 ? 64 : I8P_NT;
 }
 
-struct I8Maps {  // of the row codes and of y
-    CUtensorMap x, y;
-};
-
 template <typename TO, bool SWIGLU>
-static int launch_i8_pair_t(const qgq8 *h, const I8Maps &m, const I8Args &a, int64_t max_units,
+static int launch_i8_pair_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
                             cudaStream_t s) {
     auto kern = k_i8_pair<TO, SWIGLU>;
     constexpr int smem = I8Pair::SMEM;
@@ -1158,12 +1073,12 @@ static int launch_i8_pair_t(const qgq8 *h, const I8Maps &m, const I8Args &a, int
     }
     cfg.gridDim = dim3(2 * (unsigned)(max_units < n ? max_units : n));
     cfg.numAttrs = 2;
-    QG_CUDA(cudaLaunchKernelEx(&cfg, kern, h->tmap_w, m.x, m.y, a));
+    QG_CUDA(cudaLaunchKernelEx(&cfg, kern, h->tmap_w, tx, a));
     return QGMOE_OK;
 }
 
 template <int NT, typename TO, bool SWIGLU>
-static int launch_i8_cta_t(const qgq8 *h, const I8Maps &m, const I8Args &a,
+static int launch_i8_cta_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a,
                            int64_t max_units, cudaStream_t s) {
     auto kern = k_i8<NT, TO, SWIGLU>;
     constexpr int smem = I8Cfg<NT>::SMEM;
@@ -1175,29 +1090,29 @@ static int launch_i8_cta_t(const qgq8 *h, const I8Maps &m, const I8Args &a,
     int64_t grid = num_sms(h->device);
     if (max_units < grid) grid = max_units;
     QG_CUDA(launch_pdl(kern, dim3((unsigned)grid), dim3(I8Cfg<NT>::THREADS), smem, s, 1, h->tmap_w,
-                       m.x, m.y, a));
+                       tx, a));
     return QGMOE_OK;
 }
 
 template <int NT, typename TO, bool SWIGLU>
-static int launch_i8_t(const qgq8 *h, const I8Maps &m, const I8Args &a, int64_t max_units,
+static int launch_i8_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
                        cudaStream_t s) {
     if constexpr (NT == I8P_NT)
-        return launch_i8_pair_t<TO, SWIGLU>(h, m, a, max_units, s);
+        return launch_i8_pair_t<TO, SWIGLU>(h, tx, a, max_units, s);
     else
-        return launch_i8_cta_t<NT, TO, SWIGLU>(h, m, a, max_units, s);
+        return launch_i8_cta_t<NT, TO, SWIGLU>(h, tx, a, max_units, s);
 }
 
 template <int NT>
-static int launch_i8(const qgq8 *h, const I8Maps &m, const I8Args &a, int ydt, int64_t units,
+static int launch_i8(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int ydt, int64_t units,
                      cudaStream_t s) {
     if (h->swiglu)
-        return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, true>(h, m, a, units, s)
-               : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, true>(h, m, a, units, s)
-                                     : launch_i8_t<NT, __nv_bfloat16, true>(h, m, a, units, s);
-    return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, false>(h, m, a, units, s)
-           : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, false>(h, m, a, units, s)
-                                 : launch_i8_t<NT, __nv_bfloat16, false>(h, m, a, units, s);
+        return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, true>(h, tx, a, units, s)
+               : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, true>(h, tx, a, units, s)
+                                     : launch_i8_t<NT, __nv_bfloat16, true>(h, tx, a, units, s);
+    return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, false>(h, tx, a, units, s)
+           : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, false>(h, tx, a, units, s)
+                                 : launch_i8_t<NT, __nv_bfloat16, false>(h, tx, a, units, s);
 }
 
 static int i8_check_product(const qgq8 *h, const int8_t *codes, int64_t ld, const float *scale,
@@ -1224,16 +1139,8 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     const int64_t per = (R + (int64_t)h->G - 1) / h->G;  // mean rows of a group
     const int nt = i8_tile(per);
     CUtensorMap tx;
-    int rc = i8_encode_codes(&tx, codes, R, h->I, ld, nt < I8P_BOX ? nt : I8P_BOX);
+    int rc = i8_encode_map(&tx, codes, R, h->I, ld, nt < I8P_BOX ? nt : I8P_BOX);
     if (rc) return rc;
-    // 16-bit y whose rows are 16-byte aligned: whole runs leave by TMA
-    const int vec = ydt != QGMOE_DT_F32 && h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
-    CUtensorMap ty = tx;  // not used otherwise
-    if (vec) {
-        rc = i8_encode(&ty, CU_TENSOR_MAP_DATA_TYPE_UINT16, y, R, h->cols, (int64_t)h->cols * 2, 64,
-                       16);
-        if (rc) return rc;
-    }
     I8Args a{};
     a.xs = scale;
     a.ws = h->ws;
@@ -1248,15 +1155,14 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     a.nt = nt;
     a.gran = pair ? 32 : 16;
     a.y = y;
-    a.vec = vec;
+    a.vec = h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
     a.err = h->err_dev;
     // row tiles: full ones, and at most one partial for each group that has rows
     const int64_t tiles = R / nt + (R < h->G ? R : h->G);
     const int64_t units = tiles * a.CT;
-    const I8Maps m{tx, ty};
-    return nt == 16   ? launch_i8<16>(h, m, a, ydt, units, s)
-           : nt == 64 ? launch_i8<64>(h, m, a, ydt, units, s)
-                      : launch_i8<I8P_NT>(h, m, a, ydt, units, s);
+    return nt == 16   ? launch_i8<16>(h, tx, a, ydt, units, s)
+           : nt == 64 ? launch_i8<64>(h, tx, a, ydt, units, s)
+                      : launch_i8<I8P_NT>(h, tx, a, ydt, units, s);
 }
 
 static void i8_free_work(qgq8 *h) {
@@ -1284,7 +1190,7 @@ static int i8_build(qgq8 *h, const int8_t *q, const float *scale, bool on_device
     int rc = i8_alloc(reinterpret_cast<void **>(&h->w), (size_t)(rows * row_bytes));
     if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->ws), sizeof(float) * rows);
     if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->err_dev), sizeof(int));
-    if (!rc) rc = i8_encode_codes(&h->tmap_w, h->w, rows * h->KB, I8_BK, I8_BK, I8_M);
+    if (!rc) rc = i8_encode_map(&h->tmap_w, h->w, rows * h->KB, I8_BK, I8_BK, I8_M);
     if (rc) return rc;
     QG_CUDA(cudaMemsetAsync(h->err_dev, 0, sizeof(int), h->stream));
     const int64_t gbytes = (int64_t)h->O * h->I;
