@@ -78,6 +78,7 @@ constexpr int I8P_BOX = 64;
 constexpr int I8P_HALF_BYTES = I8P_PART / 2 * I8_BK;
 // Stages whose second part waits at the start and the end of a tile (below).
 constexpr int I8P_STAGGER = 2;
+static_assert(I8P_STAGGER >= 1, "the accumulators' commits rely on it");
 using I8Pair = I8Cfg<I8P_PART>;
 
 struct I8Args {
@@ -158,6 +159,59 @@ __device__ __forceinline__ void tma_load_2d_pair(void *dst, const CUtensorMap *m
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar)
                  : "memory");
+}
+
+// ---- the issuing warps -----------------------------------------------------------
+// The MMA and the loading warp run their loops with all lanes and elect one for
+// each instruction: its operands are then the same in all lanes as far as the
+// compiler can see and stay in uniform registers.  Issued by a thread alone,
+// a block's four MMAs took 290 cycles to issue whatever their size, more than
+// those of a tile of 128 rows take to run.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(r));
+    return r != 0;
+}
+template <int S> struct I8Ring {
+    uint32_t s = 0, phase = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == S) {
+            s = 0;
+            phase ^= 1;
+        }
+    }
+    __device__ __forceinline__ void prev() {
+        if (s-- == 0) {
+            s = S - 1;
+            phase ^= 1;
+        }
+    }
+};
+__device__ __forceinline__ bool i8_try_wait(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __noinline__ bool i8_wait_slow(uint32_t bar, uint32_t parity, uint32_t abort_addr) {
+    const long long t0 = clock64();
+    while (!i8_try_wait(bar, parity)) {
+        if (abort_addr && ld_volatile_shared(abort_addr)) return false;
+        if (clock64() - t0 > I8_WAIT_CYCLES) return false;
+    }
+    return true;
+}
+// All lanes; the same answer in all of them.
+__device__ __forceinline__ bool i8_wait(uint32_t bar, uint32_t parity, uint32_t abort_addr) {
+    if (__all_sync(~0u, i8_try_wait(bar, parity))) return true;
+    return __all_sync(~0u, i8_wait_slow(bar, parity, abort_addr));
 }
 
 // ---- units ---------------------------------------------------------------------
@@ -590,64 +644,67 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         }
     } else if (warp == Cfg::LOAD_WARP) {
         // ============ loads: weight tile and row tile of each 128-code block ======
-        if (lane == 0) {
-            int g = 0;
+        {
+            I8Ring<S> r;
+            int loads = 0;
             bool ok = true;
+            const uint32_t empty0 = smem_u32(empty);
             for (int i = 0; i < units.count && ok; i++) {
                 const I8Unit w = units[i];
                 const int wrow = (w.g * a.RT + w.ct) * a.KB * I8_M;
-                for (int kb = 0; kb < a.KB; kb++, g++) {
-                    const int s = g % S;
-                    if (!mbar_wait(&empty[s], ((g / S) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
-                        fail();
-                        ok = false;
-                        break;
+                for (int kb = 0; kb < a.KB; kb++) {
+                    if (!(ok = i8_wait(empty0 + 8 * r.s, r.phase ^ 1, abort_addr))) break;
+                    if (elect_one()) {
+                        uint8_t *dst = base + r.s * Cfg::STAGE_BYTES;
+                        mbar_arrive_expect_tx(&full[r.s], Cfg::STAGE_BYTES);
+                        tma_load_2d(dst, &tmap_w, 0, wrow + kb * I8_M, &full[r.s]);
+                        tma_load_2d(dst + Cfg::A_BYTES, &tmap_x, kb * I8_BK, w.row0, &full[r.s]);
                     }
-                    uint8_t *dst = base + s * Cfg::STAGE_BYTES;
-                    mbar_arrive_expect_tx(&full[s], Cfg::STAGE_BYTES);
-                    tma_load_2d(dst, &tmap_w, 0, wrow + kb * I8_M, &full[s]);
-                    tma_load_2d(dst + Cfg::A_BYTES, &tmap_x, kb * I8_BK, w.row0, &full[s]);
+                    __syncwarp();
+                    loads = min(loads + 1, S);
+                    r.next();
                 }
             }
+            if (!ok) fail();
             // our own copies land before the shared memory goes, also when
             // another role gave up
-            for (int i = g > S ? g - S : 0; i < g; i++)
-                mbar_wait(&full[i % S], (i / S) & 1, 0, I8_WAIT_CYCLES);
+            for (; loads > 0; loads--) {
+                r.prev();
+                i8_wait(smem_u32(&full[r.s]), r.phase, 0);
+            }
         }
         __syncwarp();
     } else {
         // ============ MMA issuer ===================================================
-        if (lane == 0) {
-            int g = 0, lt = 0;
+        {
+            I8Ring<S> r;
             bool ok = true;
-            for (; lt < units.count && ok; lt++) {
-                const I8Unit w = units[lt];
-                const uint32_t idesc = idesc_i8(I8_M, (w.n + 15) & ~15);
+            const uint64_t da = desc_k_sw128(smem_u32(base));
+            const uint64_t db = desc_k_sw128(smem_u32(base) + Cfg::A_BYTES);
+            const uint32_t full0 = smem_u32(full);
+            for (int lt = 0; lt < units.count && ok; lt++) {
+                const uint32_t idesc = idesc_i8(I8_M, (units[lt].n + 15) & ~15);
                 const int buf = lt & 1;
-                if (!mbar_wait(&accEmpty[buf], ((lt >> 1) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
-                    fail();
-                    ok = false;
+                if (!(ok = i8_wait(smem_u32(&accEmpty[buf]), ((lt >> 1) & 1) ^ 1, abort_addr)))
                     break;
-                }
                 tc_fence_after();
-                for (int kb = 0; kb < a.KB; kb++, g++) {
-                    const int s = g % S;
-                    if (!mbar_wait(&full[s], (g / S) & 1, abort_addr, I8_WAIT_CYCLES)) {
-                        fail();
-                        ok = false;
-                        break;
-                    }
+                for (int kb = 0; kb < a.KB; kb++) {
+                    if (!(ok = i8_wait(full0 + 8 * r.s, r.phase, abort_addr))) break;
                     tc_fence_after();
-                    const uint32_t st = smem_u32(base + s * Cfg::STAGE_BYTES);
-                    umma_i8_k128(tmem + buf * Cfg::BUF, desc_k_sw128(st),
-                                 desc_k_sw128(st + Cfg::A_BYTES), idesc, kb != 0);
-                    umma_commit(&empty[s]);
+                    const uint32_t at = r.s * (Cfg::STAGE_BYTES >> 4);
+                    if (elect_one()) {
+                        umma_i8_k128(tmem + buf * Cfg::BUF, da + at, db + at, idesc, kb != 0);
+                        umma_commit(&empty[r.s]);
+                        if (kb + 1 == a.KB) umma_commit(&accFull[buf]);
+                    }
+                    __syncwarp();
+                    r.next();
                 }
-                if (ok) umma_commit(&accFull[buf]);
             }
             if (!ok) {
-                umma_commit(drain);
-                mbar_wait(drain, 0, 0, I8_WAIT_CYCLES);
+                fail();
+                if (elect_one()) umma_commit(drain);
+                i8_wait(smem_u32(drain), 0, 0);
             }
         }
         __syncwarp();
@@ -791,9 +848,12 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         }
     } else if (warp == Cfg::LOAD_WARP) {
         // ============ this CTA's half of the loads ================================
-        if (lane == 0) {
-            int g = 0;
+        {
+            I8Ring<S> r;
+            int loads = 0;
             bool ok = true;
+            const uint32_t empty0 = smem_u32(empty);
+            const uint32_t full0 = mapa_shared(smem_u32(full), 0);  // CTA 0's
             for (int i = 0; i < units.count && ok; i++) {
                 const I8Unit w = units[i];
                 const int wrow = (w.g * a.RT + w.ct * 2 + rank) * a.KB * I8_M;
@@ -803,33 +863,36 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                 const int b0 = (h0 + I8P_BOX - 1) / I8P_BOX, b1 = (h1 + I8P_BOX - 1) / I8P_BOX;
                 const int r0 = w.row0 + rank * h0, r1 = w.row0 + n0 + rank * h1;
                 const uint32_t bytes = 2 * (Cfg::A_BYTES + (b0 + b1) * I8P_BOX * I8_BK);
-                for (int kb = 0; kb < a.KB; kb++, g++) {
-                    const int s = g % S;
-                    if (!mbar_wait(&empty[s], ((g / S) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
-                        fail();
-                        ok = false;
-                        break;
+                for (int kb = 0; kb < a.KB; kb++) {
+                    if (!(ok = i8_wait(empty0 + 8 * r.s, r.phase ^ 1, abort_addr))) break;
+                    if (elect_one()) {
+                        uint8_t *dst = base + r.s * Cfg::STAGE_BYTES, *dx = dst + Cfg::A_BYTES;
+                        if (rank == 0) mbar_arrive_expect_tx(&full[r.s], bytes);
+                        const uint32_t bar = full0 + 8 * r.s;
+                        const int x = kb * I8_BK;
+                        tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
+                        for (int b = 0; b < b0; b++)
+                            tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x,
+                                             r0 + b * I8P_BOX, bar);
+                        for (int b = 0; b < b1; b++)
+                            tma_load_2d_pair(dx + I8P_HALF_BYTES + b * I8P_BOX * I8_BK, &tmap_x, x,
+                                             r1 + b * I8P_BOX, bar);
                     }
-                    uint8_t *dst = base + s * Cfg::STAGE_BYTES, *dx = dst + Cfg::A_BYTES;
-                    if (rank == 0) mbar_arrive_expect_tx(&full[s], bytes);
-                    const uint32_t bar = mapa_shared(smem_u32(&full[s]), 0);
-                    const int x = kb * I8_BK;
-                    tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
-                    for (int b = 0; b < b0; b++)
-                        tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x, r0 + b * I8P_BOX,
-                                         bar);
-                    for (int b = 0; b < b1; b++)
-                        tma_load_2d_pair(dx + I8P_HALF_BYTES + b * I8P_BOX * I8_BK, &tmap_x, x,
-                                         r1 + b * I8P_BOX, bar);
+                    __syncwarp();
+                    loads = min(loads + 1, S);
+                    r.next();
                 }
             }
+            if (!ok) fail();
             // the pair's copies land before the shared memory goes: CTA 0 sees
             // them on its barriers and CTA 1 leaves with it (below); when a
             // role gave up, some may not be counted there, and both CTAs give
             // them time
             if (rank == 0)
-                for (int i = g > S ? g - S : 0; i < g; i++)
-                    mbar_wait(&full[i % S], (i / S) & 1, abort_addr, I8_WAIT_CYCLES);
+                for (; loads > 0; loads--) {
+                    r.prev();
+                    i8_wait(smem_u32(&full[r.s]), r.phase, abort_addr);
+                }
             if (!ok || ld_volatile_shared(abort_addr)) {
                 const long long t0 = clock64();
                 while (clock64() - t0 < 1000000) {
@@ -839,78 +902,89 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         __syncwarp();
     } else if (rank == 0) {
         // ============ MMA issuer of the pair ======================================
-        if (lane == 0) {
-            int g = 0, sc = 0;
+        {
+            // first: the stages that the first part is issued on, waited for
+            // there; last: those whose last MMAs are issued, given back there
+            I8Ring<S> first, last;
+            int sc = 0;
             bool ok = true;
-            auto wait_stage = [&](int i) {
-                if (mbar_wait(&full[i % S], (i / S) & 1, abort_addr, I8_WAIT_CYCLES)) {
-                    tc_fence_after();
-                    return true;
-                }
-                return false;
-            };
+            const uint32_t base0 = smem_u32(base), full0 = smem_u32(full);
+            const uint64_t da = desc_k_sw128(base0);
+            const uint64_t db0 = desc_k_sw128(base0 + Cfg::A_BYTES);
+            const uint64_t db1 = desc_k_sw128(base0 + Cfg::A_BYTES + I8P_HALF_BYTES);
             auto wait_acc = [&](int i) {
-                if (mbar_wait(&accEmpty[i & 1], ((i >> 1) & 1) ^ 1, abort_addr, I8_WAIT_CYCLES)) {
-                    tc_fence_after();
-                    return true;
-                }
-                return false;
+                const bool got =
+                    i8_wait(smem_u32(&accEmpty[i & 1]), ((i >> 1) & 1) ^ 1, abort_addr);
+                tc_fence_after();
+                return got;
             };
             for (int i = 0; i < units.count && ok; i++) {
-                const I8Unit w = units[i];
-                const int n0 = i8p_first(w.n), n1 = w.n - n0;
+                const int n = units[i].n, n0 = i8p_first(n), n1 = n - n0;
                 const uint32_t id0 = idesc_i8(2 * I8_M, (n0 + 31) & ~31);
                 const uint32_t id1 = idesc_i8(2 * I8_M, (n1 + 31) & ~31);
-                auto part = [&](int p, int kb) {
-                    const uint32_t st = smem_u32(base + ((g + kb) % S) * Cfg::STAGE_BYTES);
-                    umma2_i8_k128(tmem + ((sc + p) & 1) * I8P_PART, desc_k_sw128(st),
-                                  desc_k_sw128(st + Cfg::A_BYTES + p * I8P_HALF_BYTES),
-                                  p ? id1 : id0, kb != 0);
+                const uint32_t acc0 = tmem + (sc & 1) * I8P_PART;
+                const uint32_t acc1 = tmem + ((sc + 1) & 1) * I8P_PART;
+                auto part0 = [&](int kb) {
+                    if (!i8_wait(full0 + 8 * first.s, first.phase, abort_addr)) return false;
+                    tc_fence_after();
+                    const uint32_t at = first.s * (Cfg::STAGE_BYTES >> 4);
+                    if (elect_one()) umma2_i8_k128(acc0, da + at, db0 + at, id0, kb != 0);
+                    __syncwarp();
+                    first.next();
+                    return true;
                 };
-                ok = wait_acc(sc);
+                auto part1 = [&](int kb) {
+                    const uint32_t at = last.s * (Cfg::STAGE_BYTES >> 4);
+                    if (elect_one()) umma2_i8_k128(acc1, da + at, db1 + at, id1, kb != 0);
+                    __syncwarp();
+                };
+                auto commit = [&](uint64_t *bar) {
+                    if (elect_one()) umma2_commit(bar);
+                    __syncwarp();
+                };
+                auto give_back = [&] {
+                    commit(&empty[last.s]);
+                    last.next();
+                };
+                if (!(ok = wait_acc(sc))) break;
                 if (n1 == 0) {
-                    for (int kb = 0; kb < a.KB && ok; kb++) {
-                        if (!(ok = wait_stage(g + kb))) break;
-                        part(0, kb);
-                        umma2_commit(&empty[(g + kb) % S]);
+                    for (int kb = 0; kb < a.KB; kb++) {
+                        if (!(ok = part0(kb))) break;
+                        give_back();
                     }
-                    if (ok) umma2_commit(&accFull[sc & 1]);
+                    if (ok) commit(&accFull[sc & 1]);
                     sc++;
                 } else {
                     // blocks [0, head): the first part alone, then the second;
                     // the middle ones together; [tail, KB) as the first ones
                     const int head = min(I8P_STAGGER, a.KB);
                     const int tail = max(head, a.KB - I8P_STAGGER);
-                    for (int kb = 0; kb < head && ok; kb++)
-                        if ((ok = wait_stage(g + kb))) part(0, kb);
-                    if (ok && head == a.KB) umma2_commit(&accFull[sc & 1]);
+                    for (int kb = 0; kb < head && ok; kb++) ok = part0(kb);
+                    if (ok && head == a.KB) commit(&accFull[sc & 1]);
                     ok = ok && wait_acc(sc + 1);
                     for (int kb = 0; kb < head && ok; kb++) {
-                        part(1, kb);
-                        umma2_commit(&empty[(g + kb) % S]);
+                        part1(kb);
+                        give_back();
                     }
                     for (int kb = head; kb < tail && ok; kb++) {
-                        if (!(ok = wait_stage(g + kb))) break;
-                        part(0, kb);
-                        part(1, kb);
-                        umma2_commit(&empty[(g + kb) % S]);
+                        if (!(ok = part0(kb))) break;
+                        part1(kb);
+                        give_back();
                     }
-                    for (int kb = tail; kb < a.KB && ok; kb++)
-                        if ((ok = wait_stage(g + kb))) part(0, kb);
-                    if (ok && tail < a.KB) umma2_commit(&accFull[sc & 1]);
+                    for (int kb = tail; kb < a.KB && ok; kb++) ok = part0(kb);
+                    if (ok && tail < a.KB) commit(&accFull[sc & 1]);
                     for (int kb = tail; kb < a.KB && ok; kb++) {
-                        part(1, kb);
-                        umma2_commit(&empty[(g + kb) % S]);
+                        part1(kb);
+                        give_back();
                     }
-                    if (ok) umma2_commit(&accFull[(sc + 1) & 1]);
+                    if (ok) commit(&accFull[(sc + 1) & 1]);
                     sc += 2;
                 }
-                g += a.KB;
             }
             if (!ok) {
                 fail();
-                umma2_commit(drain);
-                mbar_wait(drain, 0, 0, I8_WAIT_CYCLES);
+                if (elect_one()) umma2_commit(drain);
+                i8_wait(smem_u32(drain), 0, 0);
             }
         }
         __syncwarp();
