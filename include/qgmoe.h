@@ -475,10 +475,14 @@ int qgq8_destroy(qgq8_t *h);
 int qgq8_matmul_device(qgq8_t *h, const int8_t *codes, int64_t ld, const float *scale, int32_t R,
                        const int32_t *offsets, void *y, int32_t y_dtype, void *stream);
 /* qgq8_quantize_rows into the caller's codes / scale (R = T * k rows), then
- * qgq8_matmul_device on them, in one call. */
+ * qgq8_matmul_device on them, in one call.  codes and scale are scratch: what
+ * they hold afterwards is not defined.  Up to qgq8_direct_rows(h) rows of a
+ * dense product (neither pair_row nor offsets) run as one kernel that needs
+ * none; codes and scale may then be NULL.  Results are the same either way. */
 int qgq8_forward_device(qgq8_t *h, const void *x, int32_t x_dtype, int32_t T, int32_t k,
                         const int32_t *pair_row, const int32_t *offsets, int8_t *codes, int64_t ld,
                         float *scale, void *y, int32_t y_dtype, void *stream);
+int qgq8_direct_rows(const qgq8_t *h);
 /* One group, HOST pointers, blocking: x [T, in] f32 -> y f32. */
 int qgq8_forward(qgq8_t *h, const float *x, int32_t T, float *y);
 /* Waits for `stream` (NULL = the handle's stream) and reports any device

@@ -13,7 +13,11 @@
 // so that a batch of few rows costs a narrow N instead of an empty M.  Both
 // operands are tiled TMA loads of 128-byte rows (128B swizzle), accumulators
 // are int32 in TMEM, drained by eight epilogue warps while the next tile
-// accumulates.  Two kernels:
+// accumulates.  Three kernels:
+//   k_i8_few   up to 16 rows of a dense product, straight from x: every CTA
+//              quantises the rows for its own blocks while its weights load,
+//              and a cluster splits the sum, so that one launch has a single
+//              token's product spread over the whole device;
 //   k_i8       one CTA per tile of 128 channels x up to 16 or 64 rows, for few
 //              rows per group: a stream of weights;
 //   k_i8_pair  a CTA pair (cta_group::2) per tile of 256 channels x up to 512
@@ -27,13 +31,12 @@
 // following units, the group's weights in L2.  Every wait is bounded; a wait
 // that runs out raises QG_FLAG_TIMEOUT, the CTA lets its own loads and MMAs
 // finish, frees its TMEM and leaves.
-#include <cuda_bf16.h>
 #include <cudaTypedefs.h>
+#include <math_constants.h>
 
 #include <new>
 
-#include "qg_common.cuh"
-#include "qg_sm100.cuh"
+#include "qg_rows.cuh"
 
 namespace qg {
 using namespace sm100;
@@ -434,6 +437,11 @@ struct I8Epilogue {
             for (int i = 0; i < 4; i++) next_sw[i] = ws[(lane >> 2) + 8 * i];
         }
     }
+    // The channel scales alone, at once.
+    __device__ __forceinline__ void channels(const float *ws) {
+#pragma unroll
+        for (int i = 0; i < (LANES ? 1 : 4); i++) sw[i] = ws[LANES ? lane : (lane >> 2) + 8 * i];
+    }
     __device__ __forceinline__ void begin() {
 #pragma unroll
         for (int i = 0; i < (LANES ? 1 : 4); i++) sw[i] = next_sw[i];
@@ -597,7 +605,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         tmem_alloc(tmem_slot, Cfg::TMEM_COLS);
         tmem_relinquish();
     }
-    pdl_wait();
+    if (a.offsets) pdl_wait();  // else what comes before the rows needs no wait
     if (warp == 0) i8_prefix(a, prefix, lane);
     tc_fence_before();
     __syncthreads();
@@ -616,6 +624,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
 
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue: TMEM -> scaled rows ===============================
+        if (!a.offsets) pdl_wait();
         I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane,
                                                        scales + warp * I8_SCALE_BYTES);
         auto request = [&](int i) {
@@ -652,12 +661,27 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
             for (int i = 0; i < units.count && ok; i++) {
                 const I8Unit w = units[i];
                 const int wrow = (w.g * a.RT + w.ct) * a.KB * I8_M;
+                // the weights of the first stages do not wait for the kernel
+                // that makes the row codes
+                const int early = i == 0 && !a.offsets ? min(S, a.KB) : 0;
+                if (early) {
+                    if (elect_one())
+                        for (int kb = 0; kb < early; kb++) {
+                            mbar_arrive_expect_tx(&full[kb], Cfg::STAGE_BYTES);
+                            tma_load_2d(base + kb * Cfg::STAGE_BYTES, &tmap_w, 0,
+                                        wrow + kb * I8_M, &full[kb]);
+                        }
+                    __syncwarp();
+                    pdl_wait();
+                }
                 for (int kb = 0; kb < a.KB; kb++) {
                     if (!(ok = i8_wait(empty0 + 8 * r.s, r.phase ^ 1, abort_addr))) break;
                     if (elect_one()) {
                         uint8_t *dst = base + r.s * Cfg::STAGE_BYTES;
-                        mbar_arrive_expect_tx(&full[r.s], Cfg::STAGE_BYTES);
-                        tma_load_2d(dst, &tmap_w, 0, wrow + kb * I8_M, &full[r.s]);
+                        if (kb >= early) {
+                            mbar_arrive_expect_tx(&full[r.s], Cfg::STAGE_BYTES);
+                            tma_load_2d(dst, &tmap_w, 0, wrow + kb * I8_M, &full[r.s]);
+                        }
                         tma_load_2d(dst + Cfg::A_BYTES, &tmap_x, kb * I8_BK, w.row0, &full[r.s]);
                     }
                     __syncwarp();
@@ -676,6 +700,7 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         __syncwarp();
     } else {
         // ============ MMA issuer ===================================================
+        if (!a.offsets) pdl_wait();  // the limit of a wait is for this kernel's own work
         {
             I8Ring<S> r;
             bool ok = true;
@@ -773,7 +798,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         prefetch_tmap(&tmap_x);
     }
     if (warp == Cfg::MMA_WARP) tmem_alloc2(tmem_slot, 512);
-    pdl_wait();
+    if (a.offsets) pdl_wait();  // else what comes before the rows needs no wait
     if (warp == 0) i8_prefix(a, prefix, lane);
     tc_fence_before();
     __syncthreads();
@@ -793,6 +818,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 
     if (warp < Cfg::EPI_WARPS) {
         // ============ epilogue of this CTA's 128 channels =========================
+        if (!a.offsets) pdl_wait();
         I8Epilogue<TO, SWIGLU, Cfg::EPI_WARPS / 4> epi(a, warp, lane,
                                                        scales + warp * I8_SCALE_BYTES);
         // parts of units in order; sc: accumulators used so far
@@ -863,14 +889,29 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                 const int b0 = (h0 + I8P_BOX - 1) / I8P_BOX, b1 = (h1 + I8P_BOX - 1) / I8P_BOX;
                 const int r0 = w.row0 + rank * h0, r1 = w.row0 + n0 + rank * h1;
                 const uint32_t bytes = 2 * (Cfg::A_BYTES + (b0 + b1) * I8P_BOX * I8_BK);
+                // the weights of the first stages do not wait for the kernel
+                // that makes the row codes
+                const int early = i == 0 && !a.offsets ? min(S, a.KB) : 0;
+                if (early) {
+                    if (elect_one())
+                        for (int kb = 0; kb < early; kb++) {
+                            if (rank == 0) mbar_arrive_expect_tx(&full[kb], bytes);
+                            tma_load_2d_pair(base + kb * Cfg::STAGE_BYTES, &tmap_w, 0,
+                                             wrow + kb * I8_M, full0 + 8 * kb);
+                        }
+                    __syncwarp();
+                    pdl_wait();
+                }
                 for (int kb = 0; kb < a.KB; kb++) {
                     if (!(ok = i8_wait(empty0 + 8 * r.s, r.phase ^ 1, abort_addr))) break;
                     if (elect_one()) {
                         uint8_t *dst = base + r.s * Cfg::STAGE_BYTES, *dx = dst + Cfg::A_BYTES;
-                        if (rank == 0) mbar_arrive_expect_tx(&full[r.s], bytes);
                         const uint32_t bar = full0 + 8 * r.s;
                         const int x = kb * I8_BK;
-                        tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
+                        if (kb >= early) {
+                            if (rank == 0) mbar_arrive_expect_tx(&full[r.s], bytes);
+                            tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
+                        }
                         for (int b = 0; b < b0; b++)
                             tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x,
                                              r0 + b * I8P_BOX, bar);
@@ -902,6 +943,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
         __syncwarp();
     } else if (rank == 0) {
         // ============ MMA issuer of the pair ======================================
+        if (!a.offsets) pdl_wait();  // the limit of a wait is for this kernel's own work
         {
             // first: the stages that the first part is issued on, waited for
             // there; last: those whose last MMAs are issued, given back there
@@ -997,6 +1039,297 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     tc_fence_after();
     if (warp == Cfg::MMA_WARP) tmem_dealloc2(tmem, 512);
     cluster_sync();
+}
+
+// ---- few rows, straight from x -------------------------------------------------------------
+// y of up to 16 rows.  A cluster of `split` CTAs shares a tile of 128 channels,
+// each the blocks of its share of the sum.  Warps 0-7 quantise the rows (whole
+// rows for the maximum, this CTA's blocks of them into swizzled shared memory)
+// while the weights are on their way; warps 0-3 are the epilogue after that:
+// the partial sums of lane quarter q go to the CTA q * split / 4 of the
+// cluster, which adds them (exactly, as integers) and writes y.
+// One token, 2048 -> 4096: 5.6 us, where the quantiser and k_i8 took 8.3 in two
+// launches (5 us of that the product of one CTA per tile, 32 of 148 SMs).
+constexpr int I8F_ROWS = 16;
+constexpr int I8F_WARPS = 8;
+constexpr int I8F_LOAD_WARP = 8, I8F_MMA_WARP = 9;
+constexpr int I8F_THREADS = 10 * 32;
+constexpr int I8F_SPLIT = 4;   // most CTAs of a cluster
+constexpr int I8F_STAGES = 8;  // weight tiles in flight
+constexpr int I8F_BLOCKS = 32; // most blocks of a CTA: 2 KB of row codes each
+constexpr int I8F_CODE_BYTES = I8F_ROWS * I8_BK;
+constexpr int I8F_PART_BYTES = 16 * 128;  // a warp's partial sums
+struct I8FewArgs {
+    I8Args a;
+    const void *x;  // [R, K]
+    int x_dtype, x_vec, K;
+    int blocks, split;  // blocks of a CTA (the last one's may be fewer)
+};
+static int i8f_smem(int blocks) {
+    return I8F_STAGES * I8_M * I8_BK + blocks * I8F_CODE_BYTES +
+           4 * (I8F_SPLIT - 1) * I8F_PART_BYTES + 2048;
+}
+
+// Eight values of row r from column c on, zeros past the row's end.
+template <typename TI>
+__device__ __forceinline__ void i8f_load8(const void *x, int64_t at, int left, bool vec,
+                                          float (&v)[8]) {
+    const TI *p = static_cast<const TI *>(x) + at;
+    if (vec) {
+        Vec8<TI> in;
+        in.load(p);
+        in.get(v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = i < left ? Elem<TI>::load(p + i) : 0.f;
+    }
+}
+__device__ __forceinline__ void i8f_load8(const I8FewArgs &f, int r, int c, float (&v)[8]) {
+    const int64_t at = (int64_t)r * f.K + c;
+    const int left = f.K - c;
+    if (f.x_dtype == QGMOE_DT_F32)
+        i8f_load8<float>(f.x, at, left, f.x_vec, v);
+    else if (f.x_dtype == QGMOE_DT_F16)
+        i8f_load8<__half>(f.x, at, left, f.x_vec, v);
+    else
+        i8f_load8<__nv_bfloat16>(f.x, at, left, f.x_vec, v);
+}
+
+__device__ __forceinline__ bool i8_try_wait_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+template <typename TO, bool SWIGLU>
+__global__ void __launch_bounds__(I8F_THREADS, 1)
+k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
+    pdl_launch_dependents();
+    const I8Args &a = f.a;
+    constexpr int S = I8F_STAGES, STAGE = I8_M * I8_BK;
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(16) float s_scale[32];  // of the rows
+    __shared__ uint32_t s_max[I8F_ROWS][I8F_WARPS];
+    __shared__ uint64_t full[S], empty[S], codesFull, accFull, drain, partFull[4];
+    __shared__ uint32_t tmem_slot, s_abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = f.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
+    const int ct = blockIdx.x / split;  // channel tile
+    const int kb0 = rank * f.blocks, nb = max(0, min(f.blocks, a.KB - kb0));
+
+    uint8_t *base = reinterpret_cast<uint8_t *>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    const uint32_t codes = smem_u32(base + S * STAGE);
+    const uint32_t parts = codes + f.blocks * I8F_CODE_BYTES;
+    const uint32_t abort_addr = smem_u32(&s_abort);
+
+    if (tid == 0) {
+        for (int s = 0; s < S; s++) {
+            mbar_init(&full[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        mbar_init(&codesFull, I8F_WARPS);
+        mbar_init(&accFull, 1);
+        mbar_init(&drain, 1);
+        for (int q = 0; q < 4; q++) mbar_init(&partFull[q], split > 1 ? split - 1 : 1);
+        s_abort = 0;
+        fence_mbar_init();
+        prefetch_tmap(&tmap_w);
+    }
+    if (warp == I8F_MMA_WARP) {
+        tmem_alloc(&tmem_slot, 32);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();  // the others' barriers are initialised
+    tc_fence_after();
+    const uint32_t tmem = tmem_slot;
+
+    auto fail = [&]() {
+        if (!ld_volatile_shared(abort_addr)) {
+            st_volatile_shared(abort_addr, 1);
+            atomicOr(a.err, QG_FLAG_TIMEOUT);
+        }
+    };
+
+    if (warp < I8F_WARPS) {
+        pdl_wait();  // x
+        // ============ rows -> codes ===============================================
+        for (int r = 0; r < a.R; r++) {
+            float m = 0.f;  // a maximum that keeps NaN
+#pragma unroll 4
+            for (int c = tid * 8; c < f.K; c += I8F_WARPS * 256) {
+                float v[8];
+                i8f_load8(f, r, c, v);
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[i])));
+            }
+            const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(m));
+            if (lane == 0) s_max[r][warp] = top;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (tid < I8F_ROWS) {
+            uint32_t m = 0;
+            if (tid < a.R)
+                for (int w = 0; w < I8F_WARPS; w++) m = max(m, s_max[tid][w]);
+            // what was not finite makes the row's products NaN
+            s_scale[tid] = m >= 0x7F800000u ? CUDART_NAN_F : scale_of(m);
+            s_scale[16 + tid] = 0.f;
+        }
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const int lo = kb0 * I8_BK, cols = min(f.K, lo + nb * I8_BK) - lo;
+        for (int i = tid; i < a.R * (nb * I8_BK / 8); i += I8F_WARPS * 32) {
+            const int r = i / (nb * I8_BK / 8), c = (i - r * (nb * I8_BK / 8)) * 8;
+            uint2 u = make_uint2(0, 0);
+            const float s = s_scale[r];
+            if (c < cols && s == s) {
+                float v[8];
+                i8f_load8(f, r, lo + c, v);
+                u = codes_of(v, s, __frcp_rn(s));
+            }
+            const int j = c % I8_BK;
+            const uint32_t at = codes + c / I8_BK * I8F_CODE_BYTES + r * I8_BK +
+                                (((j >> 4) ^ (r & 7)) << 4) + (j & 8);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(u.x), "r"(u.y)
+                         : "memory");
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&codesFull);
+        // ============ epilogue =====================================================
+        if (warp < 4) {
+            const int q = warp, owner = q * split / 4;
+            const int rblocks = (a.R + 7) / 8;
+            I8Epilogue<TO, SWIGLU, 1> epi(a, q, lane, smem_u32(s_scale));
+            epi.channels(a.ws + ((size_t)ct * I8_M) + q * 32);
+            int v[2][16];
+            bool ok = i8_wait(smem_u32(&accFull), 0, abort_addr);
+            if (!ok) fail();
+            tc_fence_after();
+            // a CTA without blocks adds nothing (nor has it a sum)
+            if (ok && nb > 0) {
+                epi.fetch(tmem + ((uint32_t)(q * 32) << 16), v);
+                tmem_wait_ld();
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; i++) v[0][i] = v[1][i] = 0;
+            }
+            tc_fence_before();
+            // the values of the first 8 (16) rows, wherever this layout has them
+            auto value = [&](int b, int i) -> int & {
+                if constexpr (I8Epilogue<TO, SWIGLU, 1>::LANES)
+                    return v[0][b * 8 + i];
+                else
+                    return v[i >> 2][b * 4 + (i & 3)];
+            };
+            if (owner != rank) {
+                const int slot = rank < owner ? rank : rank - 1;
+                const uint32_t to = mapa_shared(
+                    parts + ((q * (I8F_SPLIT - 1) + slot) * I8F_PART_BYTES) + lane * 4, owner);
+#pragma unroll
+                for (int b = 0; b < 2; b++)
+                    if (b < rblocks)
+#pragma unroll
+                        for (int i = 0; i < 8; i++)
+                            asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(
+                                             to + (b * 8 + i) * 128),
+                                         "r"(value(b, i))
+                                         : "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    const uint32_t bar = mapa_shared(smem_u32(&partFull[q]), owner);
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                     bar)
+                                 : "memory");
+                }
+            } else {
+                if (split > 1) {
+                    bool got = __all_sync(~0u, i8_try_wait_cluster(smem_u32(&partFull[q]), 0));
+                    const long long t0 = clock64();
+                    while (!got && clock64() - t0 < I8_WAIT_CYCLES)
+                        got = i8_try_wait_cluster(smem_u32(&partFull[q]), 0);
+                    if (!__all_sync(~0u, got)) {
+                        fail();
+                        ok = false;
+                    }
+                    for (int p = 0; p < split - 1 && ok; p++) {
+                        const uint32_t from =
+                            parts + ((q * (I8F_SPLIT - 1) + p) * I8F_PART_BYTES) + lane * 4;
+#pragma unroll
+                        for (int b = 0; b < 2; b++)
+                            if (b < rblocks)
+#pragma unroll
+                                for (int i = 0; i < 8; i++)
+                                    value(b, i) += (int)ld_shared_u32(from + (b * 8 + i) * 128);
+                    }
+                }
+                if (ok)
+                    epi.template run<false>(v, smem_u32(s_scale), 0, a.R,
+                                            (ct * 4 + q) * I8Epilogue<TO, SWIGLU, 1>::CH);
+            }
+        }
+    } else if (warp == I8F_LOAD_WARP) {
+        // ============ weights ======================================================
+        I8Ring<S> r;
+        int loads = 0;
+        bool ok = true;
+        const int wrow = (ct * a.KB + kb0) * I8_M;
+        for (int kb = 0; kb < nb; kb++) {
+            if (kb == S) pdl_wait();  // stages come back once there are codes
+            if (!(ok = i8_wait(smem_u32(&empty[r.s]), r.phase ^ 1, abort_addr))) break;
+            if (elect_one()) {
+                mbar_arrive_expect_tx(&full[r.s], STAGE);
+                tma_load_2d(base + r.s * STAGE, &tmap_w, 0, wrow + kb * I8_M, &full[r.s]);
+            }
+            __syncwarp();
+            loads = min(loads + 1, S);
+            r.next();
+        }
+        if (!ok) fail();
+        for (; loads > 0; loads--) {  // the copies land before the shared memory goes
+            r.prev();
+            i8_wait(smem_u32(&full[r.s]), r.phase, 0);
+        }
+    } else {
+        // ============ MMAs =========================================================
+        I8Ring<S> r;
+        const uint64_t da = desc_k_sw128(smem_u32(base)), db = desc_k_sw128(codes);
+        const uint32_t idesc = idesc_i8(I8_M, I8F_ROWS);
+        pdl_wait();  // the limit of a wait is for this kernel's own work
+        bool ok = i8_wait(smem_u32(&codesFull), 0, abort_addr);
+        tc_fence_after();
+        for (int kb = 0; kb < nb && ok; kb++) {
+            if (!(ok = i8_wait(smem_u32(&full[r.s]), r.phase, abort_addr))) break;
+            tc_fence_after();
+            if (elect_one()) {
+                umma_i8_k128(tmem, da + r.s * (STAGE >> 4), db + kb * (I8F_CODE_BYTES >> 4), idesc,
+                             kb != 0);
+                umma_commit(&empty[r.s]);
+            }
+            __syncwarp();
+            r.next();
+        }
+        if (!ok) fail();
+        if (elect_one()) umma_commit(ok ? &accFull : &drain);
+        __syncwarp();
+        if (!ok) i8_wait(smem_u32(&drain), 0, 0);
+    }
+
+    tc_fence_before();
+    __syncthreads();
+    if (split > 1) cluster_sync();  // the partial sums have been taken
+    if (warp == I8F_MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 32);
+    }
 }
 
 // ---- weight layout -------------------------------------------------------------
@@ -1239,6 +1572,72 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
                       : launch_i8<I8P_NT>(h, tx, a, ydt, units, s);
 }
 
+// Rows up to which a dense product runs on k_i8_few: 16, if a CTA's share of
+// the row codes fits next to its weights.
+static int i8_few_split(const qgq8 *h) {
+    int split = 1;
+    while (split < I8F_SPLIT && h->live * split * 2 <= num_sms(h->device) && h->KB >= split * 4)
+        split *= 2;
+    return split;
+}
+static int i8_few_rows(const qgq8 *h) {
+    if (h->G != 1) return 0;
+    const int split = i8_few_split(h);
+    return (h->KB + split - 1) / split <= I8F_BLOCKS ? I8F_ROWS : 0;
+}
+
+template <typename TO, bool SWIGLU>
+static int launch_i8_few_t(const qgq8 *h, const I8FewArgs &f, cudaStream_t s) {
+    auto kern = k_i8_few<TO, SWIGLU>;
+    static bool done[64] = {false};
+    if (h->device >= 64 || !done[h->device]) {
+        QG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     i8f_smem(I8F_BLOCKS)));
+        if (h->device < 64) done[h->device] = true;
+    }
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see launch_pdl
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = f.split;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.gridDim = dim3((unsigned)(h->live * f.split));
+    cfg.blockDim = dim3(I8F_THREADS);
+    cfg.dynamicSmemBytes = i8f_smem(f.blocks);
+    cfg.stream = s;
+    cfg.attrs = at;
+    cfg.numAttrs = f.split > 1 ? 2 : 1;
+    QG_CUDA(cudaLaunchKernelEx(&cfg, kern, h->tmap_w, f));
+    return QGMOE_OK;
+}
+
+static int i8_few(const qgq8 *h, const void *x, int xdt, int R, void *y, int ydt, cudaStream_t s) {
+    I8FewArgs f{};
+    f.a.ws = h->ws;
+    f.a.G = 1;
+    f.a.R = R;
+    f.a.RT = h->RT;
+    f.a.KB = h->KB;
+    f.a.cols = h->cols;
+    f.a.y = y;
+    f.a.vec = h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
+    f.a.err = h->err_dev;
+    f.x = x;
+    f.x_dtype = xdt;
+    f.x_vec = h->I % 8 == 0 && !(reinterpret_cast<uintptr_t>(x) & 15);
+    f.K = h->I;
+    f.split = i8_few_split(h);
+    f.blocks = (h->KB + f.split - 1) / f.split;
+    if (h->swiglu)
+        return ydt == QGMOE_DT_F32   ? launch_i8_few_t<float, true>(h, f, s)
+               : ydt == QGMOE_DT_F16 ? launch_i8_few_t<__half, true>(h, f, s)
+                                     : launch_i8_few_t<__nv_bfloat16, true>(h, f, s);
+    return ydt == QGMOE_DT_F32   ? launch_i8_few_t<float, false>(h, f, s)
+           : ydt == QGMOE_DT_F16 ? launch_i8_few_t<__half, false>(h, f, s)
+                                 : launch_i8_few_t<__nv_bfloat16, false>(h, f, s);
+}
+
 static void i8_free_work(qgq8 *h) {
     cudaFree(h->x_dev);
     cudaFree(h->y_dev);
@@ -1377,13 +1776,19 @@ int qgq8_forward_device(qgq8_t *h, const void *x, int32_t x_dtype, int32_t T, in
                         const int32_t *pair_row, const int32_t *offsets, int8_t *codes, int64_t ld,
                         float *scale, void *y, int32_t y_dtype, void *stream) {
     if (!h) return set_error(QGMOE_ERR_INVALID_ARG, "null handle");
-    int rc = check_quantize_rows(x, x_dtype, T, k, h->I, pair_row, codes, ld, scale);
+    const bool direct = !pair_row && !offsets && k == 1 && T <= i8_few_rows(h);
+    // the direct kernel needs no codes: stand-ins that pass the checks
+    const int64_t ld_ = direct ? i8_pitch(h->I) : ld;
+    int8_t *c_ = direct ? reinterpret_cast<int8_t *>(h->w) : codes;
+    float *s_ = direct ? h->ws : scale;
+    int rc = check_quantize_rows(x, x_dtype, T, k, h->I, pair_row, c_, ld_, s_);
     if (rc) return rc;
     const int R = T * k;
-    rc = i8_check_product(h, codes, ld, scale, R, offsets, y, y_dtype);
+    rc = i8_check_product(h, c_, ld_, s_, R, offsets, y, y_dtype);
     if (rc || R == 0) return rc;
     QG_ON_DEVICE(h->device);
     cudaStream_t s = stream ? static_cast<cudaStream_t>(stream) : h->stream;
+    if (direct) return i8_few(h, x, x_dtype, R, y, y_dtype, s);
     rc = launch_quantize_rows(x, x_dtype, T, k, h->I, pair_row, codes, ld, scale, s);
     if (rc) return rc;
     return i8_product(h, codes, ld, scale, R, offsets, y, y_dtype, s);
@@ -1418,6 +1823,8 @@ int qgq8_forward(qgq8_t *h, const float *x, int32_t T, float *y) {
     QG_CUDA(cudaMemcpyAsync(y, h->y_dev, sizeof(float) * (size_t)T * h->cols, cudaMemcpyDeviceToHost, s));
     return qgq8_sync(h, nullptr);
 }
+
+int qgq8_direct_rows(const qgq8_t *h) { return h ? i8_few_rows(h) : 0; }
 
 int qgq8_sync(qgq8_t *h, void *stream) {
     if (!h) return set_error(QGMOE_ERR_INVALID_ARG, "null handle");

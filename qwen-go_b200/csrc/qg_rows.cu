@@ -15,114 +15,11 @@
 // Every kernel is organised by token, so that a token's row is read once for
 // its k expert rows, and rows that no pair owns are never touched.  A
 // pair_row outside [0, T*k) counts as a pair without a row.
-#include <cuda_bf16.h>
-#include <float.h>
 #include <math_constants.h>
 
-#include "qg_common.cuh"
-#include "qg_sm100.cuh"
+#include "qg_rows.cuh"
 
 namespace qg {
-
-// ---- row elements ---------------------------------------------------------
-// Rows are read with plain (coherent) loads: with programmatic dependent
-// launch the previous kernel may still be writing them when this one starts,
-// which the read-only path does not allow.
-__device__ __forceinline__ uint4 ld16(const void *p) {
-    uint4 v;
-    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
-                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                 : "l"(p)
-                 : "memory");
-    return v;
-}
-__device__ __forceinline__ int ld_i32(const int32_t *p) {
-    int v;
-    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-    return v;
-}
-__device__ __forceinline__ float ld_f32(const float *p) {
-    float v;
-    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
-    return v;
-}
-
-template <typename T> struct Elem;
-template <> struct Elem<float> {
-    static __device__ __forceinline__ float load(const float *p) { return ld_f32(p); }
-    static __device__ __forceinline__ void store(float *p, float v) { *p = v; }
-};
-template <> struct Elem<__half> {
-    static __device__ __forceinline__ float load(const __half *p) {
-        unsigned short u;
-        asm volatile("ld.global.u16 %0, [%1];" : "=h"(u) : "l"(p) : "memory");
-        return __half2float(__ushort_as_half(u));
-    }
-    static __device__ __forceinline__ void store(__half *p, float v) { *p = __float2half_rn(v); }
-};
-template <> struct Elem<__nv_bfloat16> {
-    static __device__ __forceinline__ float load(const __nv_bfloat16 *p) {
-        unsigned short u;
-        asm volatile("ld.global.u16 %0, [%1];" : "=h"(u) : "l"(p) : "memory");
-        return __uint_as_float((uint32_t)u << 16);
-    }
-    static __device__ __forceinline__ void store(__nv_bfloat16 *p, float v) {
-        *p = __float2bfloat16_rn(v);
-    }
-};
-
-// Eight consecutive elements, 16-byte aligned; raw as loaded, so that several
-// can be in flight before the first is widened.
-template <typename T> struct Vec8 {  // 16-bit types: one 16-byte load
-    uint4 r;
-    __device__ __forceinline__ void load(const T *p) { r = ld16(p); }
-    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            float2 f;
-            if constexpr (sizeof(T) == 2 && __is_same(T, __half))
-                f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            else
-                f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
-            v[2 * i] = f.x;
-            v[2 * i + 1] = f.y;
-        }
-    }
-    static __device__ __forceinline__ void put(T *p, const float (&v)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            if constexpr (__is_same(T, __half)) {
-                __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
-                w[i] = *reinterpret_cast<uint32_t *>(&h);
-            } else {
-                __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
-                w[i] = *reinterpret_cast<uint32_t *>(&h);
-            }
-        }
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-};
-template <> struct Vec8<float> {  // two 16-byte loads
-    uint4 a, b;
-    __device__ __forceinline__ void load(const float *p) {
-        a = ld16(p);
-        b = ld16(p + 4);
-    }
-    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y);
-        v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-        v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
-        v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-    }
-    static __device__ __forceinline__ void put(float *p, const float (&v)[8]) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-};
 
 // ---- sort -------------------------------------------------------------------
 // One cluster of up to eight CTAs, no workspace, one launch.  Each warp owns a
@@ -451,13 +348,7 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
 // scale NaN and codes 0, so that what is computed from it is NaN.  With
 // pair_row, row t goes to the k rows of its pairs.
 //
-// The quotient is Markstein's: with y the rounded reciprocal of the scale and
-// t = x y, the remainder r = x - t s is exact in one fused operation and
-// t + r y is the correctly rounded x / s (Markstein 1990; a scale whose
-// mantissa is all ones is the theorem's exception and is divided by).  Adding
-// 1.5 * 2^23 rounds it, halves to even, and leaves the code in the low byte;
-// halves are then moved away from zero, which only vectors that hold one pay
-// for.  Seven operations a value instead of some twenty.
+// (How the codes are formed: qg_rows.cuh.)
 //
 // A row belongs to `wpr` warps of a CTA.  It is copied to shared memory
 // asynchronously and read there twice, each thread the vectors it copied
@@ -468,113 +359,6 @@ constexpr int QR_WARPS = 8;
 constexpr int QR_THREADS = QR_WARPS * 32;
 constexpr int QR_ROW_BYTES = 32 * 1024;
 
-__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
-}
-// Largest magnitude of a row.  float32: a maximum that keeps NaN; 16 bits: the
-// two halves of a word at once, as integers, which order magnitudes and put
-// infinity and NaN above every number.
-template <typename T> struct AbsMax {
-    uint32_t m = 0;
-    __device__ __forceinline__ void fold(const Vec8<T> &x) {
-        const uint32_t w[4] = {x.r.x, x.r.y, x.r.z, x.r.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
-    }
-    __device__ __forceinline__ void fold1(float v) {  // one widened value
-        if constexpr (__is_same(T, __half))
-            m = __vmaxu2(m, (uint32_t)__half_as_ushort(__float2half_rn(fabsf(v))));
-        else
-            m = __vmaxu2(m, __float_as_uint(fabsf(v)) >> 16);
-    }
-    // as float32 bits, exponent all ones for infinity or NaN
-    __device__ __forceinline__ uint32_t bits() const {
-        const uint32_t h = max(m & 0xFFFFu, m >> 16);
-        if constexpr (__is_same(T, __half)) {
-            if (h >= 0x7C00u) return 0x7F800000u;
-            return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
-        }
-        return h << 16;
-    }
-};
-template <> struct AbsMax<float> {
-    float m = 0.f;
-    __device__ __forceinline__ void fold1(float v) {
-        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
-    }
-    __device__ __forceinline__ void fold(const Vec8<float> &x) {
-        float v[8];
-        x.get(v);
-#pragma unroll
-        for (int q = 0; q < 8; q++) fold1(v[q]);
-    }
-    __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(m); }
-};
-__device__ __forceinline__ float scale_of(uint32_t m) {
-    return fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), 1e-8f);
-}
-// inv: __frcp_rn(s), or 0 where the quotient has to be divided.
-__device__ __forceinline__ float inverse_of(float s) {
-    return (__float_as_uint(s) & 0x7FFFFFu) == 0x7FFFFFu ? 0.f : __frcp_rn(s);
-}
-// Pairs of float32 in a register pair, two operations per instruction.
-__device__ __forceinline__ uint64_t f2(float a, float b) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 unf2(uint64_t v) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-    return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
-    constexpr float MAGIC = 12582912.f;
-    const uint64_t minus_s = f2(-s, -s), y = f2(inv, inv);
-    const uint64_t magic = f2(MAGIC, MAGIC), minus_magic = f2(-MAGIC, -MAGIC);
-    const uint64_t minus_one = f2(-1.f, -1.f);
-    float2 q[4], e[4];
-    uint32_t c[8];
-    float far = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint64_t x = f2(v[2 * i], v[2 * i + 1]);
-        const uint64_t t = mul2(x, y);
-        uint64_t z = fma2(fma2(t, minus_s, x), y, t);
-        if (inv == 0.f) z = f2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
-        const uint64_t r = add2(z, magic);
-        q[i] = unf2(z);
-        e[i] = unf2(fma2(add2(r, minus_magic), minus_one, z));  // z - round(z), exact
-        const float2 rf = unf2(r);
-        c[2 * i] = __float_as_uint(rf.x);
-        c[2 * i + 1] = __float_as_uint(rf.y);
-        far = fmaxf(far, fmaxf(fabsf(e[i].x), fabsf(e[i].y)));
-    }
-    if (far == 0.5f) {  // some q is a half: away from zero, not to the even side
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const float z = i & 1 ? q[i >> 1].y : q[i >> 1].x, d = i & 1 ? e[i >> 1].y : e[i >> 1].x;
-            if (fabsf(d) == 0.5f)
-                c[i] = __float_as_uint(__fadd_rn(__fadd_rn(z, copysignf(0.5f, z)), MAGIC));
-        }
-    }
-    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-}
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -626,7 +410,7 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t 
     }
     if (!on) return;
     const bool bad = m >= 0x7F800000u;
-    const float s = bad ? 1.f : scale_of(m), inv = inverse_of(s);
+    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
     if constexpr (!GATHER) {
         if (part == 0 && lane == 0) scale[t] = bad ? CUDART_NAN_F : s;
         int8_t *out = codes + t * ld;
@@ -694,7 +478,7 @@ k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_
     __syncthreads();
     for (int w = 0; w < nt >> 5; w++) m = max(m, s_max[w]);
     const bool bad = m >= 0x7F800000u;
-    const float s = bad ? 1.f : scale_of(m), inv = inverse_of(s);
+    const float s = bad ? 1.f : scale_of(m), inv = __frcp_rn(s);
     const int n_dst = pair_row ? k : 1;
     auto dst_row = [&](int j) { return pair_row ? ld_i32(pair_row + t * k + j) : (int)t; };
     for (int j = tid; j < n_dst; j += nt) {

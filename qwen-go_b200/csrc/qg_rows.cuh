@@ -1,0 +1,238 @@
+// Rows of float32, float16 or bfloat16 elements, and their int8 codes: what
+// the row kernels (qg_rows.cu) and the 8-bit products that take rows directly
+// (qg_int8.cu) share.
+#pragma once
+#include <cuda_bf16.h>
+
+#include "qg_common.cuh"
+#include "qg_sm100.cuh"
+
+namespace qg {
+
+// ---- row elements ---------------------------------------------------------
+// Rows are read with plain (coherent) loads: with programmatic dependent
+// launch the previous kernel may still be writing them when this one starts,
+// which the read-only path does not allow.
+__device__ __forceinline__ uint4 ld16(const void *p) {
+    uint4 v;
+    asm volatile("ld.global.L1::no_allocate.v4.b32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p)
+                 : "memory");
+    return v;
+}
+__device__ __forceinline__ int ld_i32(const int32_t *p) {
+    int v;
+    asm volatile("ld.global.b32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float ld_f32(const float *p) {
+    float v;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(v) : "l"(p) : "memory");
+    return v;
+}
+
+template <typename T> struct Elem;
+template <> struct Elem<float> {
+    static __device__ __forceinline__ float load(const float *p) { return ld_f32(p); }
+    static __device__ __forceinline__ void store(float *p, float v) { *p = v; }
+};
+template <> struct Elem<__half> {
+    static __device__ __forceinline__ float load(const __half *p) {
+        unsigned short u;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(u) : "l"(p) : "memory");
+        return __half2float(__ushort_as_half(u));
+    }
+    static __device__ __forceinline__ void store(__half *p, float v) { *p = __float2half_rn(v); }
+};
+template <> struct Elem<__nv_bfloat16> {
+    static __device__ __forceinline__ float load(const __nv_bfloat16 *p) {
+        unsigned short u;
+        asm volatile("ld.global.u16 %0, [%1];" : "=h"(u) : "l"(p) : "memory");
+        return __uint_as_float((uint32_t)u << 16);
+    }
+    static __device__ __forceinline__ void store(__nv_bfloat16 *p, float v) {
+        *p = __float2bfloat16_rn(v);
+    }
+};
+
+// Eight consecutive elements, 16-byte aligned; raw as loaded, so that several
+// can be in flight before the first is widened.
+template <typename T> struct Vec8 {  // 16-bit types: one 16-byte load
+    uint4 r;
+    __device__ __forceinline__ void load(const T *p) { r = ld16(p); }
+    __device__ __forceinline__ void zero() { r = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            float2 f;
+            if constexpr (sizeof(T) == 2 && __is_same(T, __half))
+                f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            else
+                f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ void put(T *p, const float (&v)[8]) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if constexpr (__is_same(T, __half)) {
+                __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<uint32_t *>(&h);
+            } else {
+                __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+                w[i] = *reinterpret_cast<uint32_t *>(&h);
+            }
+        }
+        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+template <> struct Vec8<float> {  // two 16-byte loads
+    uint4 a, b;
+    __device__ __forceinline__ void load(const float *p) {
+        a = ld16(p);
+        b = ld16(p + 4);
+    }
+    __device__ __forceinline__ void zero() { a = b = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y);
+        v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
+        v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
+        v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
+    }
+    static __device__ __forceinline__ void put(float *p, const float (&v)[8]) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+
+// ---- int8 codes -----------------------------------------------------------
+// scale = max(amax / 127, 1e-8), code = clamp(round_half_away(x / scale)) with
+// an IEEE float32 quotient (the rule of quantizeInt8, model/moe.go:165-188).
+// A quotient is first formed as t = x y with y the rounded reciprocal of the
+// scale, within 2.3e-5 of x / scale as |t| <= 127; adding 1.5 * 2^23 rounds it
+// and leaves the code in the low byte.  Only a t within 1e-4 of a half can
+// round otherwise than the quotient does.  Vectors with one (one in 600 of
+// float32 values, more of 16-bit ones, whose quotients often are halves) get
+// the correctly rounded quotient, by Markstein's iteration (1990): the
+// remainder r = x - t s is exact in one fused operation and t + r y is within
+// an ulp of x / s; the same step from there is the correctly rounded x / s (a
+// scale whose mantissa is all ones is the theorem's exception and is divided
+// by).  Halves, rounded to even by the addition, then go away from zero.
+__device__ __forceinline__ uint32_t pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// Largest magnitude of a row.  float32: a maximum that keeps NaN; 16 bits: the
+// two halves of a word at once, as integers, which order magnitudes and put
+// infinity and NaN above every number.
+template <typename T> struct AbsMax {
+    uint32_t m = 0;
+    __device__ __forceinline__ void fold(const Vec8<T> &x) {
+        const uint32_t w[4] = {x.r.x, x.r.y, x.r.z, x.r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+    }
+    __device__ __forceinline__ void fold1(float v) {  // one widened value
+        if constexpr (__is_same(T, __half))
+            m = __vmaxu2(m, (uint32_t)__half_as_ushort(__float2half_rn(fabsf(v))));
+        else
+            m = __vmaxu2(m, __float_as_uint(fabsf(v)) >> 16);
+    }
+    // as float32 bits, exponent all ones for infinity or NaN
+    __device__ __forceinline__ uint32_t bits() const {
+        const uint32_t h = max(m & 0xFFFFu, m >> 16);
+        if constexpr (__is_same(T, __half)) {
+            if (h >= 0x7C00u) return 0x7F800000u;
+            return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+        }
+        return h << 16;
+    }
+};
+template <> struct AbsMax<float> {
+    float m = 0.f;
+    __device__ __forceinline__ void fold1(float v) {
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v)));
+    }
+    __device__ __forceinline__ void fold(const Vec8<float> &x) {
+        float v[8];
+        x.get(v);
+#pragma unroll
+        for (int q = 0; q < 8; q++) fold1(v[q]);
+    }
+    __device__ __forceinline__ uint32_t bits() const { return __float_as_uint(m); }
+};
+__device__ __forceinline__ float scale_of(uint32_t m) {
+    return fmaxf(__fdiv_rn(__uint_as_float(m), 127.f), 1e-8f);
+}
+// Pairs of float32 in a register pair, two operations per instruction.
+__device__ __forceinline__ uint64_t f2(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unf2(uint64_t v) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+static __device__ __noinline__ uint2 codes_near_half(float v0, float v1, float v2, float v3, float v4,
+                                              float v5, float v6, float v7, float s, float inv) {
+    constexpr float MAGIC = 12582912.f;
+    const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
+    const bool divide = (__float_as_uint(s) & 0x7FFFFFu) == 0x7FFFFFu;
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        float q = __fmul_rn(v[i], inv);
+        q = __fmaf_rn(__fmaf_rn(-q, s, v[i]), inv, q);
+        q = __fmaf_rn(__fmaf_rn(-q, s, v[i]), inv, q);
+        if (divide) q = __fdiv_rn(v[i], s);
+        const float r = __fadd_rn(q, MAGIC);
+        const float e = __fsub_rn(q, __fsub_rn(r, MAGIC));  // exact
+        c[i] = __float_as_uint(fabsf(e) == 0.5f
+                                   ? __fadd_rn(__fadd_rn(q, copysignf(0.5f, q)), MAGIC)
+                                   : r);
+    }
+    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+}
+// inv: __frcp_rn(s)
+__device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
+    constexpr float MAGIC = 12582912.f;
+    const uint64_t y = f2(inv, inv), magic = f2(MAGIC, MAGIC), minus_magic = f2(-MAGIC, -MAGIC);
+    const uint64_t minus_one = f2(-1.f, -1.f);
+    uint32_t c[8];
+    float far = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint64_t t = mul2(f2(v[2 * i], v[2 * i + 1]), y);
+        const uint64_t r = add2(t, magic);
+        const float2 e = unf2(fma2(add2(r, minus_magic), minus_one, t));  // t - round(t), exact
+        const float2 rf = unf2(r);
+        c[2 * i] = __float_as_uint(rf.x);
+        c[2 * i + 1] = __float_as_uint(rf.y);
+        far = fmaxf(far, fmaxf(fabsf(e.x), fabsf(e.y)));
+    }
+    if (far > 0.4999f)
+        return codes_near_half(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], s, inv);
+    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
+}
+
+}  // namespace qg

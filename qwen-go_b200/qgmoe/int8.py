@@ -93,6 +93,7 @@ class Int8Linear:
         _call("qgq8_create", self.groups, shape[-2], shape[-1], _q._ptr(qweight), _q._ptr(scale),
               int(bool(swiglu)), int(on_dev), self.device, C.byref(h))
         self.h = h
+        self._direct_rows = _q.lib().qgq8_direct_rows(h)
 
     def close(self):
         if getattr(self, "h", None):
@@ -151,8 +152,12 @@ class Int8Linear:
                 order.offsets
         off = self._offsets(offsets, x.device)
         y = _result(y, "y", x, (R, self.out_features), dtype)
-        # codes [R, pitch], then their scales: one allocation
         ld = _pitch(K)
+        if off is None and pair_row is None and R <= self._direct_rows:
+            _call("qgq8_forward_device", self.h, x.data_ptr(), dt, T, 1, None, None, None, ld, None,
+                  y.data_ptr(), _row_dtype(y, "y"), s)
+            return y
+        # codes [R, pitch], then their scales: one allocation
         work = x.new_empty(R * (ld + 4), dtype=_rows._torch.int8)
         at = work.data_ptr()
         _call("qgq8_forward_device", self.h, x.data_ptr(), dt, T, k, pair_row, off, at, ld,

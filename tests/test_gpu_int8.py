@@ -133,6 +133,38 @@ def test_linear(T, K, N, xt, yt):
     lin.close()
 
 
+@pytest.mark.parametrize("K,N", [(1, 1), (100, 40), (257, 300), (1000, 129), (2048, 4096),
+                                 (4104, 260), (9000, 64), (16384, 512), (40000, 24)])
+@pytest.mark.parametrize("xt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_few_rows_directly(K, N, xt, swiglu):
+    """Up to 16 rows in one kernel: bit for bit what the quantiser and the
+    product give, rows that are not finite included; one row more than that
+    takes the two kernels."""
+    t = torch_()
+    q, ws = weights((2 * N if swiglu else N, K), N)
+    lin = qgmoe.Int8Linear(q, ws, swiglu=swiglu)
+    assert qgmoe.lib().qgq8_direct_rows(lin.h) in (0, 16)
+    for T in (1, 3, 8, 9, 16, 17):
+        x = rand((T, K), dtypes()[xt], K + T)
+        if T == 9:
+            x[4, K // 2] = float("inf")
+            x[8, K - 1] = float("nan")
+            x[2] = 0
+        codes, scale = qgmoe.quantize_rows(x)
+        for yt in dtypes().values():
+            y = lin.forward_device(x, dtype=yt)
+            want = lin.matmul_device(codes, scale, dtype=yt)
+            assert t.equal(t.isnan(y), t.isnan(want))
+            assert t.equal(t.nan_to_num(y), t.nan_to_num(want))
+        if T == 9:
+            assert t.isnan(y[[4, 8]]).all() and not t.isnan(y[:4]).any()
+    off = rand((3 * K + 1,), dtypes()[xt], 1)[1:].view(3, K)   # not 16-byte aligned
+    codes, scale = qgmoe.quantize_rows(off)
+    assert t.equal(lin.forward_device(off, dtype=t.float32), lin.matmul_device(codes, scale))
+    lin.sync()
+
+
 def test_codes_at_the_limits_of_32_bits():
     """The longest row, every code -128: the sum is 2^14 * 131071 < 2^31."""
     t = torch_()
