@@ -1340,7 +1340,7 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
 // output columns [rt*64, rt*64 + 64): of each 32 tile rows the first 16 are
 // gate rows of 16 columns, the others the up rows of the same columns.
 __global__ void k_i8_layout(const int8_t *q, const float *scale, int O, int I, int swiglu, int RT,
-                            int KB, int8_t *dst, float *dscale) {
+                            int KB, int vec, int8_t *dst, float *dscale) {
     const int64_t row = blockIdx.x, tile = row / I8_M;  // of groups * RT * 128
     const int g = (int)(tile / RT);
     const int l = (int)(row - (int64_t)g * RT * I8_M);
@@ -1357,9 +1357,17 @@ __global__ void k_i8_layout(const int8_t *q, const float *scale, int O, int I, i
     }
     const int8_t *src = q + ((int64_t)g * O + o) * I;
     int8_t *d = dst + (tile * KB * I8_M + row % I8_M) * I8_BK;
-    for (int i = threadIdx.x; i < KB * I8_BK; i += blockDim.x)
-        d[(int64_t)(i / I8_BK) * (I8_M * I8_BK) + i % I8_BK] =
-            live && i < I ? src[i] : (int8_t)0;
+    if (vec) {  // 16-byte pieces: in % 16 == 0 and an aligned source
+        for (int i = threadIdx.x * 16; i < KB * I8_BK; i += blockDim.x * 16) {
+            uint4 u = make_uint4(0, 0, 0, 0);
+            if (live && i < I) u = *reinterpret_cast<const uint4 *>(src + i);
+            *reinterpret_cast<uint4 *>(d + (int64_t)(i / I8_BK) * (I8_M * I8_BK) + i % I8_BK) = u;
+        }
+    } else {
+        for (int i = threadIdx.x; i < KB * I8_BK; i += blockDim.x)
+            d[(int64_t)(i / I8_BK) * (I8_M * I8_BK) + i % I8_BK] =
+                live && i < I ? src[i] : (int8_t)0;
+    }
     if (threadIdx.x == 0) dscale[row] = live ? scale[(int64_t)g * O + o] : 0.f;
 }
 
@@ -1430,8 +1438,8 @@ struct qgq8 {
     int RT = 0, live = 0;  // 128-row weight tiles per group, and those that hold channels
     bool swiglu = false;
     cudaStream_t stream = nullptr;
-    int8_t *w = nullptr;   // [G * RT, KB, 128, 128]
-    float *ws = nullptr;   // [G * RT * 128]
+    int8_t *w = nullptr;   // [G * RT, KB, 128, 128], one allocation with
+    float *ws = nullptr;   // [G * RT * 128] and
     int *err_dev = nullptr;
     CUtensorMap tmap_w{};
     // qgq8_forward's own buffers (it blocks, so no work outlives the call)
@@ -1656,22 +1664,28 @@ static int i8_alloc(void **p, size_t bytes) {
     return QGMOE_OK;
 }
 
+static int i8_layout_vec(const qgq8 *h, const int8_t *q) {
+    return h->I % 16 == 0 && !(reinterpret_cast<uintptr_t>(q) & 15);
+}
+
 // Device copies of the weights in tile order.  Host weights travel through a
 // staging buffer of whole groups, 64 MB or one group.
 static int i8_build(qgq8 *h, const int8_t *q, const float *scale, bool on_device) {
     const int64_t rows = (int64_t)h->G * h->RT * I8_M, row_bytes = (int64_t)h->KB * I8_BK;
-    int rc = i8_alloc(reinterpret_cast<void **>(&h->w), (size_t)(rows * row_bytes));
-    if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->ws), sizeof(float) * rows);
-    if (!rc) rc = i8_alloc(reinterpret_cast<void **>(&h->err_dev), sizeof(int));
-    if (!rc) rc = i8_encode_map(&h->tmap_w, h->w, rows * h->KB, I8_BK, I8_BK, I8_M);
+    int rc = i8_alloc(reinterpret_cast<void **>(&h->w),
+                      (size_t)(rows * row_bytes) + sizeof(float) * rows + sizeof(int));
+    if (rc) return rc;
+    h->ws = reinterpret_cast<float *>(h->w + rows * row_bytes);
+    h->err_dev = reinterpret_cast<int *>(h->ws + rows);
+    rc = i8_encode_map(&h->tmap_w, h->w, rows * h->KB, I8_BK, I8_BK, I8_M);
     if (rc) return rc;
     QG_CUDA(cudaMemsetAsync(h->err_dev, 0, sizeof(int), h->stream));
     const int64_t gbytes = (int64_t)h->O * h->I;
     if (on_device) {
         // whatever stream the caller wrote the weights on
         QG_CUDA(cudaDeviceSynchronize());
-        k_i8_layout<<<(unsigned)rows, 256, 0, h->stream>>>(q, scale, h->O, h->I, h->swiglu, h->RT,
-                                                           h->KB, h->w, h->ws);
+        k_i8_layout<<<(unsigned)rows, 128, 0, h->stream>>>(q, scale, h->O, h->I, h->swiglu, h->RT,
+                                                           h->KB, i8_layout_vec(h, q), h->w, h->ws);
         QG_CUDA(cudaGetLastError());
         QG_CUDA(cudaStreamSynchronize(h->stream));
         return QGMOE_OK;
@@ -1691,8 +1705,9 @@ static int i8_build(qgq8 *h, const int8_t *q, const float *scale, bool on_device
                                 cudaMemcpyHostToDevice, h->stream);
         if (e != cudaSuccess) break;
         const int64_t r0 = g * h->RT * I8_M;
-        k_i8_layout<<<(unsigned)(n * h->RT * I8_M), 256, 0, h->stream>>>(
-            tq, ts, h->O, h->I, h->swiglu, h->RT, h->KB, h->w + r0 * row_bytes, h->ws + r0);
+        k_i8_layout<<<(unsigned)(n * h->RT * I8_M), 128, 0, h->stream>>>(
+            tq, ts, h->O, h->I, h->swiglu, h->RT, h->KB, i8_layout_vec(h, tq),
+            h->w + r0 * row_bytes, h->ws + r0);
         e = cudaGetLastError();
         if (e == cudaSuccess) e = cudaStreamSynchronize(h->stream);  // tq is reused
     }
@@ -1755,8 +1770,6 @@ int qgq8_destroy(qgq8_t *h) {
         cudaDeviceSynchronize();  // products on the caller's streams read the weights
         i8_free_work(h);
         cudaFree(h->w);
-        cudaFree(h->ws);
-        cudaFree(h->err_dev);
         if (h->stream) cudaStreamDestroy(h->stream);
     }
     delete h;

@@ -114,8 +114,8 @@ template <> struct Vec8<float> {  // two 16-byte loads
 // an IEEE float32 quotient (the rule of quantizeInt8, model/moe.go:165-188).
 // A quotient is first formed as t = x y with y the rounded reciprocal of the
 // scale, within 2.3e-5 of x / scale as |t| <= 127; adding 1.5 * 2^23 rounds it
-// and leaves the code in the low byte.  Only a t within 1e-4 of a half can
-// round otherwise than the quotient does.  Vectors with one (one in 600 of
+// and leaves the code in the low byte.  Only a t within 3e-5 of a half can
+// round otherwise than the quotient does.  Vectors with one (one in 2000 of
 // float32 values, more of 16-bit ones, whose quotients often are halves) get
 // the correctly rounded quotient, by Markstein's iteration (1990): the
 // remainder r = x - t s is exact in one fused operation and t + r y is within
@@ -193,45 +193,44 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
     return r;
 }
-static __device__ __noinline__ uint2 codes_near_half(float v0, float v1, float v2, float v3, float v4,
-                                              float v5, float v6, float v7, float s, float inv) {
-    constexpr float MAGIC = 12582912.f;
-    const float v[8] = {v0, v1, v2, v3, v4, v5, v6, v7};
-    const bool divide = (__float_as_uint(s) & 0x7FFFFFu) == 0x7FFFFFu;
-    uint32_t c[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        float q = __fmul_rn(v[i], inv);
-        q = __fmaf_rn(__fmaf_rn(-q, s, v[i]), inv, q);
-        q = __fmaf_rn(__fmaf_rn(-q, s, v[i]), inv, q);
-        if (divide) q = __fdiv_rn(v[i], s);
-        const float r = __fadd_rn(q, MAGIC);
-        const float e = __fsub_rn(q, __fsub_rn(r, MAGIC));  // exact
-        c[i] = __float_as_uint(fabsf(e) == 0.5f
-                                   ? __fadd_rn(__fadd_rn(q, copysignf(0.5f, q)), MAGIC)
-                                   : r);
-    }
-    return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
-}
 // inv: __frcp_rn(s)
 __device__ __forceinline__ uint2 codes_of(const float (&v)[8], float s, float inv) {
     constexpr float MAGIC = 12582912.f;
     const uint64_t y = f2(inv, inv), magic = f2(MAGIC, MAGIC), minus_magic = f2(-MAGIC, -MAGIC);
     const uint64_t minus_one = f2(-1.f, -1.f);
+    uint64_t t[4];
     uint32_t c[8];
     float far = 0.f;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const uint64_t t = mul2(f2(v[2 * i], v[2 * i + 1]), y);
-        const uint64_t r = add2(t, magic);
-        const float2 e = unf2(fma2(add2(r, minus_magic), minus_one, t));  // t - round(t), exact
+        t[i] = mul2(f2(v[2 * i], v[2 * i + 1]), y);
+        const uint64_t r = add2(t[i], magic);
+        const float2 e = unf2(fma2(add2(r, minus_magic), minus_one, t[i]));  // exact
         const float2 rf = unf2(r);
         c[2 * i] = __float_as_uint(rf.x);
         c[2 * i + 1] = __float_as_uint(rf.y);
         far = fmaxf(far, fmaxf(fabsf(e.x), fabsf(e.y)));
     }
-    if (far > 0.4999f)
-        return codes_near_half(v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7], s, inv);
+    if (far > 0.49997f) {
+        const uint64_t minus_s = f2(-s, -s);
+        const bool divide = (__float_as_uint(s) & 0x7FFFFFu) == 0x7FFFFFu;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t x = f2(v[2 * i], v[2 * i + 1]);
+            uint64_t q = fma2(fma2(t[i], minus_s, x), y, t[i]);
+            q = fma2(fma2(q, minus_s, x), y, q);
+            if (divide) q = f2(__fdiv_rn(v[2 * i], s), __fdiv_rn(v[2 * i + 1], s));
+            const uint64_t r = add2(q, magic);
+            const float2 e = unf2(fma2(add2(r, minus_magic), minus_one, q));
+            const float2 qf = unf2(q), rf = unf2(r);
+            auto code = [](float q, float r, float e) {
+                const float away = __fadd_rn(__fadd_rn(q, copysignf(0.5f, q)), MAGIC);
+                return __float_as_uint(fabsf(e) == 0.5f ? away : r);
+            };
+            c[2 * i] = code(qf.x, rf.x, e.x);
+            c[2 * i + 1] = code(qf.y, rf.y, e.y);
+        }
+    }
     return make_uint2(pack4(c[0], c[1], c[2], c[3]), pack4(c[4], c[5], c[6], c[7]));
 }
 

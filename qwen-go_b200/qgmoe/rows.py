@@ -35,7 +35,7 @@ def _load():
     import torch
     _DT = {torch.float32: _q.DT_F32, torch.float16: _q.DT_F16, torch.bfloat16: _q.DT_BF16}
     _raw_stream = torch._C._cuda_getCurrentRawStream
-    _cur_device = torch.cuda.current_device
+    _cur_device = torch._C._cuda_getDevice
     _torch = torch
     return torch
 
@@ -48,7 +48,9 @@ def _row_dtype(t, what: str) -> int:
 
 
 def _need(t, what: str, device, shape=None, dtype=None):
-    """A contiguous tensor on `device` of that shape (a tuple) and type."""
+    """A contiguous tensor on `device` of that shape (a tuple) and type; raises
+    ValueError with what is wrong.  The calls below test the usual case
+    themselves and come here to say why it is not."""
     if t.device != device:
         raise ValueError(f"{what}: on {t.device}, expected {device}")
     if not t.is_contiguous():
@@ -146,12 +148,13 @@ class TokenOrder:
     def sort(self, sel_idx, stream=None) -> "TokenOrder":
         """sel_idx [n_tokens, top_k] int32, as a router selects (MoeMLP's
         sel_idx, qgmoe_route_static); ids outside [0, n_experts) get no row."""
-        _need(sel_idx, "sel_idx", self.device, (self.n_tokens, self.top_k), _torch.int32)
         _on(self.device, stream, self._sort, sel_idx)
         return self
 
     def _sort(self, sel_idx, s):
-        _call("qgmoe_sort_tokens", sel_idx.data_ptr(), self.n_tokens, self.top_k, self.n_experts,
+        T, k = self.n_tokens, self.top_k
+        _need(sel_idx, "sel_idx", self.device, (T, k), _torch.int32)
+        _call("qgmoe_sort_tokens", sel_idx.data_ptr(), T, k, self.n_experts,
               self.offsets.data_ptr(), self.pair_row.data_ptr(), self.row_pair.data_ptr(), s)
 
 
@@ -169,11 +172,14 @@ def sort_tokens(sel_idx, n_experts: int, stream=None) -> TokenOrder:
 
 def _rows_of(t, what: str, order: TokenOrder, n: int):
     """(row dtype, row length) of [n, H] rows on the order's device."""
-    _need(t, what, order.device)
-    shape = t.shape
-    if len(shape) != 2 or shape[0] != n or shape[1] < 1:
-        raise ValueError(f"{what}: shape {tuple(shape)}, expected [{n}, row length]")
-    return _row_dtype(t, what), shape[1]
+    shape, dt = t.shape, _DT.get(t.dtype)
+    if dt is None or len(shape) != 2 or shape[0] != n or shape[1] < 1 or \
+            t.device != order.device or not t.is_contiguous():
+        _need(t, what, order.device)
+        if len(shape) != 2 or shape[0] != n or shape[1] < 1:
+            raise ValueError(f"{what}: shape {tuple(shape)}, expected [{n}, row length]")
+        _row_dtype(t, what)
+    return dt, shape[1]
 
 
 def _result(out, what: str, like, shape, dtype):
