@@ -35,6 +35,7 @@
 #include <math_constants.h>
 
 #include <new>
+#include <type_traits>
 
 #include "qg_rows.cuh"
 
@@ -92,7 +93,7 @@ struct I8Args {
     int CT;                  // channel tiles per group: those with channels, or RT / 2 for pairs
     int nt, gran;            // most rows of a tile; tiles are multiples of gran rows
     void *y;                 // [R, cols]
-    int vec;                 // y rows are 16-byte aligned
+    int align;               // of y's 16-bit rows, in bytes: 16, 4 or 2
     int *err;
 };
 
@@ -518,12 +519,20 @@ struct I8Epilogue {
 #pragma unroll
                     for (int e = 0; e < N / 2; e++)
                         p[e] = movmatrix(pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y));
-                    if (WHOLE || (a.vec && i * 8 + ro < nc && o < a.cols)) {
-                        if constexpr (SWIGLU)
-                            *reinterpret_cast<uint2 *>(yp) = make_uint2(p[0], p[1]);
-                        else
-                            *reinterpret_cast<uint4 *>(yp) = make_uint4(p[0], p[1], p[2], p[3]);
-                    } else if (!a.vec && i * 8 + ro < nc) {
+                    const bool real = WHOLE || i * 8 + ro < nc;
+                    if (WHOLE || a.align == 16) {  // cols % 8 == 0: all N channels or none
+                        if (WHOLE || (real && o < a.cols)) {
+                            if constexpr (SWIGLU)
+                                *reinterpret_cast<uint2 *>(yp) = make_uint2(p[0], p[1]);
+                            else
+                                *reinterpret_cast<uint4 *>(yp) = make_uint4(p[0], p[1], p[2], p[3]);
+                        }
+                    } else if (a.align >= 4) {  // an even number of columns: pairs
+#pragma unroll
+                        for (int e = 0; e < N / 2; e++)
+                            if (real && o + 2 * e < a.cols)
+                                reinterpret_cast<uint32_t *>(yp)[e] = p[e];
+                    } else if (real) {
 #pragma unroll
                         for (int e = 0; e < N; e++)
                             if (o + e < a.cols)
@@ -543,7 +552,7 @@ struct I8Epilogue {
     __device__ __forceinline__ void drain(uint32_t tmem, int64_t row0, int n, int rt, F read) {
         const int o0 = (rt * 4 + q) * CH;
         // all channels exist (and 16-bit rows are aligned): nothing to check
-        const bool whole = o0 + CH <= a.cols && (F32 || a.vec);
+        const bool whole = o0 + CH <= a.cols && (F32 || a.align == 16);
         if (first >= n) read();
 #pragma unroll
         for (int i = 0; i < RUNS; i++) {
@@ -1048,8 +1057,9 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 // while the weights are on their way; warps 0-3 are the epilogue after that:
 // the partial sums of lane quarter q go to the CTA q * split / 4 of the
 // cluster, which adds them (exactly, as integers) and writes y.
-// One token, 2048 -> 4096: 5.6 us, where the quantiser and k_i8 took 8.3 in two
-// launches (5 us of that the product of one CTA per tile, 32 of 148 SMs).
+// One token, 2048 -> 4096: 5.7 us, where the quantiser and k_i8 take 7.2 in two
+// launches, the product on 32 of 148 SMs.  What is left is latency: launch,
+// cluster start, one read of x, one exchange.
 constexpr int I8F_ROWS = 16;
 constexpr int I8F_WARPS = 8;
 constexpr int I8F_LOAD_WARP = 8, I8F_MMA_WARP = 9;
@@ -1070,29 +1080,88 @@ static int i8f_smem(int blocks) {
            4 * (I8F_SPLIT - 1) * I8F_PART_BYTES + 2048;
 }
 
-// Eight values of row r from column c on, zeros past the row's end.
-template <typename TI>
-__device__ __forceinline__ void i8f_load8(const void *x, int64_t at, int left, bool vec,
-                                          float (&v)[8]) {
-    const TI *p = static_cast<const TI *>(x) + at;
-    if (vec) {
-        Vec8<TI> in;
-        in.load(p);
-        in.get(v);
-    } else {
+// The rows' scales and this CTA's blocks of their codes, by warps 0-7.  A
+// template on the type and the alignment, not a branch per load: the loads of
+// several vectors are in flight together.
+template <typename TI, bool VEC>
+__device__ __forceinline__ void i8f_quantize(const I8FewArgs &f, int kb0, int nb, uint32_t codes,
+                                             uint32_t (*s_max)[I8F_WARPS], float *s_scale) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = f.a.R;
+    auto load = [&](int r, int c, float (&v)[8]) {
+        const TI *p = static_cast<const TI *>(f.x) + (int64_t)r * f.K + c;
+        if constexpr (VEC) {
+            Vec8<TI> in;
+            in.load(p);
+            in.get(v);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = i < left ? Elem<TI>::load(p + i) : 0.f;
+            for (int i = 0; i < 8; i++) v[i] = c + i < f.K ? Elem<TI>::load(p + i) : 0.f;
+        }
+    };
+    // a row by one warp, or by two, four or eight where rows are fewer
+    const int per = R >= 8 ? 1 : R >= 4 ? 2 : R >= 2 ? 4 : 8;
+    auto top_of = [&](auto in_flight, int r) {
+        constexpr int U = decltype(in_flight)::value;  // vectors of a lane
+        float m = 0.f;                                 // a maximum that keeps NaN
+        for (int c0 = (warp % per * 32 + lane) * 8; c0 < f.K; c0 += U * per * 256) {
+            float v[U][8];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int c = c0 + u * per * 256;
+                if (c < f.K) {
+                    load(r, c, v[u]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) v[u][i] = 0.f;
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[u][i])));
+        }
+        return __reduce_max_sync(~0u, __float_as_uint(m));
+    };
+    for (int r = warp / per; r < R; r += I8F_WARPS / per) {
+        const uint32_t top = VEC && f.K > 2 * per * 256
+                                 ? top_of(std::integral_constant<int, 8>(), r)
+                                 : top_of(std::integral_constant<int, 1>(), r);
+        if (lane == 0) s_max[r][warp % per] = top;
     }
-}
-__device__ __forceinline__ void i8f_load8(const I8FewArgs &f, int r, int c, float (&v)[8]) {
-    const int64_t at = (int64_t)r * f.K + c;
-    const int left = f.K - c;
-    if (f.x_dtype == QGMOE_DT_F32)
-        i8f_load8<float>(f.x, at, left, f.x_vec, v);
-    else if (f.x_dtype == QGMOE_DT_F16)
-        i8f_load8<__half>(f.x, at, left, f.x_vec, v);
-    else
-        i8f_load8<__nv_bfloat16>(f.x, at, left, f.x_vec, v);
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (tid < I8F_ROWS) {
+        uint32_t m = 0;
+        if (tid < R)
+            for (int w = 0; w < per; w++) m = max(m, s_max[tid][w]);
+        // what was not finite makes the row's products NaN
+        s_scale[tid] = m >= 0x7F800000u ? CUDART_NAN_F : scale_of(m);
+        s_scale[16 + tid] = 0.f;
+    }
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    const int lo = kb0 * I8_BK, cols = min(f.K, lo + nb * I8_BK) - lo, vecs = nb * (I8_BK / 8);
+    constexpr int W = VEC ? 4 : 1;
+    for (int i0 = tid; i0 < R * vecs; i0 += W * I8F_WARPS * 32) {
+        float v[W][8];
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const int i = i0 + w * I8F_WARPS * 32, r = i / vecs, c = (i - r * vecs) * 8;
+            if (i < R * vecs && c < cols) load(r, lo + c, v[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const int i = i0 + w * I8F_WARPS * 32, r = i / vecs, c = (i - r * vecs) * 8;
+            if (i >= R * vecs) break;
+            uint2 u = make_uint2(0, 0);
+            const float s = s_scale[r];
+            if (c < cols && s == s) u = codes_of(v[w], s, __frcp_rn(s));
+            const int j = c % I8_BK;
+            const uint32_t at = codes + c / I8_BK * I8F_CODE_BYTES + r * I8_BK +
+                                (((j >> 4) ^ (r & 7)) << 4) + (j & 8);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(u.x), "r"(u.y)
+                         : "memory");
+        }
+    }
 }
 
 __device__ __forceinline__ bool i8_try_wait_cluster(uint32_t bar, uint32_t parity) {
@@ -1162,44 +1231,20 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
     if (warp < I8F_WARPS) {
         pdl_wait();  // x
         // ============ rows -> codes ===============================================
-        for (int r = 0; r < a.R; r++) {
-            float m = 0.f;  // a maximum that keeps NaN
-#pragma unroll 4
-            for (int c = tid * 8; c < f.K; c += I8F_WARPS * 256) {
-                float v[8];
-                i8f_load8(f, r, c, v);
-#pragma unroll
-                for (int i = 0; i < 8; i++)
-                    asm("max.NaN.f32 %0, %0, %1;" : "+f"(m) : "f"(fabsf(v[i])));
-            }
-            const uint32_t top = __reduce_max_sync(~0u, __float_as_uint(m));
-            if (lane == 0) s_max[r][warp] = top;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (tid < I8F_ROWS) {
-            uint32_t m = 0;
-            if (tid < a.R)
-                for (int w = 0; w < I8F_WARPS; w++) m = max(m, s_max[tid][w]);
-            // what was not finite makes the row's products NaN
-            s_scale[tid] = m >= 0x7F800000u ? CUDART_NAN_F : scale_of(m);
-            s_scale[16 + tid] = 0.f;
-        }
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        const int lo = kb0 * I8_BK, cols = min(f.K, lo + nb * I8_BK) - lo;
-        for (int i = tid; i < a.R * (nb * I8_BK / 8); i += I8F_WARPS * 32) {
-            const int r = i / (nb * I8_BK / 8), c = (i - r * (nb * I8_BK / 8)) * 8;
-            uint2 u = make_uint2(0, 0);
-            const float s = s_scale[r];
-            if (c < cols && s == s) {
-                float v[8];
-                i8f_load8(f, r, lo + c, v);
-                u = codes_of(v, s, __frcp_rn(s));
-            }
-            const int j = c % I8_BK;
-            const uint32_t at = codes + c / I8_BK * I8F_CODE_BYTES + r * I8_BK +
-                                (((j >> 4) ^ (r & 7)) << 4) + (j & 8);
-            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(u.x), "r"(u.y)
-                         : "memory");
+        if (f.x_vec) {
+            if (f.x_dtype == QGMOE_DT_F32)
+                i8f_quantize<float, true>(f, kb0, nb, codes, s_max, s_scale);
+            else if (f.x_dtype == QGMOE_DT_F16)
+                i8f_quantize<__half, true>(f, kb0, nb, codes, s_max, s_scale);
+            else
+                i8f_quantize<__nv_bfloat16, true>(f, kb0, nb, codes, s_max, s_scale);
+        } else {
+            if (f.x_dtype == QGMOE_DT_F32)
+                i8f_quantize<float, false>(f, kb0, nb, codes, s_max, s_scale);
+            else if (f.x_dtype == QGMOE_DT_F16)
+                i8f_quantize<__half, false>(f, kb0, nb, codes, s_max, s_scale);
+            else
+                i8f_quantize<__nv_bfloat16, false>(f, kb0, nb, codes, s_max, s_scale);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -1549,6 +1594,11 @@ static int i8_check_product(const qgq8 *h, const int8_t *codes, int64_t ld, cons
     return QGMOE_OK;
 }
 
+static int i8_align(const qgq8 *h, const void *y) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(y);
+    return h->cols % 8 == 0 && p % 16 == 0 ? 16 : h->cols % 2 == 0 && p % 4 == 0 ? 4 : 2;
+}
+
 static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const float *scale, int R,
                       const int32_t *offsets, void *y, int ydt, cudaStream_t s) {
     const int64_t per = (R + (int64_t)h->G - 1) / h->G;  // mean rows of a group
@@ -1570,7 +1620,7 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     a.nt = nt;
     a.gran = pair ? 32 : 16;
     a.y = y;
-    a.vec = h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
+    a.align = i8_align(h, y);
     a.err = h->err_dev;
     // row tiles: full ones, and at most one partial for each group that has rows
     const int64_t tiles = R / nt + (R < h->G ? R : h->G);
@@ -1580,8 +1630,12 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
                       : launch_i8<I8P_NT>(h, tx, a, ydt, units, s);
 }
 
-// Rows up to which a dense product runs on k_i8_few: 16, if a CTA's share of
-// the row codes fits next to its weights.
+// Rows up to which a dense product runs on k_i8_few: 16, if its CTAs, each of
+// which quantises the rows, are resident at once and a CTA's share of the row
+// codes fits next to its weights.  2048 -> 4096, this kernel and the two others
+// on the device: 1 row 5.7 and 7.2 us, 8 rows 7.3 and 7.3, 16 rows 8.7 and 7.3;
+// but one launch instead of two and no workspace save 4.5 us of host time,
+// which is what a call of this size waits for.
 static int i8_few_split(const qgq8 *h) {
     int split = 1;
     while (split < I8F_SPLIT && h->live * split * 2 <= num_sms(h->device) && h->KB >= split * 4)
@@ -1589,7 +1643,7 @@ static int i8_few_split(const qgq8 *h) {
     return split;
 }
 static int i8_few_rows(const qgq8 *h) {
-    if (h->G != 1) return 0;
+    if (h->G != 1 || h->live > num_sms(h->device)) return 0;
     const int split = i8_few_split(h);
     return (h->KB + split - 1) / split <= I8F_BLOCKS ? I8F_ROWS : 0;
 }
@@ -1629,7 +1683,7 @@ static int i8_few(const qgq8 *h, const void *x, int xdt, int R, void *y, int ydt
     f.a.KB = h->KB;
     f.a.cols = h->cols;
     f.a.y = y;
-    f.a.vec = h->cols % 8 == 0 && !(reinterpret_cast<uintptr_t>(y) & 15);
+    f.a.align = i8_align(h, y);
     f.a.err = h->err_dev;
     f.x = x;
     f.x_dtype = xdt;
