@@ -389,7 +389,7 @@ int qgql_quantize_device(int32_t bits, int32_t out_features, int32_t in_features
  * output's type.  T * k is at most QGMOE_MAX_PAIRS; T = 0 is allowed.
  * Outputs may not overlap inputs. */
 #define QGMOE_MAX_PAIRS (1 << 30)
-#define QGMOE_MAX_ROW (1 << 24)
+#define QGMOE_MAX_ROW (1 << 22)
 
 /* sel_idx [T, k] int32 -> offsets [E + 1] (first row of each expert, then the
  * number of pairs that have one), pair_row [T, k] (the pair's row) and, unless

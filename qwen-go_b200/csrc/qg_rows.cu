@@ -599,7 +599,7 @@ int check_quantize_rows(const void *x, int dt, int T, int k, int K, const int32_
                         const void *codes, int64_t ld, const void *scale) {
     int rc = check_rows(T, k, K, dt, dt, "quantize_rows");
     if (rc) return rc;
-    if (!pair_row && k != 1)
+    if (T > 0 && !pair_row && k != 1)
         return set_error(QGMOE_ERR_INVALID_ARG, "quantize_rows: k=%d without pair_row", k);
     if (ld < K || ld % 16 || ld > (int64_t)QGMOE_MAX_ROW + 15)
         return set_error(QGMOE_ERR_INVALID_ARG,

@@ -207,6 +207,34 @@ def test_no_rows():
     t = torch_()
     lin = qgmoe.Int8Linear(*weights((8, 16), 1))
     assert lin.forward_device(t.empty((0, 16), device="cuda")).shape == (0, 8)
+    lin = qgmoe.Int8Linear(*weights((2, 8, 16), 1))
+    order = qgmoe.sort_tokens(t.empty((0, 3), dtype=t.int32, device="cuda"), 2)
+    x = t.empty((0, 16), device="cuda")
+    assert lin.forward_device(x, order=order).shape == (0, 8)
+    assert lin.forward_device(x, offsets=order.offsets).shape == (0, 8)
+    codes, scale = qgmoe.quantize_rows(x, order)
+    assert lin.matmul_device(codes, scale, offsets=order.offsets).shape == (0, 8)
+
+
+@pytest.mark.parametrize("N", [24, 26, 27, 130])
+@pytest.mark.parametrize("yt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_rows_of_y_at_odd_addresses(N, yt, swiglu):
+    """y's rows on 16-, 4- and 2-byte boundaries, at one, a few dozen and a few
+    hundred rows: each kernel's every way out.  What surrounds y stays."""
+    t = torch_()
+    dt = dtypes()[yt]
+    q, ws = weights((2 * N if swiglu else N, 200), N)
+    lin = qgmoe.Int8Linear(q, ws, swiglu=swiglu)
+    for T in (3, 40, 300):
+        x = rand((T, 200), t.float32, T)
+        want = lin.forward_device(x, dtype=t.float32).to(dt)
+        for off in (0, 1, 2, 8):
+            buf = t.full((T * N + off + 16,), 5.0, dtype=dt, device="cuda")
+            y = buf[off:off + T * N].view(T, N)
+            lin.forward_device(x, y)
+            assert t.equal(y, want), (T, off)
+            assert t.all(buf[:off] == 5.0) and t.all(buf[off + T * N:] == 5.0)
 
 
 # ---- products by expert -------------------------------------------------------------

@@ -5,6 +5,8 @@ Tolerances count roundings, u = 2^-24 for float32 and half an epsilon of the
 output's type: a sum of n fused products has error at most n u sum|terms|
 (first order), a product u |value|, and the final rounding eps/2 |value|; a
 factor 1.01 covers the second order."""
+import os
+
 import numpy as np
 import pytest
 
@@ -78,7 +80,8 @@ def f64(t):
 
 # ---- sort -------------------------------------------------------------------
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 8, 128), (3, 2, 5), (64, 8, 128), (333, 6, 60),
-                                   (100, 32, 64), (513, 1, 1024), (4097, 8, 128), (16384, 2, 3)])
+                                   (100, 32, 64), (513, 1, 1024), (4097, 8, 128), (16384, 2, 3),
+                                   (4000, 1, 7), (9000, 4, 1024), (40000, 8, 33)])
 @pytest.mark.parametrize("bad", [0.0, 0.3, 1.0])
 def test_sort(T, k, E, bad):
     idx = routing(T, k, E, T + k, bad)
@@ -337,6 +340,48 @@ def test_two_captured_graphs_interleaved():
         for _idx, _x, _g, res, step in (a, b):
             for got, want in zip(res, step()):
                 assert t.equal(got, want)
+
+
+_FIRST_CALLS = """
+import sys
+sys.path.insert(0, {pkg!r})
+import torch, qgmoe
+T, k, E, H = 48, 2, 4, 64
+idx = torch.randint(0, E, (T, k), dtype=torch.int32, device="cuda")
+x, w = torch.randn(T, H, device="cuda"), torch.rand(T, k, device="cuda")
+q = torch.randint(-127, 128, (E, 32, H), dtype=torch.int8, device="cuda")
+lin = qgmoe.Int8Linear(q, torch.rand(E, 32, device="cuda"))
+one = qgmoe.Int8Linear(q[0], torch.rand(32, device="cuda"))
+order = qgmoe.TokenOrder(T, k, E)
+def step():
+    order.sort(idx)
+    rows = qgmoe.gather_rows(x, order)
+    gr, gw = qgmoe.combine_rows_backward(x, rows, w, order)
+    return (rows, qgmoe.combine_rows(rows, w, order), gr, gw, qgmoe.gather_rows_backward(gr, order),
+            lin.forward_device(x, order=order), one.forward_device(x), one.forward_device(x[:3]),
+            *qgmoe.quantize_rows(x))
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+got = [t.clone() for t in got]
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+lin.sync()
+print("captured")
+"""
+
+
+def test_first_calls_inside_a_capture():
+    """A process whose first calls are captured: nothing is allocated, looked
+    up or waited for in a way that a capture does not allow."""
+    import subprocess
+    import sys
+    pkg = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "qwen-go_b200")
+    r = subprocess.run([sys.executable, "-c", _FIRST_CALLS.format(pkg=pkg)], capture_output=True,
+                       text=True, timeout=120)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
 
 
 def test_long_offsets():

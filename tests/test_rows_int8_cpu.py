@@ -27,7 +27,7 @@ def test_sort_refuses(args):
 
 @pytest.mark.parametrize("T,k,H,a,b,null", [
     (-1, 2, 8, 0, 0, None), (4, 0, 8, 0, 0, None), (BIG, 2, 8, 0, 0, None), (4, 2, 0, 0, 0, None),
-    (4, 2, (1 << 24) + 1, 0, 0, None), (4, 2, 8, 3, 0, None), (4, 2, 8, 0, 6, None),
+    (4, 2, (1 << 22) + 1, 0, 0, None), (4, 2, 8, 3, 0, None), (4, 2, 8, 0, 6, None),
     (4, 2, 8, -1, 0, None), (4, 2, 8, 0, 0, 0), (4, 2, 8, 0, 0, 1), (4, 2, 8, 0, 0, 2)])
 def test_row_calls_refuse(T, k, H, a, b, null):
     p = [None if i == null else ONE for i in range(3)]
