@@ -22,7 +22,7 @@
 namespace qg {
 
 // ---- sort -------------------------------------------------------------------
-// One cluster of up to eight CTAs, no workspace, one launch.  Each warp owns a
+// One cluster of up to sixteen CTAs, no workspace, one launch.  Each warp owns a
 // contiguous range of pairs and takes it 32 at a time: lanes with the same
 // expert find each other (a ballot per bit of the id; match.any is several
 // times slower), rank themselves in lane order on top of the warp's count of
@@ -33,7 +33,7 @@ namespace qg {
 // Every id is handled once: 32768 pairs over 128 experts take 5 us, where one
 // CTA per expert, each counting all pairs, took 12.
 constexpr int SORT_MAX_WARPS = 32;
-constexpr int SORT_MAX_CTAS = 8;
+constexpr int SORT_MAX_CTAS = 16;  // beyond eight, where the device allows it
 constexpr int SORT_STEPS = 4;  // steps of 32 whose loads are in flight together
 
 __device__ __forceinline__ int ld_i32_if(bool on, const int32_t *p, int other) {
@@ -52,15 +52,18 @@ __device__ __forceinline__ int ld_cluster_i32(uint32_t addr) {
     return v;
 }
 
-// Lanes whose v (below 2^bits) equals this lane's.
-__device__ __forceinline__ unsigned same_lanes(int v, int bits) {
-    unsigned m = ~0u;
-    for (int b = 0; b < bits; b++) {
-        const bool on = (v >> b) & 1;
-        const unsigned w = __ballot_sync(~0u, on);
-        m &= on ? w : ~w;
-    }
-    return m;
+// m[b]: the lanes whose v[b] (below 2^bits) equals this lane's.
+__device__ __forceinline__ void same_lanes(const int (&v)[SORT_STEPS], int bits,
+                                           unsigned (&m)[SORT_STEPS]) {
+#pragma unroll
+    for (int b = 0; b < SORT_STEPS; b++) m[b] = ~0u;
+    for (int bit = 0; bit < bits; bit++)
+#pragma unroll
+        for (int b = 0; b < SORT_STEPS; b++) {
+            const bool on = (v[b] >> bit) & 1;
+            const unsigned w = __ballot_sync(~0u, on);
+            m[b] &= on ? w : ~w;
+        }
 }
 
 __global__ void __launch_bounds__(SORT_MAX_WARPS * 32)
@@ -91,11 +94,16 @@ k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_
             const int64_t i = i0 + b * 32 + lane;
             id[b] = ld_i32_if(i < hi, ids + i, -1);
         }
+        int key[SORT_STEPS];
+        unsigned same[SORT_STEPS];
+#pragma unroll
+        for (int b = 0; b < SORT_STEPS; b++) key[b] = (unsigned)id[b] < (unsigned)E ? id[b] : E;
+        same_lanes(key, bits, same);
 #pragma unroll
         for (int b = 0; b < SORT_STEPS; b++) {
             const int64_t i = i0 + b * 32 + lane;
-            const bool valid = (unsigned)id[b] < (unsigned)E;
-            const unsigned peers = same_lanes(valid ? id[b] : E, bits);
+            const bool valid = key[b] < E;
+            const unsigned peers = same[b];
             const int ahead = __popc(peers & below);
             const int so_far = valid ? mine[id[b]] : 0;
             __syncwarp();
@@ -425,25 +433,45 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t 
             *reinterpret_cast<uint2 *>(out + c) = u;
         }
     } else {
+        // 16 codes a store where the row allows it, of values that other lanes
+        // of the row's warps have copied (the barrier is the maximum's)
+        const bool wide = K % 16 == 0;
+        if (wpr == 1) __syncwarp();
         for (int j0 = 0; j0 < k; j0 += 32) {
             if (j0) dst = j0 + lane < k ? ld_i32(pair_row + t * k + j0 + lane) : -1;
             const int n = min(32, k - j0);
             if (part == 0 && lane < n && (unsigned)dst < (unsigned)N)
                 scale[dst] = bad ? CUDART_NAN_F : s;
-            for (int c = c0; c - lane * 8 < K; c += span) {  // whole warps: the rows are shuffled
-                uint2 u = make_uint2(0, 0);
-                if (c < K && !bad) {
-                    Vec8<TI> in;
-                    float v[8];
-                    ld_shared_vec8(row + c * (int)sizeof(TI), in);
-                    in.get(v);
-                    u = codes_of(v, s, inv);
+            auto codes_at = [&](int c) {
+                Vec8<TI> in;
+                float v[8];
+                ld_shared_vec8(row + c * (int)sizeof(TI), in);
+                in.get(v);
+                const uint2 u = codes_of(v, s, inv);
+                return bad ? make_uint2(0, 0) : u;
+            };
+            // whole warps: the destinations are shuffled
+            const int step = wide ? 16 : 8;
+            for (int w0 = part * 32 * step; w0 < K; w0 += wpr * 32 * step) {
+                const int c = w0 + lane * step;
+                uint4 u = make_uint4(0, 0, 0, 0);
+                if (c < K) {
+                    const uint2 a = codes_at(c);
+                    u.x = a.x, u.y = a.y;
+                    if (wide) {
+                        const uint2 b = codes_at(c + 8);
+                        u.z = b.x, u.w = b.y;
+                    }
                 }
-#pragma unroll 4
+#pragma unroll 8
                 for (int j = 0; j < n; j++) {
                     const int r = __shfl_sync(~0u, dst, j);
-                    if ((unsigned)r < (unsigned)N && c < K)
-                        *reinterpret_cast<uint2 *>(codes + (int64_t)r * ld + c) = u;
+                    if ((unsigned)r >= (unsigned)N || c >= K) continue;
+                    int8_t *out = codes + (int64_t)r * ld + c;
+                    if (wide)
+                        *reinterpret_cast<uint4 *>(out) = u;
+                    else
+                        *reinterpret_cast<uint2 *>(out) = make_uint2(u.x, u.y);
                 }
             }
         }
@@ -510,6 +538,34 @@ static bool is_row_dtype(int dt) {
     return dt == QGMOE_DT_F32 || dt == QGMOE_DT_F16 || dt == QGMOE_DT_BF16;
 }
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// CTAs that a sort's cluster may have on the current device: more than eight
+// are not portable and need room for all in one GPC.
+static int sort_max_ctas() {
+    static int cache[64] = {0};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 8;
+    if (cache[dev]) return cache[dev];
+    const int smem = (int)sizeof(int) * (SORT_MAX_WARPS + 2) * QG_MAX_EXPERTS;
+    int n = 0;
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = at.val.clusterDim.y = 1;
+    at.val.clusterDim.z = SORT_MAX_CTAS;
+    cfg.gridDim = dim3(1, 1, SORT_MAX_CTAS);
+    cfg.blockDim = dim3(SORT_MAX_WARPS * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    if (cudaFuncSetAttribute(k_sort_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) !=
+            cudaSuccess ||
+        cudaFuncSetAttribute(k_sort_tokens, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) !=
+            cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k_sort_tokens, &cfg) != cudaSuccess)
+        n = 0;
+    return cache[dev] = n > 0 ? SORT_MAX_CTAS : 8;
+}
 
 // Calls f with a null pointer of the dtype's C++ type.
 template <typename F> static int with_dtype(int dt, F f) {
@@ -628,19 +684,19 @@ int qgmoe_sort_tokens(const int32_t *sel_idx, int32_t T, int32_t k, int32_t E, i
     if (!offsets || (T > 0 && (!sel_idx || !pair_row)))
         return set_error(QGMOE_ERR_INVALID_ARG, "sort_tokens: null pointer argument");
     const int N = T * k;
-    // A warp per 128 pairs, up to eight CTAs of 32 warps; the counters of 32
-    // warps over 1024 experts are 128 KB.
+    // A warp per 128 pairs, spread over as many CTAs as there are: the steps
+    // are bound by their instructions (4096 pairs take 7.1 us in one CTA of 32
+    // warps, 3.4 in eight of four).  The counters of 32 warps over
+    // 1024 experts are 128 KB.
+    const int most = sort_max_ctas();
     int64_t warps = ((int64_t)N + SORT_STEPS * 32 - 1) / (SORT_STEPS * 32);
     warps = warps < 1 ? 1 : warps;
     int C = 1;
-    while (C < SORT_MAX_CTAS && warps > C * SORT_MAX_WARPS) C *= 2;
-    int nw = (int)((warps + C - 1) / C);
+    while (C < most && warps > C * 4) C *= 2;
+    int nw = warps > (int64_t)C * SORT_MAX_WARPS ? SORT_MAX_WARPS : (int)((warps + C - 1) / C);
     if (nw < (E + 31) / 32) nw = (E + 31) / 32;  // a thread per expert for the scans
     if (nw > SORT_MAX_WARPS) nw = SORT_MAX_WARPS;
     const size_t smem = sizeof(int) * (size_t)(nw + 2) * E;
-    if (smem > 48 * 1024)
-        QG_CUDA(cudaFuncSetAttribute(k_sort_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     (int)smem));
     QG_CUDA(launch_pdl(k_sort_tokens, dim3(1, 1, C), dim3(nw * 32), smem,
                        static_cast<cudaStream_t>(stream), C, sel_idx, N, E, offsets, pair_row,
                        row_pair));
