@@ -47,7 +47,7 @@ def _quantize(x, order, s):
             raise ValueError(f"x: {T} rows, the order has {order.n_tokens} tokens")
         R, k, pair_row = order.n_rows, order.top_k, order.pair_row.data_ptr()
     dt, ld = _row_dtype(x, "x"), _pitch(K)
-    codes = x.new_empty((R, ld), dtype=_rows._torch.int8)
+    codes = x.new_empty(R, ld, dtype=_rows._torch.int8)
     scale = x.new_empty(R, dtype=_rows._torch.float32)
     _call("qgq8_quantize_rows", x.data_ptr(), dt, T, k, K, pair_row, codes.data_ptr(), ld,
           scale.data_ptr(), s)
@@ -151,17 +151,17 @@ class Int8Linear:
             R, k, pair_row, offsets = order.n_rows, order.top_k, order.pair_row.data_ptr(), \
                 order.offsets
         off = self._offsets(offsets, x.device)
-        y = _result(y, "y", x, (R, self.out_features), dtype)
+        y, ydt = _result(y, "y", x, R, self.out_features, dtype)
         ld = _pitch(K)
         if off is None and pair_row is None and R <= self._direct_rows:
             _call("qgq8_forward_device", self.h, x.data_ptr(), dt, T, 1, None, None, None, ld, None,
-                  y.data_ptr(), _row_dtype(y, "y"), s)
+                  y.data_ptr(), ydt, s)
             return y
         # codes [R, pitch], then their scales: one allocation
         work = x.new_empty(R * (ld + 4), dtype=_rows._torch.int8)
         at = work.data_ptr()
         _call("qgq8_forward_device", self.h, x.data_ptr(), dt, T, k, pair_row, off, at, ld,
-              at + R * ld, y.data_ptr(), _row_dtype(y, "y"), s)
+              at + R * ld, y.data_ptr(), ydt, s)
         return y
 
     def matmul_device(self, codes, scale, y=None, offsets=None, dtype=None, stream=None):
@@ -183,9 +183,9 @@ class Int8Linear:
         _need(scale, "scale", codes.device, (R,), _rows._torch.float32)
         ld = codes.stride(0) if R > 1 else _pitch(K)
         off = self._offsets(offsets, codes.device)
-        y = _result(y, "y", scale, (R, self.out_features), dtype)
+        y, ydt = _result(y, "y", scale, R, self.out_features, dtype)
         _call("qgq8_matmul_device", self.h, codes.data_ptr(), ld, scale.data_ptr(), R, off,
-              y.data_ptr(), _row_dtype(y, "y"), s)
+              y.data_ptr(), ydt, s)
         return y
 
     def sync(self, stream=None):

@@ -182,12 +182,18 @@ def _rows_of(t, what: str, order: TokenOrder, n: int):
     return dt, shape[1]
 
 
-def _result(out, what: str, like, shape, dtype):
-    """`out` checked, or a new tensor (call on the stream that fills it)."""
+def _result(out, what: str, like, n: int, h: int, dtype):
+    """(tensor, row dtype) of an [n, h] result: `out` checked, or a new tensor
+    (call on the stream that fills it; new_empty(n, h) costs 0.4 us less than
+    with a tuple)."""
     if out is None:
-        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
-    _need(out, what, like.device, shape, dtype)
-    return out
+        if dtype is None or dtype == like.dtype:
+            out = like.new_empty(n, h)
+        else:
+            out = like.new_empty(n, h, dtype=dtype)
+    else:
+        _need(out, what, like.device, (n, h), dtype)
+    return out, _row_dtype(out, what)
 
 
 def gather_rows(x, order: TokenOrder, out=None, dtype=None, stream=None):
@@ -197,9 +203,9 @@ def gather_rows(x, order: TokenOrder, out=None, dtype=None, stream=None):
 
 def _gather(x, order, out, dtype, s):
     dt, H = _rows_of(x, "x", order, order.n_tokens)
-    out = _result(out, "out", x, (order.n_rows, H), dtype)
+    out, odt = _result(out, "out", x, order.n_rows, H, dtype)
     _call("qgmoe_gather_rows", x.data_ptr(), dt, order.n_tokens, order.top_k, H,
-          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+          order.pair_row.data_ptr(), out.data_ptr(), odt, s)
     return out
 
 
@@ -210,9 +216,9 @@ def gather_rows_backward(grad_rows, order: TokenOrder, out=None, dtype=None, str
 
 def _gather_backward(grad_rows, order, out, dtype, s):
     dt, H = _rows_of(grad_rows, "grad_rows", order, order.n_rows)
-    out = _result(out, "out", grad_rows, (order.n_tokens, H), dtype)
+    out, odt = _result(out, "out", grad_rows, order.n_tokens, H, dtype)
     _call("qgmoe_gather_rows_backward", grad_rows.data_ptr(), dt, order.n_tokens, order.top_k, H,
-          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+          order.pair_row.data_ptr(), out.data_ptr(), odt, s)
     return out
 
 
@@ -226,9 +232,9 @@ def _combine(rows, weights, order, out, dtype, s):
     T, k = order.n_tokens, order.top_k
     dt, H = _rows_of(rows, "rows", order, order.n_rows)
     _need(weights, "weights", order.device, (T, k), _torch.float32)
-    out = _result(out, "out", rows, (T, H), dtype)
+    out, odt = _result(out, "out", rows, T, H, dtype)
     _call("qgmoe_combine_rows", rows.data_ptr(), dt, weights.data_ptr(), T, k, H,
-          order.pair_row.data_ptr(), out.data_ptr(), _row_dtype(out, "out"), s)
+          order.pair_row.data_ptr(), out.data_ptr(), odt, s)
     return out
 
 
@@ -247,8 +253,8 @@ def _combine_backward(grad_out, rows, weights, order, grad_rows, grad_weights, s
     if H != Hr:
         raise ValueError(f"grad_out: rows of {H}, expected {Hr}")
     _need(weights, "weights", order.device, (T, k), _torch.float32)
-    grad_rows = _result(grad_rows, "grad_rows", rows, (order.n_rows, H), rows.dtype)
-    grad_weights = _result(grad_weights, "grad_weights", weights, (T, k), _torch.float32)
+    grad_rows, _ = _result(grad_rows, "grad_rows", rows, order.n_rows, H, rows.dtype)
+    grad_weights, _ = _result(grad_weights, "grad_weights", weights, T, k, _torch.float32)
     _call("qgmoe_combine_rows_backward", grad_out.data_ptr(), gd, rows.data_ptr(), rd,
           weights.data_ptr(), T, k, H, order.pair_row.data_ptr(), grad_rows.data_ptr(),
           grad_weights.data_ptr(), s)
