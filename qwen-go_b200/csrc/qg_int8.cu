@@ -14,8 +14,8 @@
 // operands are tiled TMA loads of 128-byte rows (128B swizzle), accumulators
 // are int32 in TMEM, drained by eight epilogue warps while the next tile
 // accumulates.  Three kernels:
-//   k_i8_few   up to 16 rows of a dense product, straight from x: every CTA
-//              quantises the rows for its own blocks while its weights load,
+//   k_i8_few   few rows of a dense product, straight from x: every CTA
+//              quantises 16 rows for its own blocks while its weights load,
 //              and a cluster splits the sum, so that one launch has a single
 //              token's product spread over the whole device;
 //   k_i8       one CTA per tile of 128 channels x up to 16 or 64 rows, for few
@@ -1051,8 +1051,8 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 }
 
 // ---- few rows, straight from x -------------------------------------------------------------
-// y of up to 16 rows.  A cluster of `split` CTAs shares a tile of 128 channels,
-// each the blocks of its share of the sum.  Warps 0-7 quantise the rows (whole
+// A cluster of `split` CTAs shares 16 rows of a tile of 128 channels, each the
+// blocks of its share of the sum.  Warps 0-7 quantise the rows (whole
 // rows for the maximum, this CTA's blocks of them into swizzled shared memory)
 // while the weights are on their way; warps 0-3 are the epilogue after that:
 // the partial sums of lane quarter q go to the CTA q * split / 4 of the
@@ -1061,6 +1061,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 // launches, the product on 32 of 148 SMs.  What is left is latency: launch,
 // cluster start, one read of x, one exchange.
 constexpr int I8F_ROWS = 16;
+constexpr int I8F_MOST = 128;  // rows of a product that may run here
 constexpr int I8F_WARPS = 8;
 constexpr int I8F_LOAD_WARP = 8, I8F_MMA_WARP = 9;
 constexpr int I8F_THREADS = 10 * 32;
@@ -1084,11 +1085,12 @@ static int i8f_smem(int blocks) {
 // template on the type and the alignment, not a branch per load: the loads of
 // several vectors are in flight together.
 template <typename TI, bool VEC>
-__device__ __forceinline__ void i8f_quantize(const I8FewArgs &f, int kb0, int nb, uint32_t codes,
-                                             uint32_t (*s_max)[I8F_WARPS], float *s_scale) {
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, R = f.a.R;
+__device__ __forceinline__ void i8f_quantize(const I8FewArgs &f, int r0, int R, int kb0, int nb,
+                                             uint32_t codes, uint32_t (*s_max)[I8F_WARPS],
+                                             float *s_scale) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     auto load = [&](int r, int c, float (&v)[8]) {
-        const TI *p = static_cast<const TI *>(f.x) + (int64_t)r * f.K + c;
+        const TI *p = static_cast<const TI *>(f.x) + (int64_t)(r0 + r) * f.K + c;
         if constexpr (VEC) {
             Vec8<TI> in;
             in.load(p);
@@ -1191,6 +1193,7 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
     const int split = f.split, rank = split > 1 ? (int)cluster_ctarank() : 0;
     const int ct = blockIdx.x / split;  // channel tile
     const int kb0 = rank * f.blocks, nb = max(0, min(f.blocks, a.KB - kb0));
+    const int r0 = blockIdx.y * I8F_ROWS, R = min(I8F_ROWS, a.R - r0);
 
     uint8_t *base = reinterpret_cast<uint8_t *>(
         (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1233,18 +1236,18 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
         // ============ rows -> codes ===============================================
         if (f.x_vec) {
             if (f.x_dtype == QGMOE_DT_F32)
-                i8f_quantize<float, true>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<float, true>(f, r0, R, kb0, nb, codes, s_max, s_scale);
             else if (f.x_dtype == QGMOE_DT_F16)
-                i8f_quantize<__half, true>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<__half, true>(f, r0, R, kb0, nb, codes, s_max, s_scale);
             else
-                i8f_quantize<__nv_bfloat16, true>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<__nv_bfloat16, true>(f, r0, R, kb0, nb, codes, s_max, s_scale);
         } else {
             if (f.x_dtype == QGMOE_DT_F32)
-                i8f_quantize<float, false>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<float, false>(f, r0, R, kb0, nb, codes, s_max, s_scale);
             else if (f.x_dtype == QGMOE_DT_F16)
-                i8f_quantize<__half, false>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<__half, false>(f, r0, R, kb0, nb, codes, s_max, s_scale);
             else
-                i8f_quantize<__nv_bfloat16, false>(f, kb0, nb, codes, s_max, s_scale);
+                i8f_quantize<__nv_bfloat16, false>(f, r0, R, kb0, nb, codes, s_max, s_scale);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -1252,7 +1255,7 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
         // ============ epilogue =====================================================
         if (warp < 4) {
             const int q = warp, owner = q * split / 4;
-            const int rblocks = (a.R + 7) / 8;
+            const int rblocks = (R + 7) / 8;
             I8Epilogue<TO, SWIGLU, 1> epi(a, q, lane, smem_u32(s_scale));
             epi.channels(a.ws + ((size_t)ct * I8_M) + q * 32);
             int v[2][16];
@@ -1317,7 +1320,7 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
                     }
                 }
                 if (ok)
-                    epi.template run<false>(v, smem_u32(s_scale), 0, a.R,
+                    epi.template run<false>(v, smem_u32(s_scale), r0, R,
                                             (ct * 4 + q) * I8Epilogue<TO, SWIGLU, 1>::CH);
             }
         }
@@ -1630,22 +1633,33 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
                       : launch_i8<I8P_NT>(h, tx, a, ydt, units, s);
 }
 
-// Rows up to which a dense product runs on k_i8_few: 16, if its CTAs, each of
-// which quantises the rows, are resident at once and a CTA's share of the row
-// codes fits next to its weights.  2048 -> 4096, this kernel and the two others
-// on the device: 1 row 5.7 and 7.2 us, 8 rows 7.3 and 7.3, 16 rows 8.7 and 7.3;
-// but one launch instead of two and no workspace save 4.5 us of host time,
-// which is what a call of this size waits for.
-static int i8_few_split(const qgq8 *h) {
-    int split = 1;
-    while (split < I8F_SPLIT && h->live * split * 2 <= num_sms(h->device) && h->KB >= split * 4)
-        split *= 2;
-    return split;
+// CTAs of a cluster for R rows on k_i8_few: as many as keep all clusters on
+// the device at once (of four, 32 surely find room: a GPC's SMs are no multiple
+// of four; a product that did not fit took twice as long), with four blocks of
+// the sum left to each.
+static int i8_few_split(const qgq8 *h, int R) {
+    const int clusters = h->live * ((R + I8F_ROWS - 1) / I8F_ROWS), sms = num_sms(h->device);
+    if (h->KB >= 8 && clusters * 4 <= sms - 20) return 4;
+    return h->KB >= 4 && clusters * 2 <= sms ? 2 : 1;
 }
+// Rows up to which a dense product runs on k_i8_few: its CTAs have to be
+// resident at once, each with its share of the row codes in shared memory, and
+// beyond 16 rows with all its weights in flight.  2048 -> 4096, this kernel and
+// the two others on the device: 1 row 5.8 and 7.2 us, 8 rows 7.2 and 7.3, 16
+// rows 8.6 and 7.3, 32 rows 10.3 and 7.4 (48, beyond the rule, 12.1 and 7.8);
+// 1000 -> 1500: 77 rows 7.3 and 7.1.  Where the device takes longer, one launch
+// instead of two and no workspace still save 4 us of host time, which is what a
+// call of this size waits for.
 static int i8_few_rows(const qgq8 *h) {
-    if (h->G != 1 || h->live > num_sms(h->device)) return 0;
-    const int split = i8_few_split(h);
-    return (h->KB + split - 1) / split <= I8F_BLOCKS ? I8F_ROWS : 0;
+    if (h->G != 1) return 0;
+    int R = 0;
+    for (int r = I8F_ROWS; r <= I8F_MOST && h->live * (r / I8F_ROWS) <= num_sms(h->device);
+         r += I8F_ROWS) {
+        const int split = i8_few_split(h, r), blocks = (h->KB + split - 1) / split;
+        if (blocks > (r == I8F_ROWS ? I8F_BLOCKS : I8F_STAGES)) break;
+        R = r;
+    }
+    return R;
 }
 
 template <typename TO, bool SWIGLU>
@@ -1664,7 +1678,8 @@ static int launch_i8_few_t(const qgq8 *h, const I8FewArgs &f, cudaStream_t s) {
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = f.split;
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-    cfg.gridDim = dim3((unsigned)(h->live * f.split));
+    cfg.gridDim = dim3((unsigned)(h->live * f.split),
+                       (unsigned)((f.a.R + I8F_ROWS - 1) / I8F_ROWS));
     cfg.blockDim = dim3(I8F_THREADS);
     cfg.dynamicSmemBytes = i8f_smem(f.blocks);
     cfg.stream = s;
@@ -1689,7 +1704,7 @@ static int i8_few(const qgq8 *h, const void *x, int xdt, int R, void *y, int ydt
     f.x_dtype = xdt;
     f.x_vec = h->I % 8 == 0 && !(reinterpret_cast<uintptr_t>(x) & 15);
     f.K = h->I;
-    f.split = i8_few_split(h);
+    f.split = i8_few_split(h, R);
     f.blocks = (h->KB + f.split - 1) / f.split;
     if (h->swiglu)
         return ydt == QGMOE_DT_F32   ? launch_i8_few_t<float, true>(h, f, s)

@@ -138,18 +138,19 @@ def test_linear(T, K, N, xt, yt):
 @pytest.mark.parametrize("xt", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("swiglu", [False, True])
 def test_few_rows_directly(K, N, xt, swiglu):
-    """Up to 16 rows in one kernel: bit for bit what the quantiser and the
-    product give, rows that are not finite included; one row more than that
-    takes the two kernels."""
+    """Few rows in one kernel: bit for bit what the quantiser and the product
+    give, rows that are not finite included; one row more than it takes goes
+    to the two kernels."""
     t = torch_()
     q, ws = weights((2 * N if swiglu else N, K), N)
     lin = qgmoe.Int8Linear(q, ws, swiglu=swiglu)
-    assert qgmoe.lib().qgq8_direct_rows(lin.h) in (0, 16)
-    for T in (1, 3, 8, 9, 16, 17):
+    most = qgmoe.lib().qgq8_direct_rows(lin.h)
+    assert most % 16 == 0 and 0 <= most <= 128
+    for T in sorted({1, 3, 8, 9, 16, 17, 40, max(1, most), most + 1}):
         x = rand((T, K), dtypes()[xt], K + T)
-        if T == 9:
+        if T >= 9:
             x[4, K // 2] = float("inf")
-            x[8, K - 1] = float("nan")
+            x[T - 1, K - 1] = float("nan")
             x[2] = 0
         codes, scale = qgmoe.quantize_rows(x)
         for yt in dtypes().values():
@@ -157,8 +158,8 @@ def test_few_rows_directly(K, N, xt, swiglu):
             want = lin.matmul_device(codes, scale, dtype=yt)
             assert t.equal(t.isnan(y), t.isnan(want))
             assert t.equal(t.nan_to_num(y), t.nan_to_num(want))
-        if T == 9:
-            assert t.isnan(y[[4, 8]]).all() and not t.isnan(y[:4]).any()
+        if T >= 9:
+            assert t.isnan(y[[4, T - 1]]).all() and not t.isnan(y[:4]).any()
     off = rand((3 * K + 1,), dtypes()[xt], 1)[1:].view(3, K)   # not 16-byte aligned
     codes, scale = qgmoe.quantize_rows(off)
     assert t.equal(lin.forward_device(off, dtype=t.float32), lin.matmul_device(codes, scale))
