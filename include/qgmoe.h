@@ -384,8 +384,8 @@ int qgql_quantize_device(int32_t bits, int32_t out_features, int32_t in_features
  * anything between calls or uses a workspace: calls on different streams
  * overlap freely and every call can be captured into a CUDA graph.
  * Rows are QGMOE_DT_F32, _F16 or _BF16, contiguous, of 1..QGMOE_MAX_ROW
- * elements (16-byte aligned rows, multiples of 8 elements, are read and
- * written 16 bytes at a time); arithmetic is float32, rounded once to the
+ * elements, aligned to their type (16-byte aligned rows, multiples of 8
+ * elements, are read and written 16 bytes at a time); arithmetic is float32, rounded once to the
  * output's type.  T * k is at most QGMOE_MAX_PAIRS; T = 0 is allowed.
  * Outputs may not overlap inputs. */
 #define QGMOE_MAX_PAIRS (1 << 30)
@@ -443,7 +443,8 @@ int qgmoe_combine_rows_backward(const void *grad_out, int32_t out_dtype, const v
  * [T, K] with row pitch ld, scale [T].  With pair_row [T, k]
  * (qgmoe_sort_tokens): row t goes to the rows pair_row[t, 0..k) of codes
  * [T * k, K] and scale [T * k] -- gathered and quantised in one pass; other
- * rows are left as they are.  ld is a multiple of 16, codes 16-byte aligned;
+ * rows are left as they are (a product without offsets takes them as they
+ * are).  ld is a multiple of 16, codes 16-byte aligned;
  * bytes of a row between K and ld are undefined.  The same call makes the
  * weights' codes from float rows.  DEVICE pointers on the current device;
  * stream and capture rules as for qgmoe_gather_rows. */
@@ -469,9 +470,9 @@ int qgq8_destroy(qgq8_t *h);
  * group are left as they are.  A group whose range is not inside [0, R] is
  * skipped and raises the error flag (qgq8_sync).  NULL with one group: all
  * R rows.  DEVICE pointers; enqueued on `stream` (NULL = the handle's
- * stream, cudaStreamLegacy = the legacy default stream).  Nothing is kept between calls: calls of one handle may overlap on
- * the GPU and be captured into graphs.  The caller's current device is left
- * as it was. */
+ * stream, cudaStreamLegacy = the legacy default stream).  Nothing is kept
+ * between calls: calls of one handle may overlap on the GPU and be captured
+ * into graphs.  The caller's current device is left as it was. */
 int qgq8_matmul_device(qgq8_t *h, const int8_t *codes, int64_t ld, const float *scale, int32_t R,
                        const int32_t *offsets, void *y, int32_t y_dtype, void *stream);
 /* qgq8_quantize_rows into the caller's codes / scale (R = T * k rows), then

@@ -12,7 +12,7 @@
 //   D[channels, rows] = Q[channels, I] * C[rows, I]^T   (tcgen05.mma kind::i8)
 // so that a batch of few rows costs a narrow N instead of an empty M.  Both
 // operands are tiled TMA loads of 128-byte rows (128B swizzle), accumulators
-// are int32 in TMEM, drained by eight epilogue warps while the next tile
+// are int32 in TMEM, drained by 4, 8 or 16 epilogue warps while the next tile
 // accumulates.  Three kernels:
 //   k_i8_few   few rows of a dense product, straight from x: every CTA
 //              quantises 16 rows for its own blocks while its weights load,
@@ -21,11 +21,14 @@
 //   k_i8       one CTA per tile of 128 channels x up to 16 or 64 rows, for few
 //              rows per group: a stream of weights;
 //   k_i8_pair  a CTA pair (cta_group::2) per tile of 256 channels x up to 512
-//              rows, for prompts.  A tile's operands come from L2, and an
-//              SM gets about 43 bytes a clock from it (128 x 256 tiles of one
-//              CTA need 96 at the MMA's full rate and ran at 45 % of it): the
-//              pair shares its row codes, and 512 rows a tile halve what the
-//              weights cost, 47 bytes a clock in all.
+//              rows, for prompts.  A tile's operands come from L2: the pair
+//              shares its row codes, and 512 rows a tile halve what the
+//              weights cost.  Main loop alone, 256 rows a tile 2.96 POPS, 512
+//              rows 3.57 (256 channels x 512 rows are all of the pair's TMEM).
+// Measured (device time of the product): 4096 rows, 2048 -> 4096, bf16: 26.9 us,
+// 2.55 POPS (tensor pipe busy half of the time); the rest is the start, 1.7 rounds
+// of tiles on 74 pairs and the last tile's conversion.  128 experts of
+// 2048 -> 2 x 768, SwiGLU, 512 rows: 67.5 us, 6.0 TB/s of weights.
 // Persistent, one CTA per SM, units (group, row tile, channel tile) with the
 // channel tile fastest, so that concurrent CTAs share a row tile and, over the
 // following units, the group's weights in L2.  Every wait is bounded; a wait
@@ -1382,8 +1385,9 @@ k_i8_few(const __grid_constant__ CUtensorMap tmap_w, const I8FewArgs f) {
 
 // ---- weight layout -------------------------------------------------------------
 // Tiles of 128 rows x 128 codes, each 16 KB in one piece, a row tile's blocks
-// after one another: read as a box of a plain [rows, in] matrix a tile is 128
-// pieces of 128 bytes, of which HBM gave 3.9 TB/s.  Zeros past a group's rows
+// after one another: a plain [rows, in] matrix would give a tile as 128 pieces
+// of 128 bytes each in a row of its own (128 experts of 2048 -> 2 x 768 and 512
+// rows took 74 us that way, 73 this way).  Zeros past a group's rows
 // and past I; scales [groups * RT * 128] alike.  With SwiGLU, tile rt holds
 // output columns [rt*64, rt*64 + 64): of each 32 tile rows the first 16 are
 // gate rows of 16 columns, the others the up rows of the same columns.
@@ -1421,6 +1425,7 @@ __global__ void k_i8_layout(const int8_t *q, const float *scale, int O, int I, i
 
 // ---- host side -------------------------------------------------------------------
 int check_pairs(int32_t T, int32_t k, const char *what);
+bool on_element(const void *p, int dt);
 int check_quantize_rows(const void *x, int dt, int T, int k, int K, const int32_t *pair_row,
                         const void *codes, int64_t ld, const void *scale);
 int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32_t *pair_row,
@@ -1594,6 +1599,7 @@ static int i8_check_product(const qgq8 *h, const int8_t *codes, int64_t ld, cons
     if (!codes || !scale || !y) return set_error(QGMOE_ERR_INVALID_ARG, "null pointer argument");
     if (reinterpret_cast<uintptr_t>(codes) & 15)
         return set_error(QGMOE_ERR_INVALID_ARG, "codes must be 16-byte aligned");
+    if (!on_element(y, ydt)) return set_error(QGMOE_ERR_INVALID_ARG, "y is not aligned to its type");
     return QGMOE_OK;
 }
 
@@ -1728,8 +1734,10 @@ static void i8_free_work(qgq8 *h) {
 static int i8_alloc(void **p, size_t bytes) {
     *p = nullptr;
     cudaError_t e = cudaMalloc(p, bytes);
-    if (e != cudaSuccess)
+    if (e != cudaSuccess) {
+        cudaGetLastError();  // reported here; the next launch anyone checks did not fail
         return set_error(QGMOE_ERR_CUDA, "cudaMalloc(%zu): %s", bytes, cudaGetErrorString(e));
+    }
     return QGMOE_OK;
 }
 

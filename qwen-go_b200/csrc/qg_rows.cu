@@ -26,10 +26,11 @@ namespace qg {
 // contiguous range of pairs and takes it 32 at a time: lanes with the same
 // expert find each other (a ballot per bit of the id; match.any is several
 // times slower), rank themselves in lane order on top of the warp's count of
-// that expert so far, and the first adds their number to the count.  The counts of the CTA's warps, then of the cluster's CTAs
-// (distributed shared memory), then of the experts are summed in order; a
-// pair's row is the three prefixes and its rank.  The order within an expert
-// is the pairs' own by construction; no atomics.
+// that expert so far, and the first adds their number to the count.  The counts
+// of the CTA's warps, then of the cluster's CTAs (distributed shared memory),
+// then of the experts are summed in order; a pair's row is the three prefixes
+// and its rank.  The order within an expert is the pairs' own by construction;
+// no atomics.
 // Every id is handled once: 32768 pairs over 128 experts take 5 us, where one
 // CTA per expert, each counting all pairs, took 12.
 constexpr int SORT_MAX_WARPS = 32;
@@ -538,6 +539,14 @@ static bool is_row_dtype(int dt) {
     return dt == QGMOE_DT_F32 || dt == QGMOE_DT_F16 || dt == QGMOE_DT_BF16;
 }
 static bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+// Rows start on an element of their type, wherever in a buffer that is.
+bool on_element(const void *p, int dt) {
+    return (reinterpret_cast<uintptr_t>(p) & (dt == QGMOE_DT_F32 ? 3 : 1)) == 0;
+}
+static int check_elements(const void *a, int dt_a, const void *b, int dt_b, const char *what) {
+    if (on_element(a, dt_a) && on_element(b, dt_b)) return QGMOE_OK;
+    return set_error(QGMOE_ERR_INVALID_ARG, "%s: rows are not aligned to their type", what);
+}
 
 // CTAs that a sort's cluster may have on the current device: more than eight
 // are not portable and need room for all in one GPC.
@@ -664,6 +673,7 @@ int check_quantize_rows(const void *x, int dt, int T, int k, int K, const int32_
     if (T == 0) return QGMOE_OK;
     if (!x || !codes || !scale)
         return set_error(QGMOE_ERR_INVALID_ARG, "quantize_rows: null pointer argument");
+    if ((rc = check_elements(x, dt, nullptr, dt, "quantize_rows"))) return rc;
     if (!aligned16(codes))
         return set_error(QGMOE_ERR_INVALID_ARG, "quantize_rows: codes must be 16-byte aligned");
     return QGMOE_OK;
@@ -710,6 +720,7 @@ int qgmoe_gather_rows(const void *x, int32_t x_dtype, int32_t T, int32_t k, int3
     if (T == 0) return QGMOE_OK;
     if (!x || !pair_row || !rows)
         return set_error(QGMOE_ERR_INVALID_ARG, "gather_rows: null pointer argument");
+    if ((rc = check_elements(x, x_dtype, rows, rows_dtype, "gather_rows"))) return rc;
     const bool vec = H % 8 == 0 && aligned16(x) && aligned16(rows);
     dim3 grid;
     int th;
@@ -735,6 +746,8 @@ int qgmoe_gather_rows_backward(const void *grad_rows, int32_t rows_dtype, int32_
     if (T == 0) return QGMOE_OK;
     if (!grad_rows || !pair_row || !grad_x)
         return set_error(QGMOE_ERR_INVALID_ARG, "gather_rows_backward: null pointer argument");
+    if ((rc = check_elements(grad_rows, rows_dtype, grad_x, x_dtype, "gather_rows_backward")))
+        return rc;
     return launch_combine_rows(grad_rows, rows_dtype, nullptr, T, k, H, pair_row, grad_x, x_dtype,
                                static_cast<cudaStream_t>(stream));
 }
@@ -747,6 +760,7 @@ int qgmoe_combine_rows(const void *rows, int32_t rows_dtype, const float *w, int
     if (T == 0) return QGMOE_OK;
     if (!rows || !w || !pair_row || !out)
         return set_error(QGMOE_ERR_INVALID_ARG, "combine_rows: null pointer argument");
+    if ((rc = check_elements(rows, rows_dtype, out, out_dtype, "combine_rows"))) return rc;
     return launch_combine_rows(rows, rows_dtype, w, T, k, H, pair_row, out, out_dtype,
                                static_cast<cudaStream_t>(stream));
 }
@@ -760,6 +774,9 @@ int qgmoe_combine_rows_backward(const void *grad_out, int32_t out_dtype, const v
     if (T == 0 || (!grad_rows && !grad_w)) return QGMOE_OK;
     if (!grad_out || !pair_row || (grad_w && !rows) || (grad_rows && !w))
         return set_error(QGMOE_ERR_INVALID_ARG, "combine_rows_backward: null pointer argument");
+    if ((rc = check_elements(rows, rows_dtype, grad_rows, rows_dtype, "combine_rows_backward")) ||
+        (rc = check_elements(grad_out, out_dtype, nullptr, out_dtype, "combine_rows_backward")))
+        return rc;
     const bool vec = H % 8 == 0 && aligned16(grad_out) && (!rows || aligned16(rows)) &&
                      (!grad_rows || aligned16(grad_rows));
     const int N = T * k;

@@ -489,3 +489,16 @@ def test_device_refusals():
         assert e.value.status == qgmoe.ERR_INVALID_ARG
     with pytest.raises(qgmoe.QgmoeError):
         lin.forward(np.zeros((2, 16), np.float32))
+
+
+def test_weights_that_do_not_fit_leave_nothing_behind():
+    # 272 GB: refused by the allocation, before the (here bad) weights are read.  The error is the
+    # call's own and is not found again by the next launch that anyone checks.
+    t = torch_()
+    h = C.c_void_p()
+    assert qgmoe.lib().qgq8_create(1024, 32512, 8192, C.c_void_p(256), C.c_void_p(256), 0, 0, 0,
+                                   C.byref(h)) == qgmoe.ERR_CUDA
+    assert not h.value and "cudaMalloc" in qgmoe.last_error()
+    assert float(t.ones(4, device="cuda").sum()) == 4
+    lin = qgmoe.Int8Linear(t.ones((8, 16), dtype=t.int8, device="cuda"), t.ones(8, device="cuda"))
+    assert lin.forward_device(t.ones((2, 16), device="cuda")).shape == (2, 8)

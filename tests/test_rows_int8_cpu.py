@@ -47,6 +47,22 @@ def test_combine_refuses_null_weights():
     assert L().qgmoe_combine_rows_backward(ONE, 0, ONE, 0, ONE, 4, 2, 8, ONE, None, None, None) == 0
 
 
+@pytest.mark.parametrize("dt,at", [(0, 258), (0, 257), (qgmoe.DT_F16, 257), (qgmoe.DT_BF16, 257)])
+def test_rows_off_their_elements_are_refused(dt, at):
+    odd = C.c_void_p(at)
+    for a, b in ((odd, ONE), (ONE, odd)):
+        assert L().qgmoe_gather_rows(a, dt, 4, 2, 8, ONE, b, dt, None) == INV
+        assert "aligned" in qgmoe.last_error()
+        assert L().qgmoe_gather_rows_backward(a, dt, 4, 2, 8, ONE, b, dt, None) == INV
+        assert L().qgmoe_combine_rows(a, dt, ONE, 4, 2, 8, ONE, b, dt, None) == INV
+    for p in ((odd, ONE, ONE), (ONE, odd, ONE), (ONE, ONE, odd)):
+        assert L().qgmoe_combine_rows_backward(p[0], dt, p[1], dt, ONE, 4, 2, 8, ONE, p[2], ONE,
+                                               None) == INV
+        assert "aligned" in qgmoe.last_error()
+    assert L().qgq8_quantize_rows(odd, dt, 4, 1, 8, None, ONE, 16, ONE, None) == INV
+    assert "aligned" in qgmoe.last_error()
+
+
 def test_no_tokens_need_no_pointers():
     assert L().qgmoe_gather_rows(None, 0, 0, 2, 8, None, None, 0, None) == 0
     assert L().qgmoe_combine_rows(None, 0, None, 0, 2, 8, None, None, 0, None) == 0
