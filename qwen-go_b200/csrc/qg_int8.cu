@@ -69,7 +69,8 @@ struct I8Cfg {
     static constexpr int EPI_WARPS = NT <= 32 ? 4 : NT <= 64 ? 8 : 16;
     static constexpr int LOAD_WARP = EPI_WARPS, MMA_WARP = EPI_WARPS + 1;
     static constexpr int THREADS = (EPI_WARPS + 2) * 32;
-    static constexpr int TAB_BYTES = (I8_MAX_GROUPS + 1) * 4 + 12 + I8_UNITS * 16;
+    static constexpr int PREFIXES = NT > 64 ? 2 : 1;  // (light groups have their own)
+    static constexpr int TAB_BYTES = PREFIXES * (I8_MAX_GROUPS + 1) * 4 + 12 + I8_UNITS * 16;
     static constexpr int EPI_BYTES = EPI_WARPS * I8_SCALE_BYTES;
     static constexpr int REST = EPI_BYTES + 8 * 5 + 16 + TAB_BYTES + 1024;
     static constexpr int S = (I8_SMEM - REST) / (STAGE_BYTES + 16);  // two barriers a stage
@@ -83,6 +84,13 @@ constexpr int I8P_PART = 256;
 constexpr int I8P_NT = 2 * I8P_PART;
 constexpr int I8P_BOX = 64;
 constexpr int I8P_HALF_BYTES = I8P_PART / 2 * I8_BK;
+// Light tiles, of up to two boxes of rows, wait for their weights more than for
+// their MMAs: a stage then holds two blocks of the sum (weights at 0 and
+// A_BYTES, row codes behind them), so that twice as many weights are in
+// flight.  128 experts of 2048 -> 2 x 768: 94 rows each 73.5 us instead of 79.9,
+// 69 rows 71.1 instead of 77.7.
+constexpr int I8P_LIGHT = 2 * I8P_BOX;
+constexpr int I8P_BOX_BYTES = I8P_BOX * I8_BK;
 // Stages whose second part waits at the start and the end of a tile (below).
 constexpr int I8P_STAGGER = 2;
 static_assert(I8P_STAGGER >= 1, "the accumulators' commits rely on it");
@@ -227,9 +235,12 @@ struct I8Unit {
 };
 
 // Row tiles before each group, and their total at prefix[G] (one warp).  A
-// group whose range is not one has none and raises the flag.
+// group whose range is not one has none and raises the flag.  With LIGHT the
+// tiles of groups of up to I8P_LIGHT rows, one each, are counted apart, in
+// prefix[G + 1 ..], and come after all others.
+template <bool LIGHT>
 __device__ __forceinline__ void i8_prefix(const I8Args &a, int *prefix, int lane) {
-    int total = 0;
+    int total = 0, lights = 0;
     for (int g0 = 0; g0 < a.G; g0 += 32) {
         const int g = g0 + lane;
         int n = 0;
@@ -245,6 +256,13 @@ __device__ __forceinline__ void i8_prefix(const I8Args &a, int *prefix, int lane
                 n = a.R;
             }
         }
+        if constexpr (LIGHT) {
+            const bool light = n > 0 && n <= I8P_LIGHT;
+            const unsigned w = __ballot_sync(~0u, light);
+            if (g < a.G) prefix[a.G + 1 + g] = lights + __popc(w & ((1u << lane) - 1));
+            lights += __popc(w);
+            if (light) n = 0;
+        }
         int t = (n + a.nt - 1) / a.nt, sum = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -254,14 +272,22 @@ __device__ __forceinline__ void i8_prefix(const I8Args &a, int *prefix, int lane
         if (g < a.G) prefix[g] = total + sum - t;
         total += __shfl_sync(~0u, sum, 31);
     }
-    if (lane == 0) prefix[a.G] = total;
+    if (lane == 0) {
+        prefix[a.G] = total;
+        if (LIGHT) prefix[2 * a.G + 1] = lights;
+    }
 }
 
 // Unit u.  The row tiles of a group are as even as multiples of gran allow.
+template <bool LIGHT>
 __device__ __forceinline__ I8Unit i8_unit(const I8Args &a, const int *prefix, int u) {
     I8Unit w;
-    const int ti = u / a.CT;
+    int ti = u / a.CT;
     w.ct = u - ti * a.CT;
+    if (LIGHT && ti >= prefix[a.G]) {
+        ti -= prefix[a.G];
+        prefix += a.G + 1;
+    }
     int lo = 0, hi = a.G - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -285,27 +311,40 @@ __device__ __forceinline__ I8Unit i8_unit(const I8Args &a, const int *prefix, in
 // I8_UNITS of them are decoded together at the start (fill, all threads, then
 // a barrier): a role that looks its next unit up pays a search and two loads
 // of offsets, some 1500 cycles in which it does nothing else.
-struct I8Units {
+// With LIGHT, where both kinds of row tiles are many, the pairs of every other
+// row tile take their units from the last to the first, so that at any time
+// some of them stream the weights of light groups while others multiply: 4096
+// tokens over 128 experts as a skewed router spreads them (2048 -> 2 x 768)
+// 121 us instead of 124, 2048 tokens of 768 -> 2048 50.4 instead of 53.5.
+// Where all tiles are of one kind it costs up to 4 % (row codes are read again
+// later) and is not done.
+template <bool LIGHT> struct I8Units {
     const I8Args &a;
     const int *prefix;
     uint32_t table;  // [I8_UNITS] x 16 bytes
     int first, step, count;
     __device__ __forceinline__ I8Units(const I8Args &a, const int *prefix, int first, int step)
         : a(a), prefix(prefix),
-          table((smem_u32(prefix + a.G + 1) + 15) & ~15u), first(first), step(step) {
-        const int n = prefix[a.G] * a.CT;
+          table((smem_u32(prefix + (LIGHT ? 2 : 1) * (a.G + 1)) + 15) & ~15u), first(first),
+          step(step) {
+        const int others = prefix[a.G], lights = LIGHT ? prefix[2 * a.G + 1] : 0;
+        const int n = (others + lights) * a.CT;
         count = first < n ? (n - first + step - 1) / step : 0;
+        if (LIGHT && min(others, lights) > max(others, lights) / 3 && (first / a.CT & 1)) {
+            this->first = first + (count - 1) * step;
+            this->step = -step;
+        }
     }
     __device__ __forceinline__ void fill(int tid, int threads) const {
         for (int i = tid; i < min(count, I8_UNITS); i += threads) {
-            const I8Unit w = i8_unit(a, prefix, first + i * step);
+            const I8Unit w = i8_unit<LIGHT>(a, prefix, first + i * step);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(table + i * 16), "r"(w.g),
                          "r"(w.ct), "r"(w.row0), "r"(w.n)
                          : "memory");
         }
     }
     __device__ __forceinline__ I8Unit operator[](int i) const {
-        if (i >= I8_UNITS) return i8_unit(a, prefix, first + i * step);
+        if (i >= I8_UNITS) return i8_unit<LIGHT>(a, prefix, first + i * step);
         const uint4 v = ld_shared_v4(table + i * 16);
         return I8Unit{(int)v.x, (int)v.y, (int)v.z, (int)v.w};
     }
@@ -618,12 +657,12 @@ k_i8(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CUtenso
         tmem_relinquish();
     }
     if (a.offsets) pdl_wait();  // else what comes before the rows needs no wait
-    if (warp == 0) i8_prefix(a, prefix, lane);
+    if (warp == 0) i8_prefix<false>(a, prefix, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const I8Units units(a, prefix, blockIdx.x, gridDim.x);
+    const I8Units<false> units(a, prefix, blockIdx.x, gridDim.x);
     units.fill(tid, Cfg::THREADS);
     __syncthreads();
 
@@ -811,13 +850,13 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
     }
     if (warp == Cfg::MMA_WARP) tmem_alloc2(tmem_slot, 512);
     if (a.offsets) pdl_wait();  // else what comes before the rows needs no wait
-    if (warp == 0) i8_prefix(a, prefix, lane);
+    if (warp == 0) i8_prefix<true>(a, prefix, lane);
     tc_fence_before();
     __syncthreads();
     cluster_sync();  // the other CTA's barriers are initialised
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const I8Units units(a, prefix, blockIdx.x >> 1, gridDim.x >> 1);
+    const I8Units<true> units(a, prefix, blockIdx.x >> 1, gridDim.x >> 1);
     units.fill(tid, Cfg::THREADS);
     __syncthreads();
 
@@ -900,10 +939,43 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                 const int h0 = ((n0 + 31) & ~31) / 2, h1 = ((n1 + 31) & ~31) / 2;
                 const int b0 = (h0 + I8P_BOX - 1) / I8P_BOX, b1 = (h1 + I8P_BOX - 1) / I8P_BOX;
                 const int r0 = w.row0 + rank * h0, r1 = w.row0 + n0 + rank * h1;
-                const uint32_t bytes = 2 * (Cfg::A_BYTES + (b0 + b1) * I8P_BOX * I8_BK);
+                const uint32_t bytes = 2 * (Cfg::A_BYTES + (b0 + b1) * I8P_BOX_BYTES);
                 // the weights of the first stages do not wait for the kernel
                 // that makes the row codes
-                const int early = i == 0 && !a.offsets ? min(S, a.KB) : 0;
+                const bool ahead = i == 0 && !a.offsets;
+                if (w.n <= I8P_LIGHT) {  // two blocks a stage; its own loop: the other's is
+                                         // slower by 5 % with what the two have not in common
+                    const int early = ahead ? min(2 * S, a.KB) : 0;
+                    auto weights = [&](int stage, int kb, int blocks) {  // an elected lane
+                        if (rank == 0) mbar_arrive_expect_tx(&full[stage], blocks * bytes);
+                        for (int j = 0; j < blocks; j++)
+                            tma_load_2d_pair(base + stage * Cfg::STAGE_BYTES + j * Cfg::A_BYTES,
+                                             &tmap_w, 0, wrow + (kb + j) * I8_M, full0 + 8 * stage);
+                    };
+                    if (early) {
+                        if (elect_one())
+                            for (int kb = 0; kb < early; kb += 2)
+                                weights(kb / 2, kb, min(2, a.KB - kb));
+                        __syncwarp();
+                        pdl_wait();
+                    }
+                    for (int kb = 0; kb < a.KB; kb += 2) {
+                        if (!(ok = i8_wait(empty0 + 8 * r.s, r.phase ^ 1, abort_addr))) break;
+                        if (elect_one()) {
+                            const int blocks = min(2, a.KB - kb);
+                            if (kb >= early) weights(r.s, kb, blocks);
+                            for (int j = 0; j < blocks; j++)
+                                tma_load_2d_pair(base + r.s * Cfg::STAGE_BYTES + 2 * Cfg::A_BYTES +
+                                                     j * I8P_BOX_BYTES,
+                                                 &tmap_x, (kb + j) * I8_BK, r0, full0 + 8 * r.s);
+                        }
+                        __syncwarp();
+                        loads = min(loads + 1, S);
+                        r.next();
+                    }
+                    continue;
+                }
+                const int early = ahead ? min(S, a.KB) : 0;
                 if (early) {
                     if (elect_one())
                         for (int kb = 0; kb < early; kb++) {
@@ -925,10 +997,10 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                             tma_load_2d_pair(dst, &tmap_w, 0, wrow + kb * I8_M, bar);
                         }
                         for (int b = 0; b < b0; b++)
-                            tma_load_2d_pair(dx + b * I8P_BOX * I8_BK, &tmap_x, x,
+                            tma_load_2d_pair(dx + b * I8P_BOX_BYTES, &tmap_x, x,
                                              r0 + b * I8P_BOX, bar);
                         for (int b = 0; b < b1; b++)
-                            tma_load_2d_pair(dx + I8P_HALF_BYTES + b * I8P_BOX * I8_BK, &tmap_x, x,
+                            tma_load_2d_pair(dx + I8P_HALF_BYTES + b * I8P_BOX_BYTES, &tmap_x, x,
                                              r1 + b * I8P_BOX, bar);
                     }
                     __syncwarp();
@@ -966,6 +1038,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
             const uint64_t da = desc_k_sw128(base0);
             const uint64_t db0 = desc_k_sw128(base0 + Cfg::A_BYTES);
             const uint64_t db1 = desc_k_sw128(base0 + Cfg::A_BYTES + I8P_HALF_BYTES);
+            const uint64_t dl = desc_k_sw128(base0 + 2 * Cfg::A_BYTES);
             auto wait_acc = [&](int i) {
                 const bool got =
                     i8_wait(smem_u32(&accEmpty[i & 1]), ((i >> 1) & 1) ^ 1, abort_addr);
@@ -1001,7 +1074,24 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
                     last.next();
                 };
                 if (!(ok = wait_acc(sc))) break;
-                if (n1 == 0) {
+                if (n <= I8P_LIGHT) {
+                    for (int kb = 0; kb < a.KB; kb += 2) {
+                        if (!(ok = i8_wait(full0 + 8 * first.s, first.phase, abort_addr))) break;
+                        tc_fence_after();
+                        const uint32_t at = first.s * (Cfg::STAGE_BYTES >> 4);
+                        if (elect_one()) {
+                            umma2_i8_k128(acc0, da + at, dl + at, id0, kb != 0);
+                            if (kb + 1 < a.KB)
+                                umma2_i8_k128(acc0, da + at + (Cfg::A_BYTES >> 4),
+                                              dl + at + (I8P_BOX_BYTES >> 4), id0, 1);
+                        }
+                        __syncwarp();
+                        first.next();
+                        give_back();
+                    }
+                    if (ok) commit(&accFull[sc & 1]);
+                    sc++;
+                } else if (n1 == 0) {
                     for (int kb = 0; kb < a.KB; kb++) {
                         if (!(ok = part0(kb))) break;
                         give_back();
