@@ -19,16 +19,16 @@
 //              and a cluster splits the sum, so that one launch has a single
 //              token's product spread over the whole device;
 //   k_i8       one CTA per tile of 128 channels x up to 16 or 64 rows, for few
-//              rows per group: a stream of weights;
+//              rows of few or small groups;
 //   k_i8_pair  a CTA pair (cta_group::2) per tile of 256 channels x up to 512
-//              rows, for prompts.  A tile's operands come from L2: the pair
+//              rows, for prompts and for long streams of weights.  A tile's operands come from L2: the pair
 //              shares its row codes, and 512 rows a tile halve what the
 //              weights cost.  Main loop alone, 256 rows a tile 2.96 POPS, 512
 //              rows 3.57 (256 channels x 512 rows are all of the pair's TMEM).
 // Measured (device time of the product): 4096 rows, 2048 -> 4096, bf16: 26.9 us,
 // 2.55 POPS (tensor pipe busy half of the time); the rest is the start, 1.7 rounds
 // of tiles on 74 pairs and the last tile's conversion.  128 experts of
-// 2048 -> 2 x 768, SwiGLU, 512 rows: 67.5 us, 6.0 TB/s of weights.
+// 2048 -> 2 x 768, SwiGLU, 512 rows: 63.9 us, 6.3 TB/s of weights.
 // Persistent, one CTA per SM, units (group, row tile, channel tile) with the
 // channel tile fastest, so that concurrent CTAs share a row tile and, over the
 // following units, the group's weights in L2.  Every wait is bounded; a wait
@@ -1595,10 +1595,20 @@ namespace qg {
 
 static int64_t i8_pitch(int64_t I) { return (I + 15) & ~int64_t(15); }
 
-// Most rows of a tile.  Short tiles for few rows per group (the stages then
-// hold mostly weights), CTA pairs for prompts.
-static int i8_tile(int64_t rows_per_group) {
-    return rows_per_group <= 16 ? 16 : rows_per_group <= 64 ? 64 : I8P_NT;
+// Most rows of a tile, and with it the kernel: CTA pairs for more than 64 rows
+// per group and where the weights that R rows may touch are more than L2
+// holds, so that their stream and not its start decides; else k_i8, whose
+// smaller units spread over more SMs.  k_i8 and pairs, on the device: 128
+// experts of 2048 -> 2 x 768 (400 MB), 4 rows each 67.5 and 63.9 us, 32 rows 70.4
+// and 68.0; 60 of 1000 -> 2 x 640 (77 MB), 3 rows 12.7 and 14.5; 16 of 1024 ->
+// 2 x 512, 32 rows 6.2 and 7.4.  Of k_i8, 16 and 64 rows a tile, the latter with
+// 4 rows per group 5.8 and 6.3 us, with 16, which some groups exceed, 7.6
+// and 5.9; without groups R is what a tile holds.
+static int i8_tile(const qgq8 *h, int64_t R) {
+    const int64_t per = (R + h->G - 1) / h->G;  // mean rows of a group
+    const int64_t blocks = (int64_t)(R < h->G ? R : h->G) * h->RT * h->KB;  // of 16 KB
+    if (per > 64 || blocks >= 8192) return I8P_NT;
+    return per <= (h->G > 1 ? 8 : 16) ? 16 : 64;
 }
 
 template <typename TO, bool SWIGLU>
@@ -1700,8 +1710,7 @@ static int i8_align(const qgq8 *h, const void *y) {
 
 static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const float *scale, int R,
                       const int32_t *offsets, void *y, int ydt, cudaStream_t s) {
-    const int64_t per = (R + (int64_t)h->G - 1) / h->G;  // mean rows of a group
-    const int nt = i8_tile(per);
+    const int nt = i8_tile(h, R);
     CUtensorMap tx;
     int rc = i8_encode_map(&tx, codes, R, h->I, ld, nt < I8P_BOX ? nt : I8P_BOX);
     if (rc) return rc;
