@@ -307,7 +307,7 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
     TR *gx = grad_rows + (int64_t)r * H;
     float dot = 0.f;
     if constexpr (VEC) {
-        constexpr int U = 2;
+        constexpr int U = 4;
         for (int c0 = lane * 8; c0 < H; c0 += U * 256) {
             Vec8<TG> gv[U];
             Vec8<TR> xv[U];
