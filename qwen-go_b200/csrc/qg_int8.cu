@@ -1150,7 +1150,7 @@ k_i8_pair(const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ CU
 // while the weights are on their way; warps 0-3 are the epilogue after that:
 // the partial sums of lane quarter q go to the CTA q * split / 4 of the
 // cluster, which adds them (exactly, as integers) and writes y.
-// One token, 2048 -> 4096: 5.7 us, where the quantiser and k_i8 take 7.2 in two
+// One token, 2048 -> 4096: 5.8 us, where the quantiser and k_i8 take 7.2 in two
 // launches, the product on 32 of 148 SMs.  What is left is latency: launch,
 // cluster start, one read of x, one exchange.
 constexpr int I8F_ROWS = 16;
@@ -1750,9 +1750,9 @@ static int i8_few_split(const qgq8 *h, int R) {
 // Rows up to which a dense product runs on k_i8_few: its CTAs have to be
 // resident at once, each with its share of the row codes in shared memory, and
 // beyond 16 rows with all its weights in flight.  2048 -> 4096, this kernel and
-// the two others on the device: 1 row 5.8 and 7.2 us, 8 rows 7.2 and 7.3, 16
-// rows 8.6 and 7.3, 32 rows 10.3 and 7.4 (48, beyond the rule, 12.1 and 7.8);
-// 1000 -> 1500: 77 rows 7.3 and 7.1.  Where the device takes longer, one launch
+// the quantiser with k_i8 on the device: 1 row 5.8 and 7.2 us, 8 rows 6.7 and
+// 7.3, 16 rows 7.8 and 7.4, 32 rows 9.4 and 7.4 (48, beyond the rule, 12 and 8);
+// 1000 -> 1500, 77 rows: 7.1 and with CTA pairs 6.5.  Where the device takes longer, one launch
 // instead of two and no workspace still save 4 us of host time, which is what a
 // call of this size waits for.
 static int i8_few_rows(const qgq8 *h) {

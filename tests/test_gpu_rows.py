@@ -218,6 +218,34 @@ def test_combine_backward(T, k, E, H, rt, gt):
     assert not f64(grad_w)[~live].any()
 
 
+@pytest.mark.parametrize("H", [8, 264, 1000])
+def test_float32_rows_between_32_byte_boundaries(H):
+    """Rows are read and written 32 bytes at a time where they are aligned to
+    that; 16 bytes past it every result is the same, bit for bit."""
+    t = torch_()
+    T, k, E = 23, 3, 7
+
+    def shifted(v):
+        flat = t.empty(v.numel() + 4, dtype=v.dtype, device=v.device)
+        s = flat[4:].view(v.shape)
+        assert s.data_ptr() % 32 == 16
+        return s.copy_(v)
+
+    order = qgmoe.sort_tokens(t.from_numpy(routing(T, k, E, H, 0.2)).cuda(), E)
+    x, rows = rand((T, H), t.float32, 1), rand((T * k, H), t.float32, 2)
+    w, zero = t.softmax(rand((T, k), t.float32, 3), 1), t.zeros((T * k, H), device="cuda")
+    for to in (t.clone, shifted):
+        got = qgmoe.gather_rows(to(x), order, out=to(zero))
+        out = qgmoe.combine_rows(to(rows), w, order, out=to(x))
+        gx = qgmoe.gather_rows_backward(to(rows), order, out=to(x))
+        gr, gw = qgmoe.combine_rows_backward(to(x), to(rows), w, order, grad_rows=to(zero))
+        codes, scale = qgmoe.quantize_rows(to(x))
+        now = [v.clone() for v in (got, out, gx, gr, gw, codes, scale)]
+        if to is shifted:
+            assert all(t.equal(a, b) for a, b in zip(first, now))
+        first = now
+
+
 def test_gradients_against_differences():
     """The loss sum(c * out) is linear in rows and in weights, and the token
     gradient is linear in x: central differences of the 64-bit form agree
