@@ -238,6 +238,20 @@ def test_rows_of_y_at_odd_addresses(N, yt, swiglu):
             assert t.all(buf[:off] == 5.0) and t.all(buf[off + T * N:] == 5.0)
 
 
+@pytest.mark.parametrize("T", [65, 128, 129, 256, 257])
+@pytest.mark.parametrize("K", [64, 300, 1100, 2048])
+def test_dense_rows_around_a_tile(T, K):
+    """Sizes where loading changes, with fewer and more blocks than stages; the
+    quantiser runs just before, so that the weights are under way earlier."""
+    t = torch_()
+    q, ws = weights((4100, K), T)
+    lin = qgmoe.Int8Linear(q, ws)
+    x = rand((T, K), t.float32, K)
+    y = lin.forward_device(x)
+    check_rows(y, *plain_quantize(f64(x)), q, ws)
+    assert t.equal(lin.matmul_device(*qgmoe.quantize_rows(x)), y)
+
+
 # ---- products by expert -------------------------------------------------------------
 @pytest.mark.parametrize("T,k,E,K,N,bad", [
     (1, 1, 1, 64, 64, 0.0), (1, 8, 128, 256, 130, 0.0), (5, 2, 3, 100, 40, 0.3),
@@ -274,6 +288,50 @@ def test_experts(T, k, E, K, N, bad, swiglu):
         yd = t.full((T * k, N), 9.0, device="cuda", dtype=dt)
         lin.forward_device(x, yd, order=order)
         assert t.equal(yd, y.to(dt))
+
+
+MIXED = [600, 0, 1, 128, 129, 5, 256, 257, 512, 513, 31, 1200, 64, 0, 33, 100, 7, 320, 2, 90]
+
+
+@pytest.mark.parametrize("sizes,K,N", [
+    (MIXED, 64, 40), (MIXED, 300, 300), (MIXED, 512, 130),       # 1, 3 and 4 blocks of the sum
+    ([3, 2, 700, 1, 0, 2], 256, 64), ([128] * 7, 130, 257), ([0, 0, 129, 0], 128, 24),
+    ([1, 2, 0, 5] * 32, 64, 10000),                              # more units per CTA than its table
+    ([1, 0, 3, 2, 40] * 204 + [1] * 4, 400, 200)])               # as many groups as there may be
+@pytest.mark.parametrize("swiglu", [False, True])
+def test_groups_of_every_size(sizes, K, N, swiglu):
+    """Groups around the sizes where tiles, parts and loading change, large and
+    small ones mixed; what lies outside the groups keeps what it held."""
+    t = torch_()
+    G, lead, R = len(sizes), 2, sum(sizes) + 5
+    off = np.cumsum([lead] + sizes)
+    N = N // 2 if swiglu and N > 1000 else N
+    q, ws = weights((G, 2 * N if swiglu else N, K), G + K)
+    lin = qgmoe.Int8Linear(q, ws, swiglu=swiglu)
+    codes = t.randint(-127, 128, (R, (K + 15) // 16 * 16), dtype=t.int8, device="cuda",
+                      generator=t.Generator("cuda").manual_seed(K))[:, :K]
+    scale = t.linspace(0.5, 2.0, R, device="cuda") * 1e-3
+    offsets = t.from_numpy(off.astype(np.int32)).cuda()
+    y = t.full((R, N), 3.0, device="cuda")
+    lin.matmul_device(codes, scale, y=y, offsets=offsets)
+    lin.sync()
+    assert t.all(y[:lead] == 3.0) and t.all(y[off[-1]:] == 3.0)
+    c, sc = codes.cpu().numpy(), scale.cpu().numpy()
+    some = [g for g in range(G) if sizes[g]]
+    for g in some if len(some) < 40 else some[::max(1, len(some) // 24)]:
+        r = slice(off[g], off[g + 1])
+        check_rows(y, c[r], sc[r], q[g], ws[g], swiglu, r)
+    yb = t.full((R, N), 3.0, device="cuda", dtype=t.bfloat16)
+    lin.matmul_device(codes, scale, y=yb, offsets=offsets)
+    assert t.equal(yb, y.to(t.bfloat16))
+    # a group that is not one, among groups that are: skipped, flagged, nothing else moves
+    offsets[3] = R + 1
+    z = t.full((R, N), 3.0, device="cuda")
+    lin.matmul_device(codes, scale, y=z, offsets=offsets)
+    with pytest.raises(qgmoe.QgmoeError):
+        lin.sync()
+    assert t.all(z[off[2]:off[4]] == 3.0)
+    assert t.equal(z[:off[2]], y[:off[2]]) and t.equal(z[off[4]:], y[off[4]:])
 
 
 def test_swiglu_far_from_zero():
