@@ -1611,6 +1611,31 @@ static int i8_tile(const qgq8 *h, int64_t R) {
     return per <= (h->G > 1 ? 8 : 16) ? 16 : 64;
 }
 
+// Rows of a dense product's tiles on CTA pairs: of the heights that R divides
+// into, from I8P_NT down to a quarter of it, the one whose rounds over the
+// device's pairs are shortest.  A tile counts as its rows, 128 where it has
+// fewer (its weights take as long), and 40 for its start and end.  2048 -> 4096:
+// 1024 rows 14.4 us in tiles of 512 (32 of them), 10.2 in tiles of 256; 512 rows
+// 14.3 (512) and 7.7 (128); 3000 rows 25.1 (512: 96 tiles on 74 pairs) and 20.0
+// (352); 4096 rows 26.6 (512) and 25.5 (480); 256 rows of 4096 -> 4096 12.9 (256),
+// 8.9 (128) and 9.7 (64).  A few heights from the top are enough: with many
+// rounds the last one matters little.
+static int i8_height(const qgq8 *h, int64_t R) {
+    const int64_t pairs = num_sms(h->device) / 2, ct = h->RT / 2;
+    const int64_t t0 = (R + I8P_NT - 1) / I8P_NT;
+    int best = I8P_NT;
+    int64_t least = INT64_MAX;
+    for (int64_t t = t0; t <= 4 * t0 && t < t0 + 16; t++) {
+        const int64_t rows = ((R + t - 1) / t + 31) / 32 * 32;
+        const int64_t cost = (t * ct + pairs - 1) / pairs * ((rows > 128 ? rows : 128) + 40);
+        if (cost < least) {
+            least = cost;
+            best = (int)rows;
+        }
+    }
+    return best;
+}
+
 template <typename TO, bool SWIGLU>
 static int launch_i8_pair_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int64_t max_units,
                             cudaStream_t s) {
@@ -1725,13 +1750,13 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     a.cols = h->cols;
     const bool pair = nt == I8P_NT;
     a.CT = pair ? h->RT / 2 : h->live;
-    a.nt = nt;
+    a.nt = pair && !offsets ? i8_height(h, R) : nt;
     a.gran = pair ? 32 : 16;
     a.y = y;
     a.align = i8_align(h, y);
     a.err = h->err_dev;
     // row tiles: full ones, and at most one partial for each group that has rows
-    const int64_t tiles = R / nt + (R < h->G ? R : h->G);
+    const int64_t tiles = R / a.nt + (R < h->G ? R : h->G);
     const int64_t units = tiles * a.CT;
     return nt == 16   ? launch_i8<16>(h, tx, a, ydt, units, s)
            : nt == 64 ? launch_i8<64>(h, tx, a, ydt, units, s)
