@@ -1611,17 +1611,22 @@ static int i8_tile(const qgq8 *h, int64_t R) {
     return per <= (h->G > 1 ? 8 : 16) ? 16 : 64;
 }
 
-// Rows of a dense product's tiles on CTA pairs: of the heights that R divides
-// into, from I8P_NT down to a quarter of it, the one whose rounds over the
-// device's pairs are shortest.  A tile counts as its rows, 128 where it has
+// Rows of a tile on CTA pairs: of the heights that R rows (of each of `groups`)
+// divide into, from I8P_NT down to a quarter of it, the one whose rounds over
+// the device's pairs are shortest.  A tile counts as its rows, 128 where it has
 // fewer (its weights take as long), and 40 for its start and end.  2048 -> 4096:
 // 1024 rows 14.4 us in tiles of 512 (32 of them), 10.2 in tiles of 256; 512 rows
 // 14.3 (512) and 7.7 (128); 3000 rows 25.1 (512: 96 tiles on 74 pairs) and 20.0
 // (352); 4096 rows 26.6 (512) and 25.5 (480); 256 rows of 4096 -> 4096 12.9 (256),
 // 8.9 (128) and 9.7 (64).  A few heights from the top are enough: with many
-// rounds the last one matters little.
-static int i8_height(const qgq8 *h, int64_t R) {
-    const int64_t pairs = num_sms(h->device) / 2, ct = h->RT / 2;
+// rounds the last one matters little.  Groups count as of their mean size, where
+// one tile of each leaves the device room: 8 groups of 4096 -> 1024 and 256 rows
+// skewed 25.1 us and 16.9; 4 of 1024 -> 2 x 512, 256 rows, 9.8 and
+// 7.7.  With more groups the sizes, which the host does not know, decide the
+// rounds.
+static int i8_height(const qgq8 *h, int64_t R, int groups) {
+    const int64_t pairs = num_sms(h->device) / 2, ct = (int64_t)h->RT / 2 * groups;
+    if (groups > 1 && ct > pairs) return I8P_NT;
     const int64_t t0 = (R + I8P_NT - 1) / I8P_NT;
     int best = I8P_NT;
     int64_t least = INT64_MAX;
@@ -1750,7 +1755,7 @@ static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const floa
     a.cols = h->cols;
     const bool pair = nt == I8P_NT;
     a.CT = pair ? h->RT / 2 : h->live;
-    a.nt = pair && !offsets ? i8_height(h, R) : nt;
+    a.nt = pair ? i8_height(h, (R + (int64_t)h->G - 1) / h->G, h->G) : nt;
     a.gran = pair ? 32 : 16;
     a.y = y;
     a.align = i8_align(h, y);
