@@ -382,14 +382,14 @@ template <typename T> __device__ __forceinline__ void ld_shared_vec8(uint32_t ad
 
 template <typename TI, bool GATHER>
 __global__ void __launch_bounds__(QR_THREADS)
-k_quantize_rows(const TI *x, int T, int k, int K, int N, int wpr, const int32_t *pair_row,
+k_quantize_rows(const TI *x, int T, int k, int K, int N, int wlog, const int32_t *pair_row,
                 int8_t *codes, int64_t ld, float *scale) {
     extern __shared__ __align__(16) unsigned char qr_smem[];
     __shared__ uint32_t s_max[QR_WARPS];
     pdl_enter();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int part = warp % wpr, span = wpr * 256, in_cta = warp / wpr;
-    const int64_t t = (int64_t)blockIdx.x * (QR_WARPS / wpr) + in_cta;
+    const int wpr = 1 << wlog, part = warp & (wpr - 1), span = wpr * 256, in_cta = warp >> wlog;
+    const int64_t t = (int64_t)blockIdx.x * (QR_WARPS >> wlog) + in_cta;
     const bool on = t < T;
     const TI *src = x + t * K;
     const int c0 = (part * 32 + lane) * 8;
@@ -640,7 +640,7 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
     int wpr = 1;
     while (wpr < QR_WARPS && (int64_t)T * wpr < 8192 && K > wpr * 256) wpr *= 2;
     while (wpr < QR_WARPS && QR_WARPS / wpr * (int64_t)row_bytes > QR_ROW_BYTES) wpr *= 2;
-    const int rows = QR_WARPS / wpr;
+    const int rows = QR_WARPS / wpr, wlog = wpr == 1 ? 0 : wpr == 2 ? 1 : wpr == 4 ? 2 : 3;
     return with_dtype(dt, [&](auto *ip) {
         using TI = std::remove_pointer_t<decltype(ip)>;
         if (!vec || rows * (int64_t)row_bytes > QR_ROW_BYTES) {
@@ -654,7 +654,7 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
         auto kern = pair_row ? k_quantize_rows<TI, true> : k_quantize_rows<TI, false>;
         QG_CUDA(launch_pdl(kern, dim3((unsigned)((T + (int64_t)rows - 1) / rows)),
                            dim3(QR_THREADS), (size_t)(rows * row_bytes), s, 1,
-                           static_cast<const TI *>(x), T, k, K, N, wpr, pair_row, codes, ld,
+                           static_cast<const TI *>(x), T, k, K, N, wlog, pair_row, codes, ld,
                            scale));
         return (int)QGMOE_OK;
     });
