@@ -1638,7 +1638,7 @@ static int i8_height(const qgq8 *h, int64_t R, int groups) {
             best = (int)rows;
         }
     }
-    return best;
+    return best < 128 ? 128 : best;  // (a group may be larger than the mean)
 }
 
 template <typename TO, bool SWIGLU>

@@ -635,8 +635,8 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
     const int N = pair_row ? T * k : T;
     const int row_bytes = K * (dt == QGMOE_DT_F32 ? 4 : 2);
     // As many warps for a row as fill the device about once (8192 warps): 4096
-    // bf16 rows of 2048 take 8.8 us with one or two warps each and 14.3 with
-    // eight, 1024 rows 6.0, 5.4, 4.3 and 4.5 us with one, two, four and eight.
+    // bf16 rows of 2048 take 10.0 us with one warp each, 8.2 with two and 11.8 with
+    // eight, 1024 rows 4.9, 5.4, 4.4 and 4.1 us with one, two, four and eight.
     int wpr = 1;
     while (wpr < QR_WARPS && (int64_t)T * wpr < 8192 && K > wpr * 256) wpr *= 2;
     while (wpr < QR_WARPS && QR_WARPS / wpr * (int64_t)row_bytes > QR_ROW_BYTES) wpr *= 2;
