@@ -1189,8 +1189,10 @@ __device__ __forceinline__ void i8f_quantize(const I8FewArgs &f, int r0, int R, 
             in.load(p);
             in.get(v);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = c + i < f.K ? Elem<TI>::load(p + i) : 0.f;
+            const TI *x = static_cast<const TI *>(f.x);
+            Vec8<TI> in = load_any(p, x, x + (int64_t)f.a.R * f.K, false);
+            zero_from(in, f.K - c);
+            in.get(v);
         }
     };
     // a row by one warp, or by two, four or eight where rows are fewer

@@ -202,16 +202,29 @@ k_sort_tokens(const int32_t *ids, int N, int E, int32_t *offsets, int32_t *pair_
     if (C > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
+// How rows are read and written:
+//   ROW_VEC       16-byte aligned, whole runs of 8 elements;
+//   ROW_ANY       a thread has a run of 8 of the row that is written, between two
+//                 boundaries of 8 elements, and reads its inputs wherever they lie;
+//   ROW_ELEMENTS  one element a thread: short rows, of which most runs would be
+//                 parts.
+// 32768 bfloat16 rows of 2048, and of 2047 as ROW_ANY and ROW_ELEMENTS: gathered
+// 25.4, 42 and 59 us, combined 24.3, 47 and 115, the gradients of combine 46.8,
+// 88 and 120.  Rows of 333: 13.4 and 11.0, 10.9 and 17.1, 27.1 and 24.3; of 100:
+// 8.0 and 5.1, 7.1 and 7.2, 17.5 and 10.8.
+enum { ROW_VEC, ROW_ANY, ROW_ELEMENTS };
+constexpr int SHORT_GATHER = 384, SHORT_COMBINE = 128, SHORT_BACKWARD = 512;  // elements below
+
 // ---- gather -------------------------------------------------------------------
-template <typename TI, typename TO, bool VEC>
+template <typename TI, typename TO, int HOW>
 __global__ void k_gather_rows(const TI *x, int k, int H, int N, const int32_t *pair_row,
                               TO *rows) {
     pdl_enter();
     const int64_t t = blockIdx.x;
     const int i = blockIdx.y * blockDim.x + threadIdx.x;
-    const int c = VEC ? i * 8 : i;
-    if (c >= H) return;
-    if constexpr (VEC) {
+    const int c = i * 8;
+    if constexpr (HOW == ROW_VEC) {
+        if (c >= H) return;
         Vec8<TI> in;
         in.load(x + t * H + c);
         float v[8];
@@ -220,11 +233,24 @@ __global__ void k_gather_rows(const TI *x, int k, int H, int N, const int32_t *p
             const int r = ld_i32(pair_row + t * k + j);
             if ((unsigned)r < (unsigned)N) Vec8<TO>::put(rows + (int64_t)r * H + c, v);
         }
-    } else {
-        const float v = Elem<TI>::load(x + t * H + c);
+    } else if constexpr (HOW == ROW_ANY) {
+        const TI *src = x + t * H, *end = x + (int64_t)gridDim.x * H;
+        const bool inner = inner_row(src, H, x, end);
         for (int j = 0; j < k; j++) {
             const int r = ld_i32(pair_row + t * k + j);
-            if ((unsigned)r < (unsigned)N) Elem<TO>::store(rows + (int64_t)r * H + c, v);
+            TO *row = rows + (int64_t)r * H;
+            const int c0 = c - run_shift(row);
+            if ((unsigned)r >= (unsigned)N || c0 >= H) continue;
+            float v[8];
+            load_any(src + c0, x, end, inner).get(v);
+            put_run(row, c0, H, v);
+        }
+    } else {
+        if (i >= H) return;
+        const float v = Elem<TI>::load(x + t * H + i);
+        for (int j = 0; j < k; j++) {
+            const int r = ld_i32(pair_row + t * k + j);
+            if ((unsigned)r < (unsigned)N) Elem<TO>::store(rows + (int64_t)r * H + i, v);
         }
     }
 }
@@ -232,40 +258,15 @@ __global__ void k_gather_rows(const TI *x, int k, int H, int N, const int32_t *p
 // ---- combine --------------------------------------------------------------------
 // Four of the token's rows are in flight per thread.  w == null: weights of
 // one (the gradient of gather).
-template <typename TI, typename TO, bool VEC>
+template <typename TI, typename TO, int HOW>
 __global__ void k_combine_rows(const TI *rows, const float *w, int k, int H, int N,
                                const int32_t *pair_row, TO *out) {
     pdl_enter();
     const int64_t t = blockIdx.x;
     const int i = blockIdx.y * blockDim.x + threadIdx.x;
-    const int c = VEC ? i * 8 : i;
-    if (c >= H) return;
     constexpr int U = 4;
-    if constexpr (VEC) {
-        float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        for (int j0 = 0; j0 < k; j0 += U) {
-            int r[U];
-            float wj[U];
-            Vec8<TI> in[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                r[u] = j0 + u < k ? ld_i32(pair_row + t * k + j0 + u) : -1;
-                wj[u] = w && j0 + u < k ? ld_f32(w + t * k + j0 + u) : 1.f;
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if ((unsigned)r[u] < (unsigned)N) in[u].load(rows + (int64_t)r[u] * H + c);
-#pragma unroll
-            for (int u = 0; u < U; u++)
-                if ((unsigned)r[u] < (unsigned)N) {
-                    float v[8];
-                    in[u].get(v);
-#pragma unroll
-                    for (int q = 0; q < 8; q++) acc[q] = fmaf(wj[u], v[q], acc[q]);
-                }
-        }
-        Vec8<TO>::put(out + t * H + c, acc);
-    } else {
+    if constexpr (HOW == ROW_ELEMENTS) {
+        if (i >= H) return;
         float acc = 0.f;
         for (int j0 = 0; j0 < k; j0 += U) {
             float v[U], wj[U];
@@ -274,13 +275,49 @@ __global__ void k_combine_rows(const TI *rows, const float *w, int k, int H, int
                 const int r = j0 + u < k ? ld_i32(pair_row + t * k + j0 + u) : -1;
                 const bool on = (unsigned)r < (unsigned)N;
                 wj[u] = !on ? 0.f : w ? ld_f32(w + t * k + j0 + u) : 1.f;
-                v[u] = on ? Elem<TI>::load(rows + (int64_t)r * H + c) : 0.f;
+                v[u] = on ? Elem<TI>::load(rows + (int64_t)r * H + i) : 0.f;
             }
 #pragma unroll
             for (int u = 0; u < U; u++) acc = fmaf(wj[u], v[u], acc);
         }
-        Elem<TO>::store(out + t * H + c, acc);
+        Elem<TO>::store(out + t * H + i, acc);
+        return;
     }
+    const int c = HOW == ROW_VEC ? i * 8 : i * 8 - run_shift(out + t * H);
+    if (c >= H) return;
+    const TI *end = rows + (int64_t)N * H;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    for (int j0 = 0; j0 < k; j0 += U) {
+        int r[U];
+        float wj[U];
+        Vec8<TI> in[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            r[u] = j0 + u < k ? ld_i32(pair_row + t * k + j0 + u) : -1;
+            wj[u] = w && j0 + u < k ? ld_f32(w + t * k + j0 + u) : 1.f;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if ((unsigned)r[u] < (unsigned)N) {
+                const TI *row = rows + (int64_t)r[u] * H;
+                if constexpr (HOW == ROW_VEC)
+                    in[u].load(row + c);
+                else
+                    in[u] = load_any(row + c, rows, end, inner_row(row, H, rows, end));
+            }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if ((unsigned)r[u] < (unsigned)N) {
+                float v[8];
+                in[u].get(v);
+#pragma unroll
+                for (int q = 0; q < 8; q++) acc[q] = fmaf(wj[u], v[q], acc[q]);
+            }
+    }
+    if constexpr (HOW == ROW_VEC)
+        Vec8<TO>::put(out + t * H + c, acc);
+    else
+        put_run(out + t * H, c, H, acc);
 }
 
 // ---- combine, backward ------------------------------------------------------------
@@ -288,7 +325,7 @@ __global__ void k_combine_rows(const TI *rows, const float *w, int k, int H, int
 // gradient once, for the dot product (dw) and the scaled copy (drows).  The k
 // warps of a token share its gradient row through L1.
 constexpr int CB_WARPS = 8;
-template <typename TG, typename TR, bool VEC>
+template <typename TG, typename TR, int HOW>
 __global__ void __launch_bounds__(CB_WARPS * 32)
 k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int k, int H, int N,
                         const int32_t *pair_row, TR *grad_rows, float *grad_w) {
@@ -306,41 +343,58 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
     const TR *x = rows + (int64_t)r * H;
     TR *gx = grad_rows + (int64_t)r * H;
     float dot = 0.f;
-    if constexpr (VEC) {
-        constexpr int U = 4;
-        for (int c0 = lane * 8; c0 < H; c0 += U * 256) {
-            Vec8<TG> gv[U];
-            Vec8<TR> xv[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int c = c0 + u * 256;
-                gv[u].zero();
-                xv[u].zero();
-                if (c < H) {
-                    gv[u].load(g + c);
-                    if (grad_w) xv[u].load(x + c);
-                }
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int c = c0 + u * 256;
-                float a[8], b[8];
-                gv[u].get(a);
-                xv[u].get(b);
-#pragma unroll
-                for (int q = 0; q < 8; q++) dot = fmaf(a[q], b[q], dot);
-                if (grad_rows && c < H) {
-#pragma unroll
-                    for (int q = 0; q < 8; q++) a[q] *= wp;
-                    Vec8<TR>::put(gx + c, a);
-                }
-            }
-        }
-    } else {
+    if constexpr (HOW == ROW_ELEMENTS) {
         for (int c = lane; c < H; c += 32) {
             const float a = Elem<TG>::load(g + c);
             if (grad_w) dot = fmaf(a, Elem<TR>::load(x + c), dot);
             if (grad_rows) Elem<TR>::store(gx + c, a * wp);
+        }
+    }
+    constexpr bool VEC = HOW == ROW_VEC;
+    constexpr int U = VEC ? 4 : 2;
+    const int shift = VEC ? 0 : run_shift(grad_rows ? gx : const_cast<TR *>(x));
+    const TG *g_end = grad_out + (int64_t)(N / k) * H;
+    const TR *x_end = rows + (int64_t)N * H;
+    const bool g_inner = inner_row(g, H, grad_out, g_end);
+    const bool x_inner = inner_row(x, H, rows, x_end);
+    for (int c0 = HOW == ROW_ELEMENTS ? H : lane * 8 - shift; c0 < H; c0 += U * 256) {
+        Vec8<TG> gv[U];
+        Vec8<TR> xv[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = c0 + u * 256;
+            gv[u].zero();
+            xv[u].zero();
+            if (c < H) {
+                if constexpr (VEC) {
+                    gv[u].load(g + c);
+                    if (grad_w) xv[u].load(x + c);
+                } else {
+                    gv[u] = load_any(g + c, grad_out, g_end, g_inner);
+                    if (grad_w) xv[u] = load_any(x + c, rows, x_end, x_inner);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int c = c0 + u * 256;
+            float a[8], b[8];
+            gv[u].get(a);
+            xv[u].get(b);
+            if (!VEC && (c < 0 || c + 8 > H))  // what lies outside the row
+#pragma unroll
+                for (int q = 0; q < 8; q++)
+                    if (c + q < 0 || c + q >= H) a[q] = b[q] = 0.f;
+#pragma unroll
+            for (int q = 0; q < 8; q++) dot = fmaf(a[q], b[q], dot);
+            if (grad_rows && c < H) {
+#pragma unroll
+                for (int q = 0; q < 8; q++) a[q] *= wp;
+                if constexpr (VEC)
+                    Vec8<TR>::put(gx + c, a);
+                else
+                    put_run(gx, c, H, a);
+            }
         }
     }
     if (grad_w) {
@@ -360,7 +414,8 @@ k_combine_rows_backward(const TG *grad_out, const TR *rows, const float *w, int 
 // (How the codes are formed: qg_rows.cuh.)
 //
 // A row belongs to `wpr` warps of a CTA.  It is copied to shared memory
-// asynchronously and read there twice, each thread the vectors it copied
+// asynchronously (VEC; through registers where it is unaligned: 4096 bfloat16
+// rows of 2047 take 12.3 us, read element by element 16.2) and read there twice, each thread the vectors it copied
 // itself, which keeps the code small and the registers few: a row per warp and
 // seven CTAs' rows in flight on an SM.  Rows beyond QR_ROW_BYTES are read from
 // memory twice (k_quantize_long).
@@ -380,7 +435,22 @@ template <typename T> __device__ __forceinline__ void ld_shared_vec8(uint32_t ad
     }
 }
 
-template <typename TI, bool GATHER>
+template <typename T>
+__device__ __forceinline__ void st_shared_vec8(uint32_t addr, const Vec8<T> &v) {
+    auto put = [](uint32_t at, const uint4 &u) {
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(u.x), "r"(u.y),
+                     "r"(u.z), "r"(u.w)
+                     : "memory");
+    };
+    if constexpr (sizeof(T) == 4) {
+        put(addr, v.a);
+        put(addr + 16, v.b);
+    } else {
+        put(addr, v.r);
+    }
+}
+
+template <typename TI, bool GATHER, bool VEC>
 __global__ void __launch_bounds__(QR_THREADS)
 k_quantize_rows(const TI *x, int T, int k, int K, int N, int wlog, const int32_t *pair_row,
                 int8_t *codes, int64_t ld, float *scale) {
@@ -393,12 +463,21 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wlog, const int32_t
     const bool on = t < T;
     const TI *src = x + t * K;
     const int c0 = (part * 32 + lane) * 8;
-    const uint32_t row = sm100::smem_u32(qr_smem) + in_cta * K * (int)sizeof(TI);
-    if (on)
+    const uint32_t row = sm100::smem_u32(qr_smem) + in_cta * ((K + 7) & ~7) * (int)sizeof(TI);
+    if (on && VEC) {
         for (int c = c0; c < K; c += span) {
             cp_async16(row + c * sizeof(TI), src + c);
             if (sizeof(TI) == 4) cp_async16(row + c * sizeof(TI) + 16, src + c + 4);
         }
+    } else if (on) {
+        const bool inner = inner_row(src, K, x, x + (int64_t)T * K);
+#pragma unroll 4
+        for (int c = c0; c < K; c += span) {
+            Vec8<TI> in = load_any(src + c, x, x + (int64_t)T * K, inner);
+            zero_from(in, K - c);
+            st_shared_vec8(row + c * (int)sizeof(TI), in);
+        }
+    }
     // destination rows, lane j the j-th of this run of up to 32
     int dst = -1;
     if (GATHER && on && lane < k) dst = ld_i32(pair_row + t * k + lane);
@@ -479,8 +558,8 @@ k_quantize_rows(const TI *x, int T, int k, int K, int N, int wlog, const int32_t
     }
 }
 
-// One CTA per row, read twice: rows longer than the registers hold, and rows
-// that are not 16-byte aligned or no multiple of 8 (VEC false).
+// One CTA per row, read twice: rows beyond QR_ROW_BYTES; VEC false where they
+// are not 16-byte aligned or no multiple of 8.
 template <typename TI, bool VEC>
 __global__ void __launch_bounds__(QR_THREADS)
 k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_t *codes,
@@ -491,17 +570,20 @@ k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_
     const int tid = threadIdx.x, nt = blockDim.x;
     const TI *src = x + t * K;
     AbsMax<TI> top;
-    if constexpr (VEC) {
-#pragma unroll 4
-        for (int c = tid * 8; c < K; c += nt * 8) {
-            Vec8<TI> in;
+    const TI *end = x + (int64_t)gridDim.x * K;
+    const bool inner = inner_row(src, K, x, end);
+    auto load = [&](int c) {
+        Vec8<TI> in;
+        if constexpr (VEC) {
             in.load(src + c);
-            top.fold(in);
+        } else {
+            in = load_any(src + c, x, end, inner);
+            zero_from(in, K - c);
         }
-    } else {
+        return in;
+    };
 #pragma unroll 4
-        for (int c = tid; c < K; c += nt) top.fold1(Elem<TI>::load(src + c));
-    }
+    for (int c = tid * 8; c < K; c += nt * 8) top.fold(load(c));
     uint32_t m = __reduce_max_sync(~0u, top.bits());
     if ((tid & 31) == 0) s_max[tid >> 5] = m;
     __syncthreads();
@@ -517,14 +599,7 @@ k_quantize_long(const TI *x, int k, int K, int N, const int32_t *pair_row, int8_
     // ld is a multiple of 16, so a store of 8 that ends past K stays in the row
     for (int c = tid * 8; c < K; c += nt * 8) {
         float v[8];
-        if constexpr (VEC) {
-            Vec8<TI> in;
-            in.load(src + c);
-            in.get(v);
-        } else {
-#pragma unroll
-            for (int q = 0; q < 8; q++) v[q] = c + q < K ? Elem<TI>::load(src + c + q) : 0.f;
-        }
+        load(c).get(v);
         const uint2 u = bad ? make_uint2(0, 0) : codes_of(v, s, inv);
         for (int j = 0; j < n_dst; j++) {
             const int r = dst_row(j);
@@ -583,9 +658,21 @@ template <typename F> static int with_dtype(int dt, F f) {
     return f(static_cast<__nv_bfloat16 *>(nullptr));
 }
 
+// Unaligned rows of `shortest` elements on take ROW_ANY.
+static int row_how(bool vec, int H, int shortest) {
+    return vec ? ROW_VEC : H >= shortest ? ROW_ANY : ROW_ELEMENTS;
+}
+// f(HOW) as a constant.
+template <typename F> static int with_how(int how, F f) {
+    return how == ROW_VEC   ? f(std::integral_constant<int, ROW_VEC>())
+           : how == ROW_ANY ? f(std::integral_constant<int, ROW_ANY>())
+                            : f(std::integral_constant<int, ROW_ELEMENTS>());
+}
 // Threads of a CTA and CTAs along a row for one element group per thread.
-static void row_grid(int64_t T, int H, bool vec, dim3 *grid, int *threads) {
-    const int n = vec ? H / 8 : H;
+static void row_grid(int64_t T, int H, int how, dim3 *grid, int *threads) {
+    const int n = how == ROW_VEC   ? H / 8
+                  : how == ROW_ANY ? (H + 7) / 8 + 1  // runs of 8 that a row may touch
+                                   : H;
     int th = (n + 31) / 32 * 32;
     if (th > 256) th = 256;
     *threads = th;
@@ -613,18 +700,20 @@ static int check_rows(int32_t T, int32_t k, int32_t H, int dt_a, int dt_b, const
 
 static int launch_combine_rows(const void *rows, int rdt, const float *w, int T, int k, int H,
                                const int32_t *pair_row, void *out, int odt, cudaStream_t s) {
-    const bool vec = H % 8 == 0 && aligned16(rows) && aligned16(out);
+    const int how = row_how(H % 8 == 0 && aligned16(rows) && aligned16(out), H, SHORT_COMBINE);
     dim3 grid;
     int th;
-    row_grid(T, H, vec, &grid, &th);
+    row_grid(T, H, how, &grid, &th);
     return with_dtype(rdt, [&](auto *ip) {
         return with_dtype(odt, [&](auto *op) {
             using TI = std::remove_pointer_t<decltype(ip)>;
             using TO = std::remove_pointer_t<decltype(op)>;
-            auto kern = vec ? k_combine_rows<TI, TO, true> : k_combine_rows<TI, TO, false>;
-            QG_CUDA(launch_pdl(kern, grid, dim3(th), 0, s, 1, static_cast<const TI *>(rows), w, k,
-                               H, T * k, pair_row, static_cast<TO *>(out)));
-            return (int)QGMOE_OK;
+            return with_how(how, [&](auto h) {
+                QG_CUDA(launch_pdl(k_combine_rows<TI, TO, decltype(h)::value>, grid, dim3(th), 0, s,
+                                   1, static_cast<const TI *>(rows), w, k, H, T * k, pair_row,
+                                   static_cast<TO *>(out)));
+                return (int)QGMOE_OK;
+            });
         });
     });
 }
@@ -633,7 +722,7 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
                          int8_t *codes, int64_t ld, float *scale, cudaStream_t s) {
     const bool vec = K % 8 == 0 && aligned16(x);
     const int N = pair_row ? T * k : T;
-    const int row_bytes = K * (dt == QGMOE_DT_F32 ? 4 : 2);
+    const int row_bytes = ((K + 7) & ~7) * (dt == QGMOE_DT_F32 ? 4 : 2);
     // As many warps for a row as fill the device about once (8192 warps): 4096
     // bf16 rows of 2048 take 10.0 us with one warp each, 8.2 with two and 11.8 with
     // eight, 1024 rows 4.9, 5.4, 4.4 and 4.1 us with one, two, four and eight.
@@ -643,7 +732,7 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
     const int rows = QR_WARPS / wpr, wlog = wpr == 1 ? 0 : wpr == 2 ? 1 : wpr == 4 ? 2 : 3;
     return with_dtype(dt, [&](auto *ip) {
         using TI = std::remove_pointer_t<decltype(ip)>;
-        if (!vec || rows * (int64_t)row_bytes > QR_ROW_BYTES) {
+        if (rows * (int64_t)row_bytes > QR_ROW_BYTES) {
             auto kern = vec ? k_quantize_long<TI, true> : k_quantize_long<TI, false>;
             int th = ((K + 7) / 8 + 31) / 32 * 32;
             if (th > QR_THREADS) th = QR_THREADS;
@@ -651,7 +740,9 @@ int launch_quantize_rows(const void *x, int dt, int T, int k, int K, const int32
                                static_cast<const TI *>(x), k, K, N, pair_row, codes, ld, scale));
             return (int)QGMOE_OK;
         }
-        auto kern = pair_row ? k_quantize_rows<TI, true> : k_quantize_rows<TI, false>;
+        auto kern = vec ? (pair_row ? k_quantize_rows<TI, true, true> : k_quantize_rows<TI, false, true>)
+                        : (pair_row ? k_quantize_rows<TI, true, false>
+                                    : k_quantize_rows<TI, false, false>);
         QG_CUDA(launch_pdl(kern, dim3((unsigned)((T + (int64_t)rows - 1) / rows)),
                            dim3(QR_THREADS), (size_t)(rows * row_bytes), s, 1,
                            static_cast<const TI *>(x), T, k, K, N, wlog, pair_row, codes, ld,
@@ -721,19 +812,20 @@ int qgmoe_gather_rows(const void *x, int32_t x_dtype, int32_t T, int32_t k, int3
     if (!x || !pair_row || !rows)
         return set_error(QGMOE_ERR_INVALID_ARG, "gather_rows: null pointer argument");
     if ((rc = check_elements(x, x_dtype, rows, rows_dtype, "gather_rows"))) return rc;
-    const bool vec = H % 8 == 0 && aligned16(x) && aligned16(rows);
+    const int how = row_how(H % 8 == 0 && aligned16(x) && aligned16(rows), H, SHORT_GATHER);
     dim3 grid;
     int th;
-    row_grid(T, H, vec, &grid, &th);
+    row_grid(T, H, how, &grid, &th);
     return with_dtype(x_dtype, [&](auto *ip) {
         return with_dtype(rows_dtype, [&](auto *op) {
             using TI = std::remove_pointer_t<decltype(ip)>;
             using TO = std::remove_pointer_t<decltype(op)>;
-            auto kern = vec ? k_gather_rows<TI, TO, true> : k_gather_rows<TI, TO, false>;
-            QG_CUDA(launch_pdl(kern, grid, dim3(th), 0, static_cast<cudaStream_t>(stream), 1,
-                               static_cast<const TI *>(x), k, H, T * k, pair_row,
-                               static_cast<TO *>(rows)));
-            return (int)QGMOE_OK;
+            return with_how(how, [&](auto h) {
+                QG_CUDA(launch_pdl(k_gather_rows<TI, TO, decltype(h)::value>, grid, dim3(th), 0,
+                                   static_cast<cudaStream_t>(stream), 1, static_cast<const TI *>(x),
+                                   k, H, T * k, pair_row, static_cast<TO *>(rows)));
+                return (int)QGMOE_OK;
+            });
         });
     });
 }
@@ -777,20 +869,23 @@ int qgmoe_combine_rows_backward(const void *grad_out, int32_t out_dtype, const v
     if ((rc = check_elements(rows, rows_dtype, grad_rows, rows_dtype, "combine_rows_backward")) ||
         (rc = check_elements(grad_out, out_dtype, nullptr, out_dtype, "combine_rows_backward")))
         return rc;
-    const bool vec = H % 8 == 0 && aligned16(grad_out) && (!rows || aligned16(rows)) &&
-                     (!grad_rows || aligned16(grad_rows));
+    const int how = row_how(H % 8 == 0 && aligned16(grad_out) && (!rows || aligned16(rows)) &&
+                                (!grad_rows || aligned16(grad_rows)),
+                            H, SHORT_BACKWARD);
     const int N = T * k;
     return with_dtype(out_dtype, [&](auto *gp) {
         return with_dtype(rows_dtype, [&](auto *rp) {
             using TG = std::remove_pointer_t<decltype(gp)>;
             using TR = std::remove_pointer_t<decltype(rp)>;
-            auto kern = vec ? k_combine_rows_backward<TG, TR, true>
-                            : k_combine_rows_backward<TG, TR, false>;
-            QG_CUDA(launch_pdl(kern, dim3((unsigned)((N + CB_WARPS - 1) / CB_WARPS)),
-                               dim3(CB_WARPS * 32), 0, static_cast<cudaStream_t>(stream), 1,
-                               static_cast<const TG *>(grad_out), static_cast<const TR *>(rows), w,
-                               k, H, N, pair_row, static_cast<TR *>(grad_rows), grad_w));
-            return (int)QGMOE_OK;
+            return with_how(how, [&](auto h) {
+                QG_CUDA(launch_pdl(k_combine_rows_backward<TG, TR, decltype(h)::value>,
+                                   dim3((unsigned)((N + CB_WARPS - 1) / CB_WARPS)),
+                                   dim3(CB_WARPS * 32), 0, static_cast<cudaStream_t>(stream), 1,
+                                   static_cast<const TG *>(grad_out),
+                                   static_cast<const TR *>(rows), w, k, H, N, pair_row,
+                                   static_cast<TR *>(grad_rows), grad_w));
+                return (int)QGMOE_OK;
+            });
         });
     });
 }

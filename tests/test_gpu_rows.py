@@ -246,6 +246,59 @@ def test_float32_rows_between_32_byte_boundaries(H):
         first = now
 
 
+@pytest.mark.parametrize("H", [33, 127, 129, 255, 383, 385, 511, 513, 1000, 2047])
+@pytest.mark.parametrize("rt,ot", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f32"), ("f32", "bf16")])
+@pytest.mark.parametrize("off", [0, 1, 2, 3, 6])
+def test_rows_of_any_length_at_any_address(H, rt, ot, off):
+    """Bit for bit what aligned rows of whole runs of 8 give; nothing beside a
+    tensor is written."""
+    t = torch_()
+    T, k, E = 13, 3, 5
+    P = (H + 7) // 8 * 8
+    rd, od = dtypes()[rt], dtypes()[ot]
+    order = qgmoe.sort_tokens(t.from_numpy(routing(T, k, E, H, 0.2)).cuda(), E)
+
+    def padded(n, dt, seed):
+        v = t.zeros((n, P), dtype=dt, device="cuda")
+        v[:, :H] = rand((n, H), dt, seed)
+        return v
+
+    def odd(v):  # its first H columns, `off` elements past a boundary, guarded
+        flat = t.full((v.shape[0] * H + off + 64,), 9.0, dtype=v.dtype, device="cuda")
+        m = flat[off:off + v.shape[0] * H].view(v.shape[0], H)
+        m.copy_(v[:, :H])
+        return flat, m
+
+    def same(flat, m, want):
+        assert t.equal(m, want[:, :H])
+        assert t.all(flat[:off] == 9.0) and t.all(flat[off + m.numel():] == 9.0)
+
+    x, g, rows = padded(T, od, 1), padded(T, od, 2), padded(T * k, rd, 3)
+    w = t.softmax(rand((T, k), t.float32, 4), 1)
+    zeros_r, zeros_t = t.zeros_like(rows), t.zeros_like(x)
+    (_, xo), (_, go), (_, ro) = odd(x), odd(g), odd(rows)
+    flat, out = odd(zeros_r)
+    qgmoe.gather_rows(xo, order, out=out)
+    same(flat, out, qgmoe.gather_rows(x, order, out=zeros_r.clone()))
+    flat, out = odd(zeros_t)
+    qgmoe.combine_rows(ro, w, order, out=out)
+    same(flat, out, qgmoe.combine_rows(rows, w, order, dtype=od))
+    qgmoe.gather_rows_backward(ro, order, out=out)
+    same(flat, out, qgmoe.gather_rows_backward(rows, order, dtype=od))
+    flat, out = odd(zeros_r)
+    _, gw = qgmoe.combine_rows_backward(go, ro, w, order, grad_rows=out)
+    want, want_w = qgmoe.combine_rows_backward(g, rows, w, order, grad_rows=zeros_r.clone())
+    same(flat, out, want)
+    # both sum at most H products (one rounding each) in another order
+    pr = order.pair_row.cpu().numpy()
+    terms = np.abs(f64(rows))[np.maximum(pr, 0)] * np.abs(f64(g))[:, None, :]
+    assert np.all(np.abs(f64(gw) - f64(want_w)) <= 2.02 * H * U * terms.sum(2))
+    for v, vo in ((x, xo), (rows, ro)):
+        c, s = qgmoe.quantize_rows(vo)
+        cp, sp = qgmoe.quantize_rows(v)
+        assert t.equal(c, cp[:, :H]) and t.equal(s, sp)
+
+
 def test_gradients_against_differences():
     """The loss sum(c * out) is linear in rows and in weights, and the token
     gradient is linear in x: central differences of the 64-bit form agree
