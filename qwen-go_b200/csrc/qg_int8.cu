@@ -104,7 +104,7 @@ struct I8Args {
     int CT;                  // channel tiles per group: those with channels, or RT / 2 for pairs
     int nt, gran;            // most rows of a tile; tiles are multiples of gran rows
     void *y;                 // [R, cols]
-    int align;               // of y's 16-bit rows, in bytes: 16, 4 or 2
+    int align;               // of y's 16-bit rows, in bytes: 16, 4 (SwiGLU) or 2 (Single)
     int *err;
 };
 
@@ -449,9 +449,25 @@ __host__ __device__ __forceinline__ int i8_channel(int row, bool swiglu) {  // o
     const int m = row / 8, j = row % 8 / 2, b = row & 1;
     return (swiglu ? 4 : 8) * j + 2 * m + b;
 }
+// 16-bit rows whose runs of 8 are not aligned leave as float32 rows do, an
+// element a lane: 4096 x 2048 -> 4094 bfloat16 that way 29 us, as pairs of a
+// thread 37, one by one 100 (-> 4096: 25).  With SwiGLU pairs are faster, 47 and
+// 52, where there are pairs.
+template <typename T> struct Single {
+    T v;
+};
+__device__ __forceinline__ void put_one(float *p, float v) { *p = v; }
+__device__ __forceinline__ void put_one(Single<__half> *p, float v) { p->v = __float2half_rn(v); }
+__device__ __forceinline__ void put_one(Single<__nv_bfloat16> *p, float v) {
+    p->v = __float2bfloat16_rn(v);
+}
+template <typename T> constexpr bool i8_singles = true;
+template <> constexpr bool i8_singles<__half> = false;
+template <> constexpr bool i8_singles<__nv_bfloat16> = false;
+
 template <typename TO, bool SWIGLU, int SUBS>
 struct I8Epilogue {
-    static constexpr bool F32 = sizeof(TO) == 4;
+    static constexpr bool F32 = i8_singles<TO>;
     static constexpr bool LANES = F32 && !SWIGLU;  // a lane is a channel
     static constexpr int CH = SWIGLU ? 16 : 32;    // channels of this warp
     static constexpr int RUNS = SUBS == 4 ? 2 : 1;  // of an accumulator, per warp
@@ -523,7 +539,7 @@ struct I8Epilogue {
                 const float f[4] = {f0.x, f0.y, f1.x, f1.y};
 #pragma unroll
                 for (int b = 0; b < 4; b++) {
-                    if (WHOLE || (o < a.cols && c + b < nc)) *yp = f[b];
+                    if (WHOLE || (o < a.cols && c + b < nc)) put_one(yp, f[b]);
                     yp += pitch;
                 }
             }
@@ -553,8 +569,8 @@ struct I8Epilogue {
 #pragma unroll
                     for (int e = 0; e < 2; e++)
                         if (WHOLE || o + 2 * e < a.cols) {
-                            if (WHOLE || c < nc) yp[2 * e] = f[e].x;
-                            if (WHOLE || c + 1 < nc) yp[pitch + 2 * e] = f[e].y;
+                            if (WHOLE || c < nc) put_one(yp + 2 * e, f[e].x);
+                            if (WHOLE || c + 1 < nc) put_one(yp + pitch + 2 * e, f[e].y);
                         }
                 } else {
                     uint32_t p[N / 2];
@@ -562,24 +578,18 @@ struct I8Epilogue {
                     for (int e = 0; e < N / 2; e++)
                         p[e] = movmatrix(pack2(static_cast<TO *>(nullptr), f[e].x, f[e].y));
                     const bool real = WHOLE || i * 8 + ro < nc;
-                    if (WHOLE || a.align == 16) {  // cols % 8 == 0: all N channels or none
+                    if (!SWIGLU || WHOLE || a.align == 16) {  // all N channels or none
                         if (WHOLE || (real && o < a.cols)) {
                             if constexpr (SWIGLU)
                                 *reinterpret_cast<uint2 *>(yp) = make_uint2(p[0], p[1]);
                             else
                                 *reinterpret_cast<uint4 *>(yp) = make_uint4(p[0], p[1], p[2], p[3]);
                         }
-                    } else if (a.align >= 4) {  // an even number of columns: pairs
+                    } else {  // pairs
 #pragma unroll
                         for (int e = 0; e < N / 2; e++)
                             if (real && o + 2 * e < a.cols)
                                 reinterpret_cast<uint32_t *>(yp)[e] = p[e];
-                    } else if (real) {
-#pragma unroll
-                        for (int e = 0; e < N; e++)
-                            if (o + e < a.cols)
-                                reinterpret_cast<uint16_t *>(yp)[e] =
-                                    (uint16_t)(p[e >> 1] >> (16 * (e & 1)));
                     }
                 }
                 yp += 8 * pitch;
@@ -1703,16 +1713,23 @@ static int launch_i8_t(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, in
         return launch_i8_cta_t<NT, TO, SWIGLU>(h, tx, a, max_units, s);
 }
 
+// f with a null pointer of the type that y's rows are written as.
+template <typename F> static int with_y(int ydt, int align, F f) {
+    if (ydt == QGMOE_DT_F32) return f(static_cast<float *>(nullptr));
+    if (ydt == QGMOE_DT_F16)
+        return align == 2 ? f(static_cast<Single<__half> *>(nullptr)) : f(static_cast<__half *>(nullptr));
+    return align == 2 ? f(static_cast<Single<__nv_bfloat16> *>(nullptr))
+                      : f(static_cast<__nv_bfloat16 *>(nullptr));
+}
+
 template <int NT>
 static int launch_i8(const qgq8 *h, const CUtensorMap &tx, const I8Args &a, int ydt, int64_t units,
                      cudaStream_t s) {
-    if (h->swiglu)
-        return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, true>(h, tx, a, units, s)
-               : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, true>(h, tx, a, units, s)
-                                     : launch_i8_t<NT, __nv_bfloat16, true>(h, tx, a, units, s);
-    return ydt == QGMOE_DT_F32   ? launch_i8_t<NT, float, false>(h, tx, a, units, s)
-           : ydt == QGMOE_DT_F16 ? launch_i8_t<NT, __half, false>(h, tx, a, units, s)
-                                 : launch_i8_t<NT, __nv_bfloat16, false>(h, tx, a, units, s);
+    return with_y(ydt, a.align, [&](auto *yp) {
+        using TO = std::remove_pointer_t<decltype(yp)>;
+        return h->swiglu ? launch_i8_t<NT, TO, true>(h, tx, a, units, s)
+                         : launch_i8_t<NT, TO, false>(h, tx, a, units, s);
+    });
 }
 
 static int i8_check_product(const qgq8 *h, const int8_t *codes, int64_t ld, const float *scale,
@@ -1737,7 +1754,8 @@ static int i8_check_product(const qgq8 *h, const int8_t *codes, int64_t ld, cons
 
 static int i8_align(const qgq8 *h, const void *y) {
     const uintptr_t p = reinterpret_cast<uintptr_t>(y);
-    return h->cols % 8 == 0 && p % 16 == 0 ? 16 : h->cols % 2 == 0 && p % 4 == 0 ? 4 : 2;
+    if (h->cols % 8 == 0 && p % 16 == 0) return 16;
+    return h->swiglu && h->cols % 2 == 0 && p % 4 == 0 ? 4 : 2;  // (see Single)
 }
 
 static int i8_product(const qgq8 *h, const int8_t *codes, int64_t ld, const float *scale, int R,
@@ -1843,13 +1861,10 @@ static int i8_few(const qgq8 *h, const void *x, int xdt, int R, void *y, int ydt
     f.K = h->I;
     f.split = i8_few_split(h, R);
     f.blocks = (h->KB + f.split - 1) / f.split;
-    if (h->swiglu)
-        return ydt == QGMOE_DT_F32   ? launch_i8_few_t<float, true>(h, f, s)
-               : ydt == QGMOE_DT_F16 ? launch_i8_few_t<__half, true>(h, f, s)
-                                     : launch_i8_few_t<__nv_bfloat16, true>(h, f, s);
-    return ydt == QGMOE_DT_F32   ? launch_i8_few_t<float, false>(h, f, s)
-           : ydt == QGMOE_DT_F16 ? launch_i8_few_t<__half, false>(h, f, s)
-                                 : launch_i8_few_t<__nv_bfloat16, false>(h, f, s);
+    return with_y(ydt, f.a.align, [&](auto *yp) {
+        using TO = std::remove_pointer_t<decltype(yp)>;
+        return h->swiglu ? launch_i8_few_t<TO, true>(h, f, s) : launch_i8_few_t<TO, false>(h, f, s);
+    });
 }
 
 static void i8_free_work(qgq8 *h) {
