@@ -25,10 +25,10 @@
 //              shares its row codes, and 512 rows a tile halve what the
 //              weights cost.  Main loop alone, 256 rows a tile 2.96 POPS, 512
 //              rows 3.57 (256 channels x 512 rows are all of the pair's TMEM).
-// Measured (device time of the product): 4096 rows, 2048 -> 4096, bf16: 26.9 us,
-// 2.55 POPS (tensor pipe busy half of the time); the rest is the start, 1.7 rounds
-// of tiles on 74 pairs and the last tile's conversion.  128 experts of
-// 2048 -> 2 x 768, SwiGLU, 512 rows: 63.9 us, 6.3 TB/s of weights.
+// Measured (device time of the product): 4096 rows, 2048 -> 4096, bf16: 25.9 us,
+// 2.65 POPS (tensor pipe busy half of the time); the rest is the start, 1.95
+// rounds of tiles on 74 pairs and the last tile's conversion.  128 experts of
+// 2048 -> 2 x 768, SwiGLU, 512 rows: 64.4 us, 6.3 TB/s of weights.
 // Persistent, one CTA per SM, units (group, row tile, channel tile) with the
 // channel tile fastest, so that concurrent CTAs share a row tile and, over the
 // following units, the group's weights in L2.  Every wait is bounded; a wait
