@@ -62,6 +62,18 @@ def test_quantize_rows(T, K, dt):
     assert codes.shape == (T, K) and codes.stride(0) % 16 == 0
 
 
+@pytest.mark.parametrize("K", [8185, 8191, 16383, 20001])
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("off", [0, 1, 4])
+def test_quantize_long_rows_of_odd_lengths(K, dt, off):
+    """Around the length from which a row is no longer kept in shared memory."""
+    x = rand((3 * K + off,), dtypes()[dt], K)[off:].view(3, K)
+    codes, scale = qgmoe.quantize_rows(x)
+    c, s = plain_quantize(f64(x))
+    np.testing.assert_array_equal(scale.cpu().numpy(), s)
+    np.testing.assert_array_equal(codes.cpu().numpy(), c)
+
+
 def test_quantize_rows_at_the_edges():
     """Ties away from zero, zero rows, rows under the scale's floor, the
     largest values, and rows with an infinity or NaN, whose products are NaN."""
